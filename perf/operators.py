@@ -212,9 +212,8 @@ def _run_own(s):
         return loss.detach(), lp.detach(), grad
     m, ref = s["mask"], s["ref"]
     lp = s["lp"] if op == "preference" else rl.compute_token_logprobs(s["logits"], s["tokens"], m)
-    loss, good, bad = rl.compute_preference_loss(
-        lp[:n], lp[n:], ref[:n], ref[n:], None if m is None else m[:n], None if m is None else m[n:], beta=0.1,
-        loss=c["loss"], label_smoothing=c["smoothing"], length_normalized=c["normalized"])
+    loss, good, bad = rl.compute_preference_loss(lp, ref, m, beta=0.1, loss=c["loss"],
+                                                 label_smoothing=c["smoothing"], length_normalized=c["normalized"])
     (grad,) = torch.autograd.grad(loss, s["lp"] if op == "preference" else s["logits"])
     return loss.detach(), good, bad, grad
 
