@@ -282,6 +282,143 @@ int rls_segment_summary(int alg, const void* flag0, const void* flag1, const voi
 int rls_segment_compose(const float* summaries, int rank, int world, int backward, int64_t num_envs,
                         float* carry, void* stream);
 
+/* ---- token-level policy operators (no counterpart in the reference) -------
+ * What comes before and after the estimators in the update of a policy over
+ * tokens (or any discrete actions): the log-probabilities of the tokens taken,
+ * and the losses that use them, each with its gradient.
+ *
+ * Logits are [num_envs, seq_len, vocab] in in_dtype with element strides
+ * (env_stride, step_stride, 1): rows may overlap nothing but need not be
+ * contiguous nor 16-byte aligned (element alignment is enough).  tokens is
+ * int64 [num_envs, seq_len].  `mask` (may be NULL: every step counts) is
+ * [num_envs, seq_len] in the type mask_kind names; a step counts where it is
+ * not zero.  A step that does not count has log-probability, entropy and
+ * gradient 0, and its logits, token and other inputs are not used.  A token
+ * outside [0, vocab) at a step that counts gives NaN there (and in the loss).
+ * Logits may be -inf.  All other floating arrays are fp32, contiguous.       */
+#define RLS_MASK_NONE 0
+#define RLS_MASK_U8   1   /* bool or any 8-bit integer */
+#define RLS_MASK_F32  2
+#define RLS_MASK_BF16 3
+#define RLS_MASK_I32  4
+#define RLS_MASK_I64  5
+
+/* With z = logits / temperature:  logprobs = z[token] - logsumexp(z),
+ * entropy = -sum p log p (NULL: not computed).  row_stats (fp32 [N, T,
+ * RLS_ROW_STATS], may be NULL) keeps each row's maximum and sums for the backward
+ * call; rows of at most RLS_SHORT_VOCAB logits need none.                      */
+#define RLS_ROW_STATS   8
+#define RLS_SHORT_VOCAB 1024
+int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
+                       const void* mask, int mask_kind, float* logprobs, float* entropy, float* row_stats,
+                       int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature, int in_dtype,
+                       void* stream);
+
+/* grad_logits[n, t, v] = (grad_logprobs (1[v = token] - p_v)
+ *                         - grad_entropy p_v (log p_v + entropy)) / temperature,
+ * in in_dtype with its own strides.  grad_logprobs or grad_entropy may be NULL
+ * (zero); row_stats as the forward call with an entropy output wrote it where
+ * grad_entropy is given.                                                      */
+int rls_token_logprobs_backward(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
+                                const void* mask, int mask_kind, const float* row_stats,
+                                const float* grad_logprobs, const float* grad_entropy, void* grad_logits,
+                                int64_t grad_env_stride, int64_t grad_step_stride, int64_t num_envs,
+                                int64_t seq_len, int64_t vocab, float temperature, int in_dtype, void* stream);
+
+/* The clipped policy loss.  With r = exp(logprob - old_logprob):
+ *   term = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A),
+ *          at most -dual_clip A where A < 0 (dual_clip > 0; 0: off),
+ *          + kl_coef KL(logprob, ref_logprob) - entropy_coef entropy,
+ * KL estimated per token: K1 = lp - ref, K2 = (lp - ref)^2 / 2,
+ * K3 = exp(ref - lp) - (ref - lp) - 1; and over the steps that count
+ *   RLS_REDUCE_TOKEN     loss = sum(term) / (number of them),
+ *   RLS_REDUCE_SEQUENCE  loss = mean over the envs that have any of the mean
+ *                        of the env's terms,
+ *   RLS_REDUCE_SUM       loss = sum(term).
+ * No step counts: loss 0, gradients 0.                                        */
+#define RLS_KL_K1 1
+#define RLS_KL_K2 2
+#define RLS_KL_K3 3
+#define RLS_REDUCE_TOKEN    0
+#define RLS_REDUCE_SEQUENCE 1
+#define RLS_REDUCE_SUM      2
+typedef struct rls_policy {
+    float clip_low, clip_high, dual_clip;
+    float kl_coef, entropy_coef;
+    int   kl_kind, reduction;
+} rls_policy_t;
+
+/* From log-probabilities.  advantages: [num_envs, seq_len], or [num_envs] with
+ * advantages_per_env.  ref_logprobs may be NULL (kl_coef is then unused).
+ * norm (fp32 [num_envs + 1]) is written: what the weights of the steps come
+ * from; needed where a mask is given and the reduction is not SUM, else NULL.
+ * loss: fp32 scalar.  stats: fp32[5] (may be NULL) = over the steps that count the
+ * mean KL to ref, mean r - 1 - log r, share held by the clip, mean entropy (0
+ * here), and their number.  grad_logprobs (may
+ * be NULL) receives grad_scale * d loss / d logprobs.  Deterministic.          */
+int rls_policy_loss(const float* logprobs, const float* old_logprobs, const float* advantages,
+                    int advantages_per_env, const float* ref_logprobs, const void* mask, int mask_kind,
+                    const rls_policy_t* policy, float grad_scale, float* norm, float* loss, float* stats,
+                    float* grad_logprobs, int64_t num_envs, int64_t seq_len, void* ws, size_t ws_bytes, void* stream);
+
+/* The gradient for another incoming gradient *grad_loss (device fp32): nothing
+ * is done when it equals grad_scale (grad_logprobs holds that already), unless
+ * `force`; otherwise grad_logprobs is written anew.  norm as rls_policy_loss
+ * wrote it.                                                                   */
+int rls_policy_loss_backward(const float* logprobs, const float* old_logprobs, const float* advantages,
+                             int advantages_per_env, const float* ref_logprobs, const void* mask, int mask_kind,
+                             const rls_policy_t* policy, float grad_scale, const float* grad_loss, int force,
+                             const float* norm, float* grad_logprobs, int64_t num_envs, int64_t seq_len,
+                             void* stream);
+
+/* From the logits, in one pass over them: each row's log-probability is taken
+ * and its gradient written while the row is at hand.  logprobs and row_stats
+ * (as rls_token_logprobs) are written; entropy is (and has to be given) where entropy_coef != 0, else
+ * may be NULL.  grad_logits (NULL: no gradient) = grad_scale * d loss / d logits
+ * in in_dtype.  loss and stats as rls_policy_loss (with the mean entropy where it
+ * is given). */
+int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
+                           const float* old_logprobs, const float* advantages, int advantages_per_env,
+                           const float* ref_logprobs, const void* mask, int mask_kind, const rls_policy_t* policy,
+                           float grad_scale, float* norm, float* logprobs, float* entropy, float* row_stats,
+                           float* loss, float* stats, void* grad_logits, int64_t grad_env_stride,
+                           int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature, int in_dtype,
+                           void* ws, size_t ws_bytes, void* stream);
+int rls_policy_loss_logits_backward(const void* logits, int64_t env_stride, int64_t step_stride,
+                                    const int64_t* tokens, const float* old_logprobs, const float* advantages,
+                                    int advantages_per_env, const float* ref_logprobs, const void* mask,
+                                    int mask_kind, const rls_policy_t* policy, float grad_scale,
+                                    const float* grad_loss, int force, const float* norm,
+                                    const float* row_stats, void* grad_logits, int64_t grad_env_stride,
+                                    int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab,
+                                    float temperature, int in_dtype, void* stream);
+
+/* The paired preference loss over the log-probabilities of `pairs` responses
+ * preferred (chosen [pairs, chosen_len]) and not (rejected [pairs,
+ * rejected_len]).  Per response: s = sum over the steps that count of
+ * (lp - ref) (over their number with length_normalized; 0 where none counts);
+ * ref may be NULL (0), per step [pairs, len], or per response [pairs]
+ * (ref_per_pair: s = sum lp - ref).  With x = beta (s_chosen - s_rejected):
+ *   RLS_PREFERENCE_SIGMOID  -(1 - smoothing) log sig(x) - smoothing log sig(-x),
+ *   RLS_PREFERENCE_IPO      (x / beta - 1 / (2 beta))^2,
+ *   RLS_PREFERENCE_HINGE    max(0, 1 - x),
+ * loss = the mean over the pairs (0 of none).  rewards (fp32 [2, pairs]) = beta s of the
+ * chosen, then of the rejected.  coef (fp32 [2, pairs], may be NULL) keeps
+ * d loss / d logprob of a step that counts, for the backward call, which writes
+ * *grad_loss times it at those steps and 0 elsewhere.  Deterministic.          */
+#define RLS_PREFERENCE_SIGMOID 0
+#define RLS_PREFERENCE_IPO     1
+#define RLS_PREFERENCE_HINGE   2
+int rls_preference_loss(const float* chosen, const float* rejected, const float* ref_chosen,
+                        const float* ref_rejected, int ref_per_pair, const void* chosen_mask,
+                        const void* rejected_mask, int mask_kind, int64_t pairs, int64_t chosen_len,
+                        int64_t rejected_len, float beta, float smoothing, int kind, int length_normalized,
+                        float* loss, float* rewards, float* coef, void* ws, size_t ws_bytes, void* stream);
+int rls_preference_loss_backward(const float* coef, const float* grad_loss, const void* chosen_mask,
+                                 const void* rejected_mask, int mask_kind, float* grad_chosen,
+                                 float* grad_rejected, int64_t pairs, int64_t chosen_len, int64_t rejected_len,
+                                 void* stream);
+
 /* ---- GAE for callers that cannot allocate --------------------------------
  * No counterpart in the reference (its Triton path always allocates through
  * PyTorch).  Same arguments and results as rls_gae, minus the workspace: the

@@ -20,8 +20,10 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "rl_triton", "_lib")
 LIB = os.path.join(LIBDIR, "librlscan.so")
 TORCH_LIB = os.path.join(LIBDIR, "librlscan_torch.so")
-SOURCES = ["rlscan.cu", "segment.cu", "ppo.cu"]
-HEADERS = ["common.cuh", "algs.cuh", "scan_kernel.cuh", "rows_kernel.cuh", "rows2_kernel.cuh", "tile_kernel.cuh", "tile_policies.cuh", "host_shared.h"]
+SOURCES = ["rlscan.cu", "segment.cu", "ppo.cu", "token_loss.cu", "token_lanes.cu", "token_rows.cu", "preference.cu"]
+TORCH_SOURCES = ["torch_ops.cpp", "torch_token_ops.cpp"]
+HEADERS = ["common.cuh", "algs.cuh", "scan_kernel.cuh", "rows_kernel.cuh", "rows2_kernel.cuh", "tile_kernel.cuh", "tile_policies.cuh", "host_shared.h",
+           "token_kernels.cuh", "token_launch.h"]
 
 
 def nvcc_path() -> str:
@@ -69,18 +71,26 @@ def torch_flags() -> list[str]:
 
 
 def build_torch_ops(force: bool = False) -> str:
-    """librlscan_torch.so: the rl_triton::* PyTorch operators (torch_ops.cpp),
+    """librlscan_torch.so: the rl_triton::* PyTorch operators (csrc/torch_*.cpp),
     linked against librlscan.so."""
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    if (not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) > os.path.getmtime(src)
-            and os.path.getmtime(TORCH_LIB) > os.path.getmtime(LIB)):
+    srcs = [os.path.join(CSRC, f) for f in TORCH_SOURCES]
+    deps = srcs + [os.path.join(CSRC, "torch_shared.h"), LIB]
+    if (not force and os.path.exists(TORCH_LIB)
+            and all(os.path.getmtime(TORCH_LIB) > os.path.getmtime(d) for d in deps)):
         return TORCH_LIB
     cflags, ldflags = torch_flags()
+    os.makedirs(OBJDIR, exist_ok=True)
+    objs = [os.path.join(OBJDIR, f.replace(".cpp", ".o")) for f in TORCH_SOURCES]
+    procs = [subprocess.Popen(["g++", "-O2", "-std=c++17", "-fPIC", *cflags, "-c", src, "-o", obj],
+                              stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+             for src, obj in zip(srcs, objs)]
+    logs = [(p.communicate()[0], p.returncode) for p in procs]
     tmp = TORCH_LIB + ".tmp"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *cflags, src, "-o", tmp, *ldflags]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
+    if all(rc == 0 for _, rc in logs):
+        res = subprocess.run(["g++", "-shared", *objs, "-o", tmp, *ldflags], capture_output=True, text=True)
+        logs.append((res.stdout + res.stderr, res.returncode))
+    if any(rc != 0 for _, rc in logs):
+        sys.stderr.write("".join(out for out, rc in logs if rc != 0))
         raise RuntimeError("g++ failed building librlscan_torch.so")
     os.replace(tmp, TORCH_LIB)
     return TORCH_LIB

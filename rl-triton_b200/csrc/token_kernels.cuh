@@ -1,0 +1,746 @@
+// token_kernels.cuh -- log-probabilities of tokens from a policy's logits, and
+// the gradients that flow back into the logits.
+//
+// A row is one step's logits x[0..V).  With z = x / temperature,
+//   lse = log sum_v exp z_v,  p_v = exp(z_v - lse),
+//   logprob = z_tok - lse,    entropy H = lse - sum_v p_v z_v,
+//   d logprob / d x_v = (1[v = tok] - p_v) / temperature,
+//   d H / d x_v       = -p_v (log p_v + H) / temperature.
+// Everything is computed in base 2: with c = log2(e) / temperature and an
+// offset M (the running maximum times c, rounded),
+//   d_v = x_v c - M,  S0 = sum 2^d_v,  S1 = sum 2^d_v d_v,  t = S1 / S0,
+//   logprob = ln2 (d_tok - log2 S0),   H = ln2 (log2 S0 - t),
+// one fused multiply-add and one ex2 an element, and the gradient for incoming
+// (a, b) of (logprob, H) is
+//   a 1[v = tok] / temperature - 2^d_v (A + B d_v),
+//   A = (a - b ln2 t) / (S0 temperature),  B = b ln2 / (S0 temperature).
+// The sums and the row's statistics are fp32 (each thread's partial sum covers
+// at most V / threads elements); the logprob itself is formed in fp64 from
+// them, so that it is rounded once.
+#pragma once
+#include <math.h>
+
+#include "common.cuh"
+#include "rlscan.h"
+
+namespace rls {
+namespace tok {
+
+constexpr float kLn2 = 0.693147180559945309f;
+// Where a row's maximum is so large that M = m c is rounded by whole units
+// (logits at the type's lowest value in a whole row, infinities), x c - M is
+// useless and S0 leaves [kLeast, kMost]; such rows, and rows with NaN, are
+// summed again with d = (x - m) c, the far form.
+constexpr float kFar = 1e30f;
+constexpr float kLeast = 0.25f, kMost = 1e15f;
+constexpr float kDeep = -16384.f;  // 2^kDeep is 0: keeps 2^d * d finite at d = -inf
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- mask ------------------------------------------------------------------
+// One element a step, any of the types below; non-zero counts (NaN too).
+struct Mask {
+  const void* p;
+  int kind;  // RLS_MASK_*
+};
+
+__device__ __forceinline__ bool mask_at(const Mask& m, int64_t i) {
+  switch (m.kind) {
+    case RLS_MASK_U8: return reinterpret_cast<const uint8_t*>(m.p)[i] != 0;
+    case RLS_MASK_F32: return reinterpret_cast<const float*>(m.p)[i] != 0.f;
+    case RLS_MASK_BF16: return bf16_bits_to_float(reinterpret_cast<const unsigned short*>(m.p)[i]) != 0.f;
+    case RLS_MASK_I32: return reinterpret_cast<const int32_t*>(m.p)[i] != 0;
+    case RLS_MASK_I64: return reinterpret_cast<const int64_t*>(m.p)[i] != 0;
+    default: return true;
+  }
+}
+
+// ---- rows ------------------------------------------------------------------
+template <class T>
+struct Rows {
+  const T* x;          // logits
+  int64_t es, ss;      // strides of env and step in elements
+  int64_t rows, seq;   // rows = envs * seq
+  int64_t V;
+  const int64_t* tokens;
+  Mask mask;
+  float c;             // log2(e) / temperature
+  float inv_temp;
+  bool flat;           // es == seq * ss
+
+  __device__ __forceinline__ int64_t at(int64_t row) const {
+    if (flat) return row * ss;
+    const int64_t env = row / seq;
+    return env * es + (row - env * seq) * ss;
+  }
+};
+
+template <class T>
+struct GradRows {
+  T* g;
+  int64_t es, ss;
+  bool flat;
+  __device__ __forceinline__ int64_t at(int64_t row, int64_t seq) const {
+    if (flat) return row * ss;
+    const int64_t env = row / seq;
+    return env * es + (row - env * seq) * ss;
+  }
+};
+
+// What a row's reduction leaves: m the maximum that d is taken from, S0, t,
+// and whether d has the far form.  alone: one element holds all of S0 and S1 (all others
+// are exactly 0), so the entropy is 0 and not the rounding of its parts.
+struct RowStats {
+  float m, s0, t;
+  bool far, alone;
+};
+
+// A long row's record (RLS_ROW_STATS floats, two 16-byte words): m, S0, t and
+// flags; and, written by the policy loss, the derivative a of the loss by the
+// row's log-probability, the weighted term, the KL estimate and the drift.
+constexpr int kFlagClipped = 1, kFlagFar = 2, kFlagKept = 4;
+__device__ __forceinline__ float4 stats_word(const RowStats& r, int flags) {
+  return make_float4(r.m, r.s0, r.t, __int_as_float(flags | (r.far ? kFlagFar : 0)));
+}
+__device__ __forceinline__ RowStats stats_of(const float4& q) {
+  return RowStats{q.x, q.y, q.z, (__float_as_int(q.w) & kFlagFar) != 0, false};
+}
+
+// d of one element under the row's statistics.
+struct Shift {
+  float c, off;  // d = x c - off, or (x - off) c in the far form
+  bool far;
+  __device__ __forceinline__ float operator()(float x) const { return far ? (x - off) * c : fmaf(x, c, -off); }
+};
+__device__ __forceinline__ Shift shift_of(const RowStats& r, float c) {
+  return Shift{c, r.far ? r.m : r.m * c, r.far};
+}
+
+__device__ __forceinline__ double log2_of(float s0) {
+  int e;
+  const float f = frexpf(s0, &e);
+  return (double)e + (double)log2f(f);
+}
+
+// fp64, so that what follows from it (the ratio of the policy loss) does not
+// carry the rounding of the fp32 output.
+__device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c) {
+  const Shift sh = shift_of(r, c);
+  if (ex2(sh(x_tok)) == r.s0) return 0.0;  // the others are below fp32's reach
+  const double d = sh.far ? ((double)x_tok - (double)sh.off) * (double)c
+                          : (double)x_tok * (double)c - (double)sh.off;
+  return (d - log2_of(r.s0)) * 0.693147180559945309417;
+}
+__device__ __forceinline__ float entropy_of(const RowStats& r) {
+  if (r.alone) return 0.f;
+  return (float)((log2_of(r.s0) - (double)r.t) * 0.693147180559945309417);
+}
+
+// The gradient's coefficients for incoming (a, b) of (logprob, entropy).
+struct RowGrad {
+  float a;     // added at the token
+  float A, B;  // 2^d (A + B d) is subtracted everywhere
+};
+__device__ __forceinline__ RowGrad row_grad(float a, float b, const RowStats& r, float inv_temp) {
+  const float k = inv_temp / r.s0, bl = b * kLn2;
+  return RowGrad{a * inv_temp, (a - bl * r.t) * k, bl * k};
+}
+template <bool ENT>
+__device__ __forceinline__ float grad_at(float x, const Shift& sh, const RowGrad& g) {
+  const float d = sh(x);
+  const float e = ex2(d);
+  if constexpr (ENT) return -e * fmaf(g.B, fmaxf(d, kDeep), g.A);
+  else return -e * g.A;
+}
+
+// ---- 16-byte vectors ---------------------------------------------------------
+template <class T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static constexpr unsigned kLowest = 0xff800000u;  // -inf
+  __device__ __forceinline__ static void unpack(const uint4& u, float (&f)[4]) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+  __device__ __forceinline__ static uint4 pack(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  __device__ __forceinline__ static float get(const float* p) { return *p; }
+  __device__ __forceinline__ static float put(float v) { return v; }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static constexpr unsigned kLowest = 0xff80ff80u;
+  __device__ __forceinline__ static void unpack(const uint4& u, float (&f)[8]) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[2 * k] = __uint_as_float(w[k] << 16);
+      f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+  }
+  // The gradient leaves in the logits' type: one rounding, to nearest even.
+  __device__ __forceinline__ static uint4 pack(const float (&f)[8]) {
+    unsigned w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+      w[k] = *reinterpret_cast<const unsigned*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ static float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  __device__ __forceinline__ static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+};
+
+// A row cut at 16-byte boundaries: `head` elements, `nvec` vectors, `tail`.
+struct Cut {
+  int64_t head, nvec, tail;
+};
+template <class T>
+__device__ __forceinline__ Cut cut_row(const T* p, int64_t V) {
+  constexpr int N = Vec<T>::N;
+  int64_t head = (int64_t)((16 - ((uintptr_t)p & 15)) & 15) / (int64_t)sizeof(T);
+  if (head > V) head = V;
+  const int64_t nvec = (V - head) / N;
+  return Cut{head, nvec, V - head - nvec * N};
+}
+
+// ---- running statistics --------------------------------------------------------
+// (m, s0, s1) of the elements seen: s0 = sum 2^d, s1 = sum 2^d d with d taken
+// from off = m c.  m starts at -kFar, not -inf, so that no difference of two
+// offsets is NaN; elements below it count as 0 (rows that have nothing above it
+// take the far form).
+template <bool ENT>
+struct Run {
+  float m = -kFar, off, s0 = 0.f, s1 = 0.f;
+  __device__ __forceinline__ explicit Run(float c) : off(-kFar * c) {}
+  // Moves to a larger maximum.
+  __device__ __forceinline__ void raise(float mx, float c) {
+    const float to = mx * c, by = off - to;
+    const float k = ex2(by);
+    if constexpr (ENT) s1 = fmaf(s0, fmaxf(by, kDeep), s1) * k;
+    s0 *= k;
+    m = mx;
+    off = to;
+  }
+  __device__ __forceinline__ void add(float x, float c) {
+    const float d = fmaf(x, c, -off);
+    const float e = ex2(d);
+    s0 += e;
+    if constexpr (ENT) s1 = fmaf(e, fmaxf(d, kDeep), s1);
+  }
+  template <int K>
+  __device__ __forceinline__ void add(const float (&x)[K], float c) {
+    float mx = x[0];
+#pragma unroll
+    for (int k = 1; k < K; ++k) mx = fmaxf(mx, x[k]);
+    if (mx > m) raise(mx, c);
+#pragma unroll
+    for (int k = 0; k < K; ++k) add(x[k], c);
+  }
+  __device__ __forceinline__ void join(float om, float ooff, float os0, float os1) {
+    const bool up = om > m;
+    const float to = up ? ooff : off;
+    const float d0 = off - to, d1 = ooff - to;
+    const float k0 = ex2(d0), k1 = ex2(d1);
+    if constexpr (ENT) s1 = fmaf(s0, fmaxf(d0, kDeep), s1) * k0 + fmaf(os0, fmaxf(d1, kDeep), os1) * k1;
+    s0 = s0 * k0 + os0 * k1;
+    if (up) m = om;
+    off = to;
+  }
+};
+
+template <bool ENT>
+__device__ __forceinline__ void warp_join(Run<ENT>& r, int width = 32) {
+  for (int o = width / 2; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, r.m, o);
+    const float oo = __shfl_xor_sync(0xffffffffu, r.off, o);
+    const float a = __shfl_xor_sync(0xffffffffu, r.s0, o);
+    const float b = ENT ? __shfl_xor_sync(0xffffffffu, r.s1, o) : 0.f;
+    r.join(om, oo, a, b);
+  }
+}
+
+// ---- the policy loss -------------------------------------------------------------
+struct Policy {
+  const float* old_lp;
+  const float* adv;
+  bool adv_row;          // adv holds one value a row of the batch
+  const float* ref;      // may be null
+  float lo, hi;          // ratio bounds
+  double log_lo, log_hi, log_dual;  // their logarithms: -inf, +inf where there is none
+  float dual;
+  float kl_coef;
+  int kl_kind;
+  float ent_coef;
+  // weight of a step's term: w; or norm[0], over norm[1 + env] for the mean by sequence
+  int reduction;
+  const float* norm;     // null: w alone
+  float w;
+};
+
+__device__ __forceinline__ float policy_weight(const Policy& p, int64_t env) {
+  if (!p.norm) return p.w;
+  const float n0 = p.norm[0];
+  return p.reduction == RLS_REDUCE_SEQUENCE ? n0 / p.norm[1 + env] : n0;
+}
+
+struct PolicyTerm {
+  float loss, d;         // the step's term and its derivative by the logprob
+  float kl, drift;
+  bool clipped;
+};
+
+// -min(r A, clip(r) A), at most -dual A where A < 0, plus the KL estimate:
+// k1 = lp - ref, k2 = (lp - ref)^2 / 2, k3 = exp(ref - lp) - (ref - lp) - 1.
+// Whether the clip holds is decided on log r in fp64 (exact for fp32 inputs):
+// the derivative jumps there, and exp's rounding would put steps near a bound
+// on either side of it.
+__device__ __forceinline__ PolicyTerm policy_term(const Policy& p, double lp, float old_lp, float adv, float ref) {
+  PolicyTerm o;
+  const double lr64 = lp - (double)old_lp;
+  const float lr = (float)lr64;
+  const float gain = expf(lr) * adv;
+  o.loss = -gain;
+  o.d = -gain;
+  o.clipped = false;
+  if (adv > 0.f) {
+    if (lr64 > p.log_hi) { o.loss = -p.hi * adv; o.clipped = true; }
+  } else if (adv < 0.f) {
+    if (lr64 < p.log_lo) { o.loss = -p.lo * adv; o.clipped = true; }
+    else if (lr64 > p.log_dual) { o.loss = -p.dual * adv; o.clipped = true; }
+  }
+  if (o.clipped) o.d = 0.f;
+  o.drift = expm1f(lr) - lr;
+  o.kl = 0.f;
+  if (p.ref) {
+    const float x = (float)((double)ref - lp);
+    float dk;
+    if (p.kl_kind == RLS_KL_K1) { o.kl = -x; dk = 1.f; }
+    else if (p.kl_kind == RLS_KL_K2) { o.kl = 0.5f * x * x; dk = -x; }
+    else { const float e = expm1f(x); o.kl = e - x; dk = -e; }
+    if (p.kl_coef != 0.f) {
+      o.loss = fmaf(p.kl_coef, o.kl, o.loss);
+      o.d = fmaf(p.kl_coef, dk, o.d);
+    }
+  }
+  return o;
+}
+
+// ---- sums over steps ---------------------------------------------------------------
+// loss, KL, drift, clipped, entropy, steps: fp64 per thread, then per CTA, then
+// the CTAs' in their order, so that the result does not depend on timing.
+constexpr int kSums = 6;
+struct SumOut {
+  double* partials;   // [CTAs][kSums]
+  unsigned* ticket;   // CTAs done; the last one resets it
+  float* loss;
+  float* stats;       // may be null
+};
+
+// Adds the CTA's sums to the call's; every thread of every CTA calls it once.
+// NT >= 32 kSums.
+template <int NT>
+__device__ __forceinline__ void finish_sums(double (&sum)[kSums], const SumOut& o) {
+  static_assert(NT >= 32 * kSums, "a warp for each sum");
+  __shared__ double part[NT / 32][kSums];
+  __shared__ bool last;
+#pragma unroll
+  for (int k = 0; k < kSums; ++k)
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], d);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) part[warp][k] = sum[k];
+  __syncthreads();
+  if (threadIdx.x < kSums) {
+    double s = 0;
+    for (int w = 0; w < NT / 32; ++w) s += part[w][threadIdx.x];
+    o.partials[(int64_t)blockIdx.x * kSums + threadIdx.x] = s;
+    __threadfence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(o.ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  // warp k adds sum k: lanes in strides over the CTAs, then the lanes
+  double s = 0;
+  if (warp < kSums)
+    for (int64_t b = lane; b < gridDim.x; b += 32) s += __ldcg(&o.partials[b * kSums + warp]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (warp < kSums && lane == 0) part[0][warp] = s;
+  __syncthreads();
+  if (threadIdx.x < kSums) {
+    const double n = part[0][5], v = part[0][threadIdx.x];
+    if (threadIdx.x == 0) *o.loss = (float)v;
+    else if (o.stats) o.stats[threadIdx.x - 1] = (float)(threadIdx.x == 5 ? v : n > 0 ? v / n : 0.0);
+  }
+  if (threadIdx.x == 0) *o.ticket = 0u;
+}
+
+// ---- where a row's incoming gradients come from --------------------------------
+// Given per step.
+struct GivenGrad {
+  static constexpr bool kPolicy = false;
+  const float* g_lp;
+  const float* g_ent;  // may be null
+};
+
+// Those of the policy loss, for an incoming gradient of `scale` of the loss
+// itself, or *g where g is set.
+struct PolicyGrad {
+  static constexpr bool kPolicy = true;
+  Policy p;
+  float scale;
+  const float* g;
+  bool force;
+  SumOut sums;
+  // the gradient at hand was made for that very scale
+  __device__ __forceinline__ bool skip() const { return g && !force && *g == scale; }
+  __device__ __forceinline__ float up() const { return g ? *g : scale; }
+};
+
+enum Mode { kFwd, kBwd, kBoth };
+
+// ---- any row: one CTA a row ------------------------------------------------------
+template <bool ENT, int NT>
+__device__ __forceinline__ void block_join(Run<ENT>& r, float c) {
+  __shared__ float4 part[NT / 32];
+  warp_join<ENT>(r);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();  // the last row's parts are read
+  if (lane == 0) part[warp] = make_float4(r.m, r.off, r.s0, r.s1);
+  __syncthreads();
+  constexpr int W = NT / 32;
+  const float4 q = part[lane < W ? lane : 0];
+  Run<ENT> z(c);
+  z.m = q.x; z.off = q.y;
+  z.s0 = lane < W ? q.z : 0.f;
+  z.s1 = lane < W ? q.w : 0.f;
+  warp_join<ENT>(z);
+  // The lanes join in different orders, so their last bits may differ; every
+  // thread goes on with lane 0's (the same in each warp): branches on it hold
+  // barriers.
+  r.m = __shfl_sync(0xffffffffu, z.m, 0);
+  r.off = __shfl_sync(0xffffffffu, z.off, 0);
+  r.s0 = __shfl_sync(0xffffffffu, z.s0, 0);
+  if constexpr (ENT) r.s1 = __shfl_sync(0xffffffffu, z.s1, 0);
+}
+
+template <int NT>
+__device__ __forceinline__ float block_max(float v) {
+  __shared__ float part[NT / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[0];
+  for (int w = 1; w < NT / 32; ++w) v = fmaxf(v, part[w]);
+  return v;
+}
+template <int NT>
+__device__ __forceinline__ float block_sum(float v) {
+  __shared__ float part[NT / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[0];
+  for (int w = 1; w < NT / 32; ++w) v += part[w];
+  return v;
+}
+
+// The far form: two plain passes, the true maximum first.
+template <class T, bool ENT, int NT>
+__device__ __noinline__ RowStats far_stats(const T* x, int64_t V, float c) {
+  float m = -INFINITY;
+  for (int64_t v = threadIdx.x; v < V; v += NT) m = fmaxf(m, Vec<T>::get(x + v));
+  m = block_max<NT>(m);
+  float s0 = 0.f, s1 = 0.f;
+  for (int64_t v = threadIdx.x; v < V; v += NT) {
+    const float d = (Vec<T>::get(x + v) - m) * c;
+    const float e = ex2(d);
+    s0 += e;
+    if constexpr (ENT) s1 = fmaf(e, fmaxf(d, kDeep), s1);
+  }
+  s0 = block_sum<NT>(s0);
+  if constexpr (ENT) s1 = block_sum<NT>(s1);
+  return RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f};
+}
+
+template <class T, bool ENT, int NT, int U>
+__device__ __forceinline__ RowStats row_stats(const T* x, int64_t V, float c) {
+  constexpr int N = Vec<T>::N;
+  const Cut cut = cut_row(x, V);
+  Run<ENT> run(c);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + cut.head);
+  const unsigned low = Vec<T>::kLowest;
+  for (int64_t v0 = threadIdx.x; v0 < cut.nvec; v0 += (int64_t)NT * U) {
+    uint4 u[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t v = v0 + (int64_t)k * NT;
+      u[k] = v < cut.nvec ? __ldg(xv + v) : make_uint4(low, low, low, low);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      float f[N];
+      Vec<T>::unpack(u[k], f);
+      run.add(f, c);
+    }
+  }
+  const int64_t ends = cut.head + cut.tail;
+  if (threadIdx.x < ends) {
+    const int64_t i = threadIdx.x < cut.head ? threadIdx.x : V - ends + threadIdx.x;
+    const float f[1] = {Vec<T>::get(x + i)};
+    run.add(f, c);
+  }
+  block_join<ENT, NT>(run, c);
+  if (!(run.s0 >= kLeast && run.s0 <= kMost)) return far_stats<T, ENT, NT>(x, V, c);
+  const float d = fmaf(run.m, c, -run.off), e = ex2(d);
+  return RowStats{run.m, run.s0, ENT ? run.s1 / run.s0 : 0.f, false, ENT && run.s0 == e && run.s1 == e * d};
+}
+
+template <class T, int NT>
+__device__ __forceinline__ void zero_row(T* g, int64_t V) {
+  const Cut cut = cut_row(g, V);
+  uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
+  for (int64_t v = threadIdx.x; v < cut.nvec; v += NT) __stcs(gv + v, make_uint4(0, 0, 0, 0));
+  const int64_t ends = cut.head + cut.tail;
+  if (threadIdx.x < ends) g[threadIdx.x < cut.head ? threadIdx.x : V - ends + threadIdx.x] = Vec<T>::put(0.f);
+}
+
+template <class T, bool ENT, int NT, int U>
+__device__ __forceinline__ void grad_row(const T* x, T* g, int64_t V, int64_t tok, const Shift& sh, const RowGrad& rg) {
+  constexpr int N = Vec<T>::N;
+  const Cut cut = cut_row(x, V);
+  const bool same = (((uintptr_t)x ^ (uintptr_t)g) & 15) == 0;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + cut.head);
+  for (int64_t v0 = threadIdx.x; v0 < cut.nvec; v0 += (int64_t)NT * U) {
+    uint4 u[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t v = v0 + (int64_t)k * NT;
+      if (v < cut.nvec) u[k] = __ldcs(xv + v);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t v = v0 + (int64_t)k * NT;
+      if (v >= cut.nvec) break;
+      float f[N];
+      Vec<T>::unpack(u[k], f);
+      const int64_t i0 = cut.head + v * N;
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = grad_at<ENT>(f[e], sh, rg);
+      if (tok >= i0 && tok < i0 + N) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (tok == i0 + e) f[e] += rg.a;
+      }
+      if (same) {
+        __stcs(reinterpret_cast<uint4*>(g + i0), Vec<T>::pack(f));
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) g[i0 + e] = Vec<T>::put(f[e]);
+      }
+    }
+  }
+  const int64_t ends = cut.head + cut.tail;
+  if (threadIdx.x < ends) {
+    const int64_t i = threadIdx.x < cut.head ? threadIdx.x : V - ends + threadIdx.x;
+    float f = grad_at<ENT>(Vec<T>::get(x + i), sh, rg);
+    if (i == tok) f += rg.a;
+    g[i] = Vec<T>::put(f);
+  }
+}
+
+// Outputs per row; entropy and stats may be null.
+struct RowOut {
+  float* logprob;
+  float* entropy;
+  float4* stats;  // long rows' records
+};
+
+template <class T, bool ENT, int MODE, class Src, int NT, int U>
+__global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src) {
+  if constexpr (Src::kPolicy && MODE == kBwd) {
+    if (src.skip()) return;
+  }
+  for (int64_t row = blockIdx.x; row < in.rows; row += gridDim.x) {
+    const T* x = in.x + in.at(row);
+    T* g = MODE == kFwd || !gr.g ? nullptr : gr.g + gr.at(row, in.seq);
+    if (!mask_at(in.mask, row)) {
+      if constexpr (MODE != kBwd) {
+        if (threadIdx.x == 0) {
+          out.logprob[row] = 0.f;
+          if (out.entropy) out.entropy[row] = 0.f;
+          if (out.stats) out.stats[2 * row] = out.stats[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      if (g) zero_row<T, NT>(g, in.V);
+      continue;
+    }
+    const int64_t tok = in.tokens[row];
+    const bool ok = tok >= 0 && tok < in.V;
+    RowStats r;
+    float a = 0.f, b = 0.f;
+    if constexpr (MODE != kBwd) {
+      const float xt = ok ? Vec<T>::get(x + tok) : NAN;
+      r = row_stats<T, ENT, NT, U>(x, in.V, in.c);
+      const double lp = logprob_of(xt, r, in.c);
+      float ent = 0.f;
+      if constexpr (ENT) ent = entropy_of(r);
+      int flags = kFlagKept;
+      if constexpr (Src::kPolicy) {
+        const int64_t env = row / in.seq;
+        const Policy& p = src.p;
+        const PolicyTerm o = policy_term(p, lp, p.old_lp[row], p.adv[p.adv_row ? env : row], p.ref ? p.ref[row] : 0.f);
+        const float w = policy_weight(p, env);
+        a = w * o.d;
+        if constexpr (ENT) b = -w * p.ent_coef;
+        if (o.clipped) flags |= kFlagClipped;
+        if (threadIdx.x == 0) {
+          const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
+          out.stats[2 * row + 1] = make_float4(a, w * term, o.kl, o.drift);
+        }
+      }
+      if (threadIdx.x == 0) {
+        out.logprob[row] = (float)lp;
+        if (out.entropy) out.entropy[row] = ent;
+        if (out.stats) out.stats[2 * row] = stats_word(r, flags);
+      }
+    } else {
+      r = stats_of(out.stats[2 * row]);
+      if constexpr (Src::kPolicy) {
+        a = out.stats[2 * row + 1].x;
+        if constexpr (ENT) b = -policy_weight(src.p, row / in.seq) * src.p.ent_coef;
+      } else {
+        a = src.g_lp ? src.g_lp[row] : 0.f;
+        if constexpr (ENT) b = src.g_ent[row];
+      }
+    }
+    if (g) {
+      if constexpr (Src::kPolicy) { a *= src.up(); b *= src.up(); }
+      if (!ok) a = NAN;
+      if (a == 0.f && b == 0.f) zero_row<T, NT>(g, in.V);
+      else grad_row<T, ENT, NT, U>(x, g, in.V, tok, shift_of(r, in.c), row_grad(a, b, r, in.inv_temp));
+    }
+  }
+}
+
+// ---- short rows: G lanes a row, E elements a lane, the row in registers ------------
+// Each CTA takes tiles of 256 / G rows in strides of the grid; with the policy
+// loss it adds up its own rows' terms on the way.
+template <class T, bool ENT, int MODE, class Src, int G, int E>
+__global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src) {
+  if constexpr (Src::kPolicy && MODE == kBwd) {
+    if (src.skip()) return;
+  }
+  constexpr bool kTerms = Src::kPolicy && MODE != kBwd;
+  constexpr int kPer = 256 / G;
+  const int lane = threadIdx.x & (G - 1);
+  const int V = (int)in.V;
+  double sum[kTerms ? kSums : 1] = {};
+  const int64_t tiles = (in.rows + kPer - 1) / kPer;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t row_raw = tile * kPer + threadIdx.x / G;
+    const bool live = row_raw < in.rows;
+    const int64_t row = live ? row_raw : in.rows - 1;  // idle lanes shuffle along on the last row
+    const T* x = in.x + in.at(row);
+    T* g = MODE == kFwd || !gr.g ? nullptr : gr.g + gr.at(row, in.seq);
+    const bool kept = mask_at(in.mask, row);
+    const int64_t tok = kept ? in.tokens[row] : 0;
+    const bool ok = tok >= 0 && tok < V;
+    float f[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int i = lane + k * G;
+      f[k] = i < V && kept ? Vec<T>::get(x + i) : -INFINITY;
+    }
+    const float xt = kept && ok ? Vec<T>::get(x + tok) : NAN;
+    float m = f[0];
+#pragma unroll
+    for (int k = 1; k < E; ++k) m = fmaxf(m, f[k]);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const Shift sh{in.c, m, true};
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const float d = lane + k * G < V ? sh(f[k]) : -INFINITY;
+      const float e = ex2(d);
+      s0 += e;
+      if constexpr (ENT) s1 = fmaf(e, fmaxf(d, kDeep), s1);
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) {
+      s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+      if constexpr (ENT) s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+    }
+    const RowStats r{m, s0, ENT ? s1 / s0 : 0.f, true, ENT && s0 == 1.f && s1 == 0.f};
+    double lp = 0.0;
+    float ent = 0.f;
+    if (Src::kPolicy || MODE != kBwd) lp = logprob_of(xt, r, in.c);
+    if constexpr (ENT) ent = entropy_of(r);
+    if (!kept) { lp = 0.0; ent = 0.f; }
+    float a = 0.f, b = 0.f;
+    if (kept) {
+      if constexpr (Src::kPolicy) {
+        const int64_t env = row / in.seq;
+        const Policy& p = src.p;
+        const PolicyTerm o = policy_term(p, lp, p.old_lp[row], p.adv[p.adv_row ? env : row], p.ref ? p.ref[row] : 0.f);
+        const float w = policy_weight(p, env);
+        a = w * o.d;
+        if constexpr (ENT) b = -w * p.ent_coef;
+        if constexpr (kTerms) {
+          if (live && lane == 0) {
+            const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
+            sum[0] += (double)w * (double)term;
+            sum[1] += o.kl; sum[2] += o.drift; sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent; sum[5] += 1.0;
+          }
+        }
+        a *= src.up();
+        b *= src.up();
+      } else {
+        a = src.g_lp ? src.g_lp[row] : 0.f;
+        if constexpr (ENT && MODE == kBwd) b = src.g_ent[row];
+      }
+      if (!ok) a = NAN;
+    }
+    if constexpr (MODE != kBwd) {
+      if (live && lane == 0) {
+        out.logprob[row] = (float)lp;
+        if (out.entropy) out.entropy[row] = ent;
+      }
+    }
+    if (g && live) {
+      const bool none = a == 0.f && b == 0.f;
+      const RowGrad rg = row_grad(a, b, r, in.inv_temp);
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const int i = lane + k * G;
+        if (i < V) {
+          float o = grad_at<ENT>(f[k], sh, rg);
+          if (i == tok) o += rg.a;
+          g[i] = Vec<T>::put(none ? 0.f : o);
+        }
+      }
+    }
+  }
+  if constexpr (kTerms) finish_sums<256>(sum, src.sums);
+}
+
+}  // namespace tok
+}  // namespace rls

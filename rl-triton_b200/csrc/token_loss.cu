@@ -1,0 +1,468 @@
+// token_loss.cu -- C ABI of the token-level policy operators: log-probabilities
+// from logits with their gradient, and the clipped policy loss from
+// log-probabilities or from the logits (rlscan.h has the formulas).
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "host_shared.h"
+#include "token_launch.h"
+
+using namespace rls;
+using namespace rls::tok;
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// The ticket and the counts lie in words of the workspace header that the
+// estimators do not use; every launch leaves them zero.
+unsigned* ticket_of(void* ws) { return &static_cast<WsHeader*>(ws)->pad[4]; }
+unsigned long long* total_of(void* ws) { return reinterpret_cast<unsigned long long*>(&static_cast<WsHeader*>(ws)->pad[6]); }
+unsigned* rows_of(void* ws) { return &static_cast<WsHeader*>(ws)->pad[8]; }
+static_assert(offsetof(WsHeader, pad) % 8 == 0, "the total is 8-byte aligned");
+
+int num_sms() {
+  static int sms[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!sms[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
+// ---- what the steps' weights come from ------------------------------------------
+// norm[1 + n] = steps of env n that count; norm[0] = 1 / (all of them), or
+// 1 / (envs that have any) for the mean by sequence.  Counts are whole numbers:
+// their atomics give the same sum in any order.
+__global__ void __launch_bounds__(kThreads) count_kernel(Mask mask, int64_t N, int64_t T, int reduction, float* norm,
+                                                         unsigned long long* total, unsigned* some, unsigned* ticket) {
+  __shared__ unsigned part[kThreads / 32];
+  unsigned long long sum = 0;
+  unsigned rows = 0;
+  for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
+    unsigned c = 0;
+    for (int64_t t = threadIdx.x; t < T; t += kThreads) c += mask_at(mask, n * T + t) ? 1u : 0u;
+    c = __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = c;
+    __syncthreads();
+    c = 0;
+    for (int w = 0; w < kThreads / 32; ++w) c += part[w];
+    if (threadIdx.x == 0) norm[1 + n] = (float)c;
+    sum += c;
+    rows += c > 0;
+  }
+  if (threadIdx.x == 0) {
+    atomicAdd(total, sum);
+    atomicAdd(some, rows);
+    __threadfence();
+    if (atomicAdd(ticket, 1u) == gridDim.x - 1) {
+      __threadfence();
+      const unsigned long long all = atomicExch(total, 0ull);
+      const unsigned envs = atomicExch(some, 0u);
+      const double by = reduction == RLS_REDUCE_SEQUENCE ? (double)envs : (double)all;
+      norm[0] = by > 0.0 ? (float)(1.0 / by) : 0.f;
+      *ticket = 0u;
+    }
+  }
+}
+
+// ---- the loss over log-probabilities ----------------------------------------------
+struct Terms {
+  const float* lp;
+  Policy p;
+  Mask mask;
+  int64_t M, T;
+};
+
+__device__ __forceinline__ void load4(const float* p, int64_t i, int64_t M, float (&o)[4]) {
+  if (i + 4 <= M) {
+    const float4 v = *reinterpret_cast<const float4*>(p + i);
+    o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = i + e < M ? p[i + e] : 0.f;
+  }
+}
+
+// One pass over the steps: the sums of the loss and the statistics (SUMS) and
+// the gradient (GRAD).
+template <bool SUMS, bool GRAD>
+__global__ void __launch_bounds__(kThreads) policy_kernel(Terms t, float scale, const float* g, int force, float* grad,
+                                                          SumOut out) {
+  if constexpr (!SUMS) {
+    if (g && !force && *g == scale) return;
+  }
+  const float up = g ? *g : scale;
+  double sum[kSums] = {0, 0, 0, 0, 0, 0};
+  const int64_t step = (int64_t)gridDim.x * kThreads * 4;
+  for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; i < t.M; i += step) {
+    float lp[4], old_lp[4], adv[4], ref[4], d[4];
+    load4(t.lp, i, t.M, lp);
+    load4(t.p.old_lp, i, t.M, old_lp);
+    if (!t.p.adv_row) load4(t.p.adv, i, t.M, adv);
+    if (t.p.ref) load4(t.p.ref, i, t.M, ref);
+    int64_t env = i / t.T, col = i - env * t.T;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      d[e] = 0.f;
+      if (i + e < t.M && mask_at(t.mask, i + e)) {
+        const PolicyTerm o = policy_term(t.p, (double)lp[e], old_lp[e], t.p.adv_row ? t.p.adv[env] : adv[e],
+                                         t.p.ref ? ref[e] : 0.f);
+        const float w = policy_weight(t.p, env);
+        d[e] = w * o.d * up;
+        if constexpr (SUMS) {
+          sum[0] += (double)w * (double)o.loss;
+          sum[1] += o.kl; sum[2] += o.drift; sum[3] += o.clipped ? 1.0 : 0.0; sum[5] += 1.0;
+        }
+      }
+      if (++col == t.T) { col = 0; ++env; }
+    }
+    if constexpr (GRAD) {
+      if (i + 4 <= t.M) {
+        *reinterpret_cast<float4*>(grad + i) = make_float4(d[0], d[1], d[2], d[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e < t.M) grad[i + e] = d[e];
+      }
+    }
+  }
+  if constexpr (SUMS) finish_sums<kThreads>(sum, out);
+}
+
+// The policy loss over long rows: their records' terms.
+__global__ void __launch_bounds__(kThreads) row_sums_kernel(const float4* stats, const float* entropy, int64_t rows,
+                                                       SumOut o) {
+  double sum[kSums] = {0, 0, 0, 0, 0, 0};
+  for (int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x; row < rows; row += (int64_t)gridDim.x * kThreads) {
+    const int flags = __float_as_int(stats[2 * row].w);
+    if (!(flags & kFlagKept)) continue;
+    const float4 q = stats[2 * row + 1];
+    sum[0] += q.y; sum[1] += q.z; sum[2] += q.w;
+    sum[3] += flags & kFlagClipped ? 1.0 : 0.0;
+    if (entropy) sum[4] += entropy[row];
+    sum[5] += 1.0;
+  }
+  finish_sums<kThreads>(sum, o);
+}
+
+bool aligned(const void* p, size_t a = 16) { return p == nullptr || ((uintptr_t)p % a) == 0; }
+
+bool policy_ok(const rls_policy_t* q) {
+  return q && q->kl_kind >= RLS_KL_K1 && q->kl_kind <= RLS_KL_K3 && q->reduction >= RLS_REDUCE_TOKEN &&
+         q->reduction <= RLS_REDUCE_SUM;
+}
+bool mask_ok(const void* mask, int kind) {
+  return kind >= RLS_MASK_NONE && kind <= RLS_MASK_I64 && (mask == nullptr) == (kind == RLS_MASK_NONE);
+}
+size_t mask_align(int kind) {
+  return kind == RLS_MASK_I64 ? 8 : kind == RLS_MASK_F32 || kind == RLS_MASK_I32 ? 4 : kind == RLS_MASK_BF16 ? 2 : 1;
+}
+
+Policy make_policy(const rls_policy_t& q, const float* old_lp, const float* adv, int per_env, const float* ref,
+                   const float* norm, bool masked, int64_t N, int64_t T) {
+  Policy p{};
+  p.old_lp = old_lp;
+  p.adv = adv;
+  p.adv_row = per_env != 0;
+  p.ref = ref;
+  p.lo = 1.f - q.clip_low;
+  p.hi = 1.f + q.clip_high;
+  p.dual = q.dual_clip;
+  p.log_lo = q.clip_low < 1.f ? std::log1p(-(double)q.clip_low) : -INFINITY;
+  p.log_hi = std::log1p((double)q.clip_high);
+  p.log_dual = q.dual_clip > 0.f ? std::log((double)q.dual_clip) : INFINITY;
+  p.kl_coef = q.kl_coef;
+  p.kl_kind = q.kl_kind;
+  p.ent_coef = q.entropy_coef;
+  p.reduction = q.reduction;
+  p.norm = masked && q.reduction != RLS_REDUCE_SUM ? norm : nullptr;
+  // Without a mask both means weigh every step alike.
+  p.w = q.reduction == RLS_REDUCE_SUM ? 1.f : (float)(1.0 / ((double)N * (double)T));
+  return p;
+}
+
+int launch_count(const Policy& p, const Mask& mask, float* norm, int64_t N, int64_t T, void* ws, cudaStream_t s) {
+  if (!p.norm) return RLS_OK;
+  const int64_t blocks = N < 8LL * num_sms() ? N : 8LL * num_sms();
+  count_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(mask, N, T, p.reduction, norm, total_of(ws), rows_of(ws),
+                                                     ticket_of(ws));
+  return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
+}
+
+int64_t policy_blocks(int64_t M) { return sum_blocks((M + kThreads * 4 - 1) / (kThreads * 4)); }
+
+// Where a call of `blocks` CTAs leaves its sums.
+int sums_in(void* ws, size_t wsb, int64_t blocks, float* loss, float* stats, cudaStream_t s, SumOut* o) {
+  if (64 + (size_t)blocks * kSums * sizeof(double) > wsb) return RLS_EWORKSPACE;
+  if (int st = prepare_layout(ws, wsb, kLayoutScratch, s)) return st;
+  *o = SumOut{reinterpret_cast<double*>(static_cast<char*>(ws) + 64), ticket_of(ws), loss, stats};
+  return RLS_OK;
+}
+
+// No steps at all: loss and statistics 0.
+int clear_loss(float* loss, float* stats, cudaStream_t s) {
+  DeviceGuard guard{loss, stats};
+  if (guard.status()) return guard.status();
+  if (cudaMemsetAsync(loss, 0, sizeof(float), s) != cudaSuccess) return RLS_ECUDA;
+  if (stats && cudaMemsetAsync(stats, 0, (kSums - 1) * sizeof(float), s) != cudaSuccess) return RLS_ECUDA;
+  return RLS_OK;
+}
+
+// ---- logits -----------------------------------------------------------------------
+struct LogitsCall {
+  const void* x;
+  int64_t es, ss;
+  const int64_t* tokens;
+  Mask mask;
+  void* g;
+  int64_t ges, gss;
+  int64_t N, T, V;
+  float temperature;
+  int dtype;
+};
+
+int check_logits(const LogitsCall& c) {
+  if (c.N < 0 || c.T < 0 || c.V < 1) return RLS_EINVAL;
+  if (c.dtype != RLS_F32 && c.dtype != RLS_BF16) return RLS_EINVAL;
+  if (!(c.temperature > 0.f) || !std::isfinite(c.temperature)) return RLS_EINVAL;
+  if (!mask_ok(c.mask.p, c.mask.kind)) return RLS_EINVAL;
+  if (c.T > 0 && c.N > INT64_MAX / c.T) return RLS_EINVAL;
+  if (c.N == 0 || c.T == 0) return RLS_OK;
+  if (!c.x || !c.tokens) return RLS_EINVAL;
+  if (c.es < 0 || c.ss < 0 || c.ges < 0 || c.gss < 0) return RLS_EINVAL;
+  // a gradient's rows may not overlap, in whichever order they lie
+  if (c.g) {
+    const bool steps_in = (c.T == 1 || c.gss >= c.V) && (c.N == 1 || c.ges >= (c.T - 1) * c.gss + c.V);
+    const bool envs_in = (c.N == 1 || c.ges >= c.V) && (c.T == 1 || c.gss >= (c.N - 1) * c.ges + c.V);
+    if (!steps_in && !envs_in) return RLS_EINVAL;
+  }
+  const size_t e = c.dtype == RLS_BF16 ? 2 : 4;
+  if (!aligned(c.x, e) || !aligned(c.g, e) || !aligned(c.tokens, 8) || !aligned(c.mask.p, mask_align(c.mask.kind)))
+    return RLS_EALIGN;
+  return RLS_OK;
+}
+
+template <class T>
+Rows<T> rows_of_call(const LogitsCall& c) {
+  Rows<T> r{};
+  r.x = static_cast<const T*>(c.x);
+  r.es = c.es;
+  r.ss = c.ss;
+  r.rows = c.N * c.T;
+  r.seq = c.T;
+  r.V = c.V;
+  r.tokens = c.tokens;
+  r.mask = c.mask;
+  r.c = (float)(1.4426950408889634074 / (double)c.temperature);
+  r.inv_temp = (float)(1.0 / (double)c.temperature);
+  r.flat = c.N == 1 || (c.T == 1 ? false : c.es == c.T * c.ss);
+  if (c.T == 1 && c.N > 1) { r.ss = c.es; r.flat = true; }
+  return r;
+}
+template <class T>
+GradRows<T> grad_of_call(const LogitsCall& c) {
+  GradRows<T> r{};
+  r.g = static_cast<T*>(c.g);
+  r.es = c.ges;
+  r.ss = c.gss;
+  r.flat = c.N == 1 || c.ges == c.T * c.gss;
+  if (c.T == 1 && c.N > 1) { r.ss = c.ges; r.flat = true; }
+  return r;
+}
+
+template <class T, bool ENT, int MODE, class Src>
+int launch_rows(const LogitsCall& c, const RowOut& out, const Src& src, cudaStream_t s) {
+  const Rows<T> in = rows_of_call<T>(c);
+  const GradRows<T> gr = grad_of_call<T>(c);
+  if (c.V <= kLaneVocab) return launch_lane_rows<T, ENT, MODE, Src>(in, out, gr, src, s);
+  return launch_cta_rows<T, ENT, MODE, Src>(in, out, gr, src, s);
+}
+template <int MODE, class Src>
+int launch_logits(const LogitsCall& c, bool ent, const RowOut& out, const Src& src, cudaStream_t s) {
+  if (c.dtype == RLS_F32)
+    return ent ? launch_rows<float, true, MODE>(c, out, src, s) : launch_rows<float, false, MODE>(c, out, src, s);
+  return ent ? launch_rows<__nv_bfloat16, true, MODE>(c, out, src, s)
+             : launch_rows<__nv_bfloat16, false, MODE>(c, out, src, s);
+}
+
+}  // namespace
+
+int64_t rls::tok::sum_blocks(int64_t need) {
+  const int64_t most = 8LL * num_sms();
+  return need < most ? need : most;
+}
+
+extern "C" int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
+                                  const void* mask, int mask_kind, float* logprobs, float* entropy, float* row_stats,
+                                  int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature, int in_dtype,
+                                  void* stream) {
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, nullptr, 0, 0, num_envs, seq_len,
+               vocab, temperature, in_dtype};
+  if (int st = check_logits(c)) return st;
+  if (num_envs == 0 || seq_len == 0) return RLS_OK;
+  if (!logprobs) return RLS_EINVAL;
+  if (!aligned(logprobs) || !aligned(entropy) || !aligned(row_stats)) return RLS_EALIGN;
+  DeviceGuard guard{logits, tokens, mask, logprobs, entropy, row_stats};
+  if (guard.status()) return guard.status();
+  std::lock_guard<std::recursive_mutex> lock(launch_mutex());
+  return launch_logits<kFwd>(c, entropy != nullptr, RowOut{logprobs, entropy, reinterpret_cast<float4*>(row_stats)},
+                             GivenGrad{nullptr, nullptr}, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int rls_token_logprobs_backward(const void* logits, int64_t env_stride, int64_t step_stride,
+                                           const int64_t* tokens, const void* mask, int mask_kind,
+                                           const float* row_stats, const float* grad_logprobs,
+                                           const float* grad_entropy, void* grad_logits, int64_t grad_env_stride,
+                                           int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab,
+                                           float temperature, int in_dtype, void* stream) {
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
+               grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
+  if (int st = check_logits(c)) return st;
+  if (num_envs == 0 || seq_len == 0) return RLS_OK;
+  if ((!row_stats && vocab > kLaneVocab) || !grad_logits) return RLS_EINVAL;
+  if (!aligned(row_stats) || !aligned(grad_logprobs, 4) || !aligned(grad_entropy, 4)) return RLS_EALIGN;
+  DeviceGuard guard{logits, tokens, mask, row_stats, grad_logprobs, grad_entropy, grad_logits};
+  if (guard.status()) return guard.status();
+  std::lock_guard<std::recursive_mutex> lock(launch_mutex());
+  const RowOut out{nullptr, nullptr, reinterpret_cast<float4*>(const_cast<float*>(row_stats))};
+  return launch_logits<kBwd>(c, grad_entropy != nullptr, out, GivenGrad{grad_logprobs, grad_entropy},
+                             reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int rls_policy_loss(const float* logprobs, const float* old_logprobs, const float* advantages,
+                               int advantages_per_env, const float* ref_logprobs, const void* mask, int mask_kind,
+                               const rls_policy_t* policy, float grad_scale, float* norm, float* loss,
+                               float* stats, float* grad_logprobs, int64_t num_envs, int64_t seq_len, void* ws, size_t ws_bytes,
+                               void* stream) {
+  if (num_envs < 0 || seq_len < 0 || !loss || !policy_ok(policy) || !mask_ok(mask, mask_kind)) return RLS_EINVAL;
+  if (seq_len > 0 && num_envs > INT64_MAX / seq_len) return RLS_EINVAL;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t M = num_envs * seq_len;
+  if (M == 0) {
+    return clear_loss(loss, stats, s);
+  }
+  if (!logprobs || !old_logprobs || !advantages || !ws) return RLS_EINVAL;
+  if (mask && policy->reduction != RLS_REDUCE_SUM && !norm) return RLS_EINVAL;
+  if (!aligned(logprobs) || !aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) ||
+      !aligned(grad_logprobs) || !aligned(ws) || !aligned(norm, 4) || !aligned(loss, 4) || !aligned(stats, 4) ||
+      !aligned(mask, mask_align(mask_kind)))
+    return RLS_EALIGN;
+  DeviceGuard guard{logprobs, old_logprobs, advantages, ref_logprobs, mask, norm, loss, stats, grad_logprobs, ws};
+  if (guard.status()) return guard.status();
+  std::lock_guard<std::recursive_mutex> lock(launch_mutex());
+  Terms t{logprobs,
+          make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm, mask != nullptr,
+                      num_envs, seq_len),
+          Mask{mask, mask_kind}, M, seq_len};
+  SumOut sums;
+  const int64_t blocks = policy_blocks(M);
+  if (int st = sums_in(ws, ws_bytes, blocks, loss, stats, s, &sums)) return st;
+  if (int st = launch_count(t.p, t.mask, norm, num_envs, seq_len, ws, s)) return st;
+  if (grad_logprobs)
+    policy_kernel<true, true><<<(unsigned)blocks, kThreads, 0, s>>>(t, grad_scale, nullptr, 0, grad_logprobs, sums);
+  else
+    policy_kernel<true, false><<<(unsigned)blocks, kThreads, 0, s>>>(t, grad_scale, nullptr, 0, nullptr, sums);
+  return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
+}
+
+extern "C" int rls_policy_loss_backward(const float* logprobs, const float* old_logprobs, const float* advantages,
+                                        int advantages_per_env, const float* ref_logprobs, const void* mask,
+                                        int mask_kind, const rls_policy_t* policy, float grad_scale,
+                                        const float* grad_loss, int force, const float* norm, float* grad_logprobs,
+                                        int64_t num_envs, int64_t seq_len, void* stream) {
+  if (num_envs < 0 || seq_len < 0 || !policy_ok(policy) || !mask_ok(mask, mask_kind)) return RLS_EINVAL;
+  if (seq_len > 0 && num_envs > INT64_MAX / seq_len) return RLS_EINVAL;
+  const int64_t M = num_envs * seq_len;
+  if (M == 0) return RLS_OK;
+  if (!logprobs || !old_logprobs || !advantages || !grad_loss || !grad_logprobs) return RLS_EINVAL;
+  if (mask && policy->reduction != RLS_REDUCE_SUM && !norm) return RLS_EINVAL;
+  if (!aligned(logprobs) || !aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) ||
+      !aligned(grad_logprobs) || !aligned(norm, 4) || !aligned(grad_loss, 4) || !aligned(mask, mask_align(mask_kind)))
+    return RLS_EALIGN;
+  DeviceGuard guard{logprobs, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, grad_logprobs};
+  if (guard.status()) return guard.status();
+  std::lock_guard<std::recursive_mutex> lock(launch_mutex());
+  Terms t{logprobs,
+          make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm, mask != nullptr,
+                      num_envs, seq_len),
+          Mask{mask, mask_kind}, M, seq_len};
+  policy_kernel<false, true><<<(unsigned)policy_blocks(M), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      t, grad_scale, grad_loss, force, grad_logprobs, SumOut{});
+  return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
+}
+
+extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_stride,
+                                      const int64_t* tokens, const float* old_logprobs, const float* advantages,
+                                      int advantages_per_env, const float* ref_logprobs, const void* mask,
+                                      int mask_kind, const rls_policy_t* policy, float grad_scale, float* norm,
+                                      float* logprobs, float* entropy, float* row_stats, float* loss, float* stats,
+                                      void* grad_logits, int64_t grad_env_stride, int64_t grad_step_stride,
+                                      int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature,
+                                      int in_dtype, void* ws, size_t ws_bytes, void* stream) {
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
+               grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
+  if (!policy_ok(policy) || !loss) return RLS_EINVAL;
+  if (int st = check_logits(c)) return st;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t M = num_envs * seq_len;
+  if (M == 0) {
+    return clear_loss(loss, stats, s);
+  }
+  if (!old_logprobs || !advantages || !logprobs || (!row_stats && vocab > kLaneVocab) || !ws) return RLS_EINVAL;
+  if (policy->entropy_coef != 0.f && !entropy) return RLS_EINVAL;
+  if (mask && policy->reduction != RLS_REDUCE_SUM && !norm) return RLS_EINVAL;
+  if (!aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) || !aligned(logprobs) ||
+      !aligned(entropy) || !aligned(row_stats) || !aligned(ws) || !aligned(norm, 4) || !aligned(loss, 4) || !aligned(stats, 4))
+    return RLS_EALIGN;
+  DeviceGuard guard{logits, tokens, old_logprobs, advantages, ref_logprobs, mask, norm, logprobs, entropy, row_stats,
+                    loss, stats, grad_logits, ws};
+  if (guard.status()) return guard.status();
+  std::lock_guard<std::recursive_mutex> lock(launch_mutex());
+  const Policy p = make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm,
+                               mask != nullptr, num_envs, seq_len);
+  PolicyGrad src{p, grad_scale, nullptr, false, SumOut{}};
+  const int64_t blocks = sum_blocks((M + kThreads - 1) / kThreads);
+  if (int st = sums_in(ws, ws_bytes, sum_blocks(M), loss, stats, s, &src.sums)) return st;
+  if (int st = launch_count(p, c.mask, norm, num_envs, seq_len, ws, s)) return st;
+  const RowOut ro{logprobs, entropy, reinterpret_cast<float4*>(row_stats)};
+  if (int st = launch_logits<kBoth>(c, entropy != nullptr, ro, src, s)) return st;
+  if (vocab <= kLaneVocab) return RLS_OK;  // its kernel added up the terms itself
+  row_sums_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(ro.stats, entropy, M, src.sums);
+  return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
+}
+
+extern "C" int rls_policy_loss_logits_backward(const void* logits, int64_t env_stride, int64_t step_stride,
+                                               const int64_t* tokens, const float* old_logprobs,
+                                               const float* advantages, int advantages_per_env,
+                                               const float* ref_logprobs, const void* mask, int mask_kind,
+                                               const rls_policy_t* policy, float grad_scale, const float* grad_loss,
+                                               int force, const float* norm,
+                                               const float* row_stats, void* grad_logits, int64_t grad_env_stride,
+                                               int64_t grad_step_stride, int64_t num_envs, int64_t seq_len,
+                                               int64_t vocab, float temperature, int in_dtype, void* stream) {
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
+               grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
+  if (!policy_ok(policy)) return RLS_EINVAL;
+  if (int st = check_logits(c)) return st;
+  if (num_envs == 0 || seq_len == 0) return RLS_OK;
+  if (!old_logprobs || !advantages || !grad_loss || (!row_stats && vocab > kLaneVocab) || !grad_logits) return RLS_EINVAL;
+  if (mask && policy->reduction != RLS_REDUCE_SUM && !norm) return RLS_EINVAL;
+  if (!aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) || !aligned(row_stats) ||
+      !aligned(norm, 4) || !aligned(grad_loss, 4))
+    return RLS_EALIGN;
+  DeviceGuard guard{logits, tokens, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, row_stats,
+                    grad_logits};
+  if (guard.status()) return guard.status();
+  std::lock_guard<std::recursive_mutex> lock(launch_mutex());
+  const Policy p = make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm,
+                               mask != nullptr, num_envs, seq_len);
+  const RowOut ro{nullptr, nullptr, reinterpret_cast<float4*>(const_cast<float*>(row_stats))};
+  return launch_logits<kBwd>(c, policy->entropy_coef != 0.f, ro, PolicyGrad{p, grad_scale, grad_loss, force != 0, SumOut{}},
+                             reinterpret_cast<cudaStream_t>(stream));
+}

@@ -26,18 +26,19 @@
 #include <vector>
 
 #include "rlscan.h"
-
-namespace {
+#include "torch_shared.h"
 
 using at::Tensor;
 using OptT = std::optional<Tensor>;
+
+namespace rls_torch {
 
 // ---- per-(device, stream) workspace ------------------------------------------
 // Zero-filled when allocated; the kernels keep it consistent from call to call
 // (epoch-tagged records).  Grown by doubling; the old buffer is released to the
 // caching allocator on the same stream, so work still queued on it is safe.
-std::mutex g_ws_mu;
-std::map<std::pair<int, cudaStream_t>, Tensor> g_ws;
+static std::mutex g_ws_mu;
+static std::map<std::pair<int, cudaStream_t>, Tensor> g_ws;
 
 Tensor workspace_for(const at::Device& dev, cudaStream_t s, int64_t num_elements) {
   const int64_t need = (int64_t)rls_workspace_bytes(num_elements < 1 ? 1 : num_elements);
@@ -66,6 +67,15 @@ Tensor ready(const Tensor& t) {
 }
 OptT ready(const OptT& t) { return t ? OptT(ready(*t)) : OptT(); }
 
+Tensor f32(const Tensor& t) { return ready(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)); }
+OptT f32(const OptT& t) { return t ? OptT(f32(*t)) : OptT(); }
+
+}  // namespace rls_torch
+
+namespace {
+
+using namespace rls_torch;
+
 // One element type for the floating [N, T] streams of a call.
 int unify(std::vector<OptT*> streams) {
   bool all_bf16 = true, any = false;
@@ -79,9 +89,6 @@ int unify(std::vector<OptT*> streams) {
     if (*s && (*s)->scalar_type() != at::kFloat) *s = (*s)->to(at::kFloat);
   return RLS_F32;
 }
-
-Tensor f32(const Tensor& t) { return ready(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)); }
-OptT f32(const OptT& t) { return t ? OptT(f32(*t)) : OptT(); }
 
 const void* P(const OptT& t) { return t ? t->data_ptr() : nullptr; }
 const void* P(const Tensor& t) { return t.data_ptr(); }

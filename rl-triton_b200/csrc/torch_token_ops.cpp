@@ -1,0 +1,597 @@
+// torch_token_ops.cpp -- the token-level policy operators (namespace rl_triton)
+// with their gradients.
+//
+// Three operators are differentiable: token_logprobs (by the logits),
+// policy_loss (by the log-probabilities) and policy_loss_logits (by the
+// logits); so is preference_loss (by the log-probabilities).  Each has an
+// autograd function here that calls operators of its own (names with a leading
+// underscore: the kernels proper) through the dispatcher, so that fake tensors
+// and torch.compile see the same calls.  The functions are in C++ because a
+// training step on a small batch is bound by the host.
+//
+// The losses' gradients are written by the forward call, for an incoming
+// gradient of grad_scale; the backward call hands that buffer out, and writes
+// it anew only when the incoming gradient differs (the device compares: the
+// host is not synchronised).  A second backward pass over a retained graph
+// gets a buffer of its own.
+#include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <tuple>
+#include <utility>
+
+#include "rlscan.h"
+#include "torch_shared.h"
+
+namespace {
+
+using namespace rls_torch;
+using at::Tensor;
+using OptT = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+const float* F(const Tensor& t) { return t.data_ptr<float>(); }
+const float* F(const OptT& t) { return t && t->defined() ? t->data_ptr<float>() : nullptr; }
+float* W(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr<float>() : nullptr; }
+OptT opt(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+Tensor plain(const OptT& t) { return t ? *t : Tensor(); }
+
+// ---- inputs ----------------------------------------------------------------------
+struct MaskArg {
+  OptT t;
+  int kind = RLS_MASK_NONE;
+  const void* ptr() const { return t ? t->data_ptr() : nullptr; }
+};
+
+MaskArg mask_arg(const OptT& mask) {
+  MaskArg m;
+  if (!mask || !mask->defined()) return m;
+  Tensor t = *mask;
+  switch (t.scalar_type()) {
+    case at::kBool: case at::kByte: case at::kChar: m.kind = RLS_MASK_U8; break;
+    case at::kFloat: m.kind = RLS_MASK_F32; break;
+    case at::kBFloat16: m.kind = RLS_MASK_BF16; break;
+    case at::kInt: m.kind = RLS_MASK_I32; break;
+    case at::kLong: m.kind = RLS_MASK_I64; break;
+    default: t = t.ne(0); m.kind = RLS_MASK_U8;
+  }
+  m.t = t.is_contiguous() ? t : t.contiguous();
+  if (m.t->numel() == 0) { m.t = OptT(); m.kind = RLS_MASK_NONE; }
+  return m;
+}
+
+// Logits as the kernels take them: any env and step strides, the vocabulary
+// contiguous.
+Tensor logits_arg(const Tensor& t) {
+  return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous();
+}
+int dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? RLS_BF16 : RLS_F32; }
+Tensor tokens_arg(const Tensor& t) {
+  Tensor c = t.scalar_type() == at::kLong ? t : t.to(at::kLong);
+  return c.is_contiguous() ? c : c.contiguous();
+}
+
+// The buffer of a logits gradient.  It takes the logits' own strides where they
+// leave no more than a quarter of the buffer unused (a slice of the steps, a
+// vocabulary cut from a padded one), and starts at the same place within 16
+// bytes: every row then has the alignment of its logits, which the kernels need
+// for 16-byte stores.
+Tensor op_grad_buffer(const Tensor& logits) {
+  const int64_t n = logits.size(0), t = logits.size(1), v = logits.size(2);
+  const int64_t e = logits.element_size();
+  const int64_t es = logits.stride(0), ss = logits.stride(1);
+  if (logits.numel() == 0 || (v > 1 && logits.stride(2) != 1)) return at::empty(logits.sizes(), logits.options());
+  const bool apart = (t == 1 || ss >= v) && (n == 1 || es >= (t - 1) * ss + v);
+  const int64_t span = (n - 1) * es + (t - 1) * ss + v;
+  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16) / e;
+  if (!apart || span > n * t * v + n * t * v / 4 || (off == 0 && logits.is_contiguous()))
+    return at::empty(logits.sizes(), logits.options());
+  return at::empty({span + off}, logits.options()).as_strided(logits.sizes(), logits.strides(), off);
+}
+
+struct LogitsArgs {
+  Tensor x, tokens;
+  MaskArg mask;
+  int64_t n, t, v;
+  LogitsArgs(const Tensor& logits, const Tensor& tok, const OptT& m)
+      : x(logits_arg(logits)), tokens(tokens_arg(tok)), mask(mask_arg(m)), n(x.size(0)), t(x.size(1)), v(x.size(2)) {}
+};
+
+Tensor like(const Tensor& t, at::IntArrayRef sizes) { return at::empty(sizes, t.options().dtype(at::kFloat)); }
+
+// What a long row keeps for the backward call.
+Tensor row_stats(const LogitsArgs& a, bool keep) {
+  return like(a.x, keep && a.v > RLS_SHORT_VOCAB ? at::IntArrayRef({a.n, a.t, RLS_ROW_STATS}) : at::IntArrayRef({0}));
+}
+
+// ---- log-probabilities -------------------------------------------------------------
+// (logprobs, entropy or an empty tensor, the rows' statistics or an empty tensor)
+std::tuple<Tensor, Tensor, Tensor> op_logprobs(const Tensor& logits, const Tensor& tokens, const OptT& mask,
+                                               double temperature, bool entropy, bool keep) {
+  const LogitsArgs a(logits, tokens, mask);
+  Tensor lp = like(a.x, {a.n, a.t});
+  Tensor ent = like(a.x, entropy ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
+  Tensor stats = row_stats(a, keep);
+  check(rls_token_logprobs(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), a.mask.ptr(),
+                           a.mask.kind, W(lp), W(ent), W(stats), a.n, a.t, a.v, (float)temperature, dtype_of(a.x),
+                           stream_of(a.x)),
+        "rls_token_logprobs");
+  return {lp, ent, stats};
+}
+
+Tensor op_logprobs_backward(const Tensor& logits, const Tensor& tokens, const OptT& mask, const Tensor& stats,
+                            const OptT& g_lp, const OptT& g_ent, double temperature) {
+  const LogitsArgs a(logits, tokens, mask);
+  const OptT gl = f32(g_lp), ge = f32(g_ent);
+  Tensor g = op_grad_buffer(a.x);
+  check(rls_token_logprobs_backward(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(),
+                                    a.mask.ptr(), a.mask.kind, W(stats), F(gl), F(ge), g.data_ptr(), g.stride(0),
+                                    g.stride(1), a.n, a.t, a.v, (float)temperature, dtype_of(a.x), stream_of(a.x)),
+        "rls_token_logprobs_backward");
+  return g;
+}
+
+// ---- policy loss ---------------------------------------------------------------------
+rls_policy_t policy_of(double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
+                       double entropy_coef, int64_t reduction) {
+  rls_policy_t p{};
+  p.clip_low = (float)clip_low;
+  p.clip_high = (float)clip_high;
+  p.dual_clip = (float)dual_clip;
+  p.kl_coef = (float)kl_coef;
+  p.entropy_coef = (float)entropy_coef;
+  p.kl_kind = (int)kl;
+  p.reduction = (int)reduction;
+  return p;
+}
+
+Tensor norm_for(const MaskArg& m, const Tensor& ref, int64_t n, int64_t reduction) {
+  return like(ref, {m.t && reduction != RLS_REDUCE_SUM ? n + 1 : 0});
+}
+
+Tensor policy_workspace(const Tensor& t) { return workspace_for(t.device(), stream_of(t), 1 << 20); }
+
+// (loss, statistics [5], norm, gradient or an empty tensor)
+std::tuple<Tensor, Tensor, Tensor, Tensor> op_policy(const Tensor& logprobs, const Tensor& old_logprobs,
+                                                     const Tensor& advantages, const OptT& mask, const OptT& ref,
+                                                     double clip_low, double clip_high, double dual_clip,
+                                                     double kl_coef, int64_t kl, int64_t reduction, double grad_scale,
+                                                     bool need_grad) {
+  const Tensor lp = f32(logprobs), old_lp = f32(old_logprobs), adv = f32(advantages);
+  const OptT rf = f32(ref);
+  const MaskArg m = mask_arg(mask);
+  const int64_t n = lp.size(0), t = lp.size(1);
+  const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, 0.0, reduction);
+  Tensor loss = like(lp, {}), stats = like(lp, {5}), norm = norm_for(m, lp, n, reduction);
+  Tensor grad = like(lp, need_grad ? at::IntArrayRef({n, t}) : at::IntArrayRef({0}));
+  Tensor ws = policy_workspace(lp);
+  check(rls_policy_loss(F(lp), F(old_lp), F(adv), adv.dim() == 1, F(rf), m.ptr(), m.kind, &p, (float)grad_scale,
+                        W(norm), loss.data_ptr<float>(), stats.data_ptr<float>(), W(grad), n, t, ws.data_ptr(),
+                        (size_t)ws.numel(), stream_of(lp)),
+        "rls_policy_loss");
+  return {loss, stats, norm, grad};
+}
+
+void op_policy_backward_(Tensor& grad, const Tensor& logprobs, const Tensor& old_logprobs, const Tensor& advantages,
+                         const OptT& mask, const OptT& ref, const Tensor& norm, const Tensor& grad_loss,
+                         double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
+                         int64_t reduction, double grad_scale, bool force) {
+  const Tensor lp = f32(logprobs), old_lp = f32(old_logprobs), adv = f32(advantages), g = f32(grad_loss);
+  const OptT rf = f32(ref);
+  const MaskArg m = mask_arg(mask);
+  const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, 0.0, reduction);
+  check(rls_policy_loss_backward(F(lp), F(old_lp), F(adv), adv.dim() == 1, F(rf), m.ptr(), m.kind, &p,
+                                 (float)grad_scale, F(g), force, W(norm), W(grad), lp.size(0), lp.size(1),
+                                 stream_of(lp)),
+        "rls_policy_loss_backward");
+}
+
+// (loss, logprobs, entropy or empty, statistics [5], norm, the rows' statistics, gradient or empty)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_policy_logits(
+    const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
+    const OptT& mask, const OptT& ref, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
+    double entropy_coef, bool entropy, double temperature, int64_t reduction, double grad_scale, bool need_grad) {
+  const LogitsArgs a(logits, tokens, mask);
+  const Tensor old_lp = f32(old_logprobs), adv = f32(advantages);
+  const OptT rf = f32(ref);
+  const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
+  Tensor loss = like(a.x, {}), stats = like(a.x, {5}), norm = norm_for(a.mask, a.x, a.n, reduction);
+  Tensor lp = like(a.x, {a.n, a.t}), rows = row_stats(a, true);
+  Tensor ent = like(a.x, entropy || entropy_coef != 0.0 ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
+  Tensor g = need_grad ? op_grad_buffer(a.x) : at::empty({0}, a.x.options());
+  Tensor ws = policy_workspace(a.x);
+  check(rls_policy_loss_logits(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), F(old_lp),
+                               F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, &p, (float)grad_scale,
+                               W(norm), W(lp), W(ent), W(rows), loss.data_ptr<float>(), stats.data_ptr<float>(),
+                               need_grad ? g.data_ptr() : nullptr, need_grad ? g.stride(0) : 0,
+                               need_grad ? g.stride(1) : 0, a.n, a.t, a.v, (float)temperature, dtype_of(a.x),
+                               ws.data_ptr(), (size_t)ws.numel(), stream_of(a.x)),
+        "rls_policy_loss_logits");
+  return {loss, lp, ent, stats, norm, rows, g};
+}
+
+void op_policy_logits_backward_(Tensor& grad, const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
+                                const Tensor& advantages, const OptT& mask, const OptT& ref, const Tensor& norm,
+                                const Tensor& rows, const Tensor& grad_loss, double clip_low,
+                                double clip_high, double dual_clip, double kl_coef, int64_t kl, double entropy_coef,
+                                double temperature, int64_t reduction, double grad_scale, bool force) {
+  const LogitsArgs a(logits, tokens, mask);
+  const Tensor old_lp = f32(old_logprobs), adv = f32(advantages), up = f32(grad_loss);
+  const OptT rf = f32(ref);
+  const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
+  check(rls_policy_loss_logits_backward(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(),
+                                        F(old_lp), F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, &p,
+                                        (float)grad_scale, F(up), force, W(norm), W(rows),
+                                        grad.data_ptr(), grad.stride(0), grad.stride(1), a.n, a.t, a.v,
+                                        (float)temperature, dtype_of(a.x), stream_of(a.x)),
+        "rls_policy_loss_logits_backward");
+}
+
+// ---- preference loss -------------------------------------------------------------------
+// rejected absent: `chosen` holds both halves, [2 pairs, T].
+struct Pairs {
+  Tensor lp[2];
+  const float* p[2];
+  const float* ref[2];
+  const void* mask[2];
+  MaskArg m[2];
+  OptT rf[2];
+  int kind = RLS_MASK_NONE;
+  int64_t b, t[2];
+  bool ref_pair = false;
+  Pairs(const Tensor& chosen, const OptT& rejected, const OptT& ref_c, const OptT& ref_r, const OptT& mask_c,
+        const OptT& mask_r) {
+    lp[0] = f32(chosen);
+    rf[0] = f32(ref_c);
+    m[0] = mask_arg(mask_c);
+    if (rejected) {
+      lp[1] = f32(*rejected);
+      rf[1] = f32(ref_r);
+      m[1] = mask_arg(mask_r);
+      if (m[0].t && m[1].t && m[0].kind != m[1].kind)
+        for (auto& x : m) x = mask_arg(x.t->ne(0));
+    }
+    const OptT& any = rf[0] ? rf[0] : rf[1];
+    ref_pair = any && any->dim() == 1;
+    if (rejected) {
+      b = lp[0].size(0);
+      for (int k = 0; k < 2; ++k) {
+        t[k] = lp[k].size(1);
+        p[k] = F(lp[k]);
+        ref[k] = F(rf[k]);
+        mask[k] = m[k].ptr();
+        if (m[k].t) kind = m[k].kind;
+      }
+      return;
+    }
+    // The second half starts b rows into the first tensor.  A half whose rows
+    // leave it off the kernels' 16-byte boundary is copied.
+    b = lp[0].size(0) / 2;
+    t[0] = t[1] = lp[0].size(1);
+    const int64_t at = b * t[0];
+    if (at % 4 != 0 && at > 0) {
+      lp[1] = lp[0].slice(0, b).clone();
+      if (rf[0] && !ref_pair) rf[1] = rf[0]->slice(0, b).clone();
+    }
+    p[0] = F(lp[0]);
+    p[1] = lp[1].defined() ? F(lp[1]) : p[0] + at;
+    ref[0] = F(rf[0]);
+    ref[1] = !rf[0] ? nullptr : rf[1] ? F(rf[1]) : ref[0] + (ref_pair ? b : at);
+    mask[0] = m[0].ptr();
+    kind = m[0].kind;
+    const int64_t esz = m[0].t ? m[0].t->element_size() : 0;
+    mask[1] = m[0].t ? static_cast<const char*>(mask[0]) + at * esz : nullptr;
+  }
+};
+
+// (loss, rewards [2, pairs], coefficients [2, pairs])
+std::tuple<Tensor, Tensor, Tensor> op_preference(const Tensor& chosen, const OptT& rejected, const OptT& ref_chosen,
+                                                 const OptT& ref_rejected, const OptT& chosen_mask,
+                                                 const OptT& rejected_mask, double beta, double smoothing,
+                                                 int64_t kind, bool normalized) {
+  const Pairs q(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask);
+  Tensor loss = like(q.lp[0], {}), rewards = like(q.lp[0], {2, q.b}), coef = like(q.lp[0], {2, q.b});
+  const int64_t want = 64 * q.b < (1 << 20) ? (1 << 20) : 64 * q.b;
+  Tensor ws = workspace_for(q.lp[0].device(), stream_of(q.lp[0]), want);
+  check(rls_preference_loss(q.p[0], q.p[1], q.ref[0], q.ref[1], q.ref_pair, q.mask[0], q.mask[1], q.kind, q.b, q.t[0],
+                            q.t[1], (float)beta, (float)smoothing, (int)kind, normalized, loss.data_ptr<float>(),
+                            W(rewards), W(coef), ws.data_ptr(), (size_t)ws.numel(), stream_of(q.lp[0])),
+        "rls_preference_loss");
+  return {loss, rewards, coef};
+}
+
+// The gradients by (chosen, rejected); where `halves`, one gradient over both
+// halves and an empty tensor.
+std::tuple<Tensor, Tensor> op_preference_backward(const Tensor& coef, const Tensor& grad_loss,
+                                                  const OptT& chosen_mask, const OptT& rejected_mask,
+                                                  int64_t chosen_len, int64_t rejected_len, bool halves) {
+  const Tensor g = f32(grad_loss);
+  const int64_t b = coef.size(1);
+  MaskArg m[2] = {mask_arg(chosen_mask), mask_arg(rejected_mask)};
+  if (m[0].t && m[1].t && m[0].kind != m[1].kind)
+    for (auto& x : m) x = mask_arg(x.t->ne(0));
+  const int kind = m[0].t ? m[0].kind : m[1].kind;
+  Tensor gc, gr;
+  if (halves) {
+    // coefficients [2, b] are those of 2b rows one below the other
+    gc = like(coef, {2 * b, chosen_len});
+    gr = like(coef, {0});
+    check(rls_preference_loss_backward(W(coef), F(g), m[0].ptr(), nullptr, kind, W(gc), nullptr, 2 * b, chosen_len, 0,
+                                       stream_of(coef)),
+          "rls_preference_loss_backward");
+  } else {
+    gc = like(coef, {b, chosen_len});
+    gr = like(coef, {b, rejected_len});
+    check(rls_preference_loss_backward(W(coef), F(g), m[0].ptr(), m[1].ptr(), kind, W(gc), W(gr), b, chosen_len,
+                                       rejected_len, stream_of(coef)),
+          "rls_preference_loss_backward");
+  }
+  return {gc, gr};
+}
+
+// ---- autograd ------------------------------------------------------------------------
+template <class Sig>
+auto op_handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+}
+
+Tensor call_grad_buffer(const Tensor& logits) {
+  static auto op = op_handle<Tensor(const Tensor&)>("rl_triton::_grad_buffer");
+  return op.call(logits);
+}
+
+struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const OptT& mask,
+                               double temperature, bool entropy) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_handle<decltype(op_logprobs)>("rl_triton::_token_logprobs");
+    auto [lp, ent, stats] = op.call(logits, tokens, mask, temperature, entropy, true);
+    ctx->save_for_backward({logits, tokens, plain(mask), stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->set_materialize_grads(false);
+    if (!entropy) ctx->mark_non_differentiable({ent});
+    return {lp, ent};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    static auto op = op_handle<decltype(op_logprobs_backward)>("rl_triton::_token_logprobs_backward");
+    const auto s = ctx->get_saved_variables();
+    Tensor out;
+    if (g[0].defined() || g[1].defined())
+      out = op.call(s[0], s[1], opt(s[2]), s[3], opt(g[0]), opt(g[1]), ctx->saved_data["temperature"].toDouble());
+    return {out, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> token_logprobs_autograd(const Tensor& logits, const Tensor& tokens, const OptT& mask,
+                                                   double temperature, bool entropy) {
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    auto o = TokenLogprobs::apply(logits, tokens, mask, temperature, entropy);
+    return {o[0], o[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = op_handle<decltype(op_logprobs)>("rl_triton::_token_logprobs");
+  auto [lp, ent, stats] = op.call(logits, tokens, mask, temperature, entropy, false);
+  return {lp, ent};
+}
+
+struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& lp, const Tensor& old_lp, const Tensor& adv,
+                               const OptT& mask, const OptT& ref, double clip_low, double clip_high, double dual_clip,
+                               double kl_coef, int64_t kl, int64_t reduction, double grad_scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_handle<decltype(op_policy)>("rl_triton::_policy_loss");
+    auto [loss, stats, norm, grad] = op.call(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl,
+                                             reduction, grad_scale, true);
+    ctx->save_for_backward({lp, old_lp, adv, plain(mask), plain(ref), norm});
+    ctx->saved_data["grad"] = grad;
+    ctx->saved_data["args"] = std::vector<double>{clip_low, clip_high, dual_clip, kl_coef, grad_scale};
+    ctx->saved_data["kl"] = kl;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->mark_non_differentiable({stats});
+    return {loss, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    static auto op = op_handle<decltype(op_policy_backward_)>("rl_triton::_policy_loss_backward_");
+    const auto s = ctx->get_saved_variables();
+    const auto a = ctx->saved_data["args"].toDoubleVector();
+    Tensor grad;
+    const auto made = ctx->saved_data.find("grad");
+    const bool fresh = made == ctx->saved_data.end();
+    if (fresh) {
+      grad = at::empty(s[0].sizes(), s[0].options().dtype(at::kFloat));
+    } else {
+      grad = made->second.toTensor();
+      ctx->saved_data.erase(made);
+    }
+    op.call(grad, s[0], s[1], s[2], opt(s[3]), opt(s[4]), s[5], g[0], a[0], a[1], a[2], a[3],
+            ctx->saved_data["kl"].toInt(), ctx->saved_data["reduction"].toInt(), a[4], fresh);
+    variable_list out(12);
+    out[0] = s[0].scalar_type() == at::kFloat ? grad : grad.to(s[0].scalar_type());
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& lp, const Tensor& old_lp, const Tensor& adv,
+                                                const OptT& mask, const OptT& ref, double clip_low, double clip_high,
+                                                double dual_clip, double kl_coef, int64_t kl, int64_t reduction,
+                                                double grad_scale) {
+  if (at::GradMode::is_enabled() && lp.requires_grad()) {
+    auto o = PolicyLoss::apply(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, reduction,
+                               grad_scale);
+    return {o[0], o[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = op_handle<decltype(op_policy)>("rl_triton::_policy_loss");
+  auto [loss, stats, norm, grad] = op.call(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl,
+                                           reduction, grad_scale, false);
+  return {loss, stats};
+}
+
+struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const Tensor& old_lp,
+                               const Tensor& adv, const OptT& mask, const OptT& ref, double clip_low, double clip_high,
+                               double dual_clip, double kl_coef, int64_t kl, double entropy_coef, bool entropy,
+                               double temperature, int64_t reduction, double grad_scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_handle<decltype(op_policy_logits)>("rl_triton::_policy_loss_logits");
+    auto [loss, lp, ent, stats, norm, rows, grad] =
+        op.call(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef,
+                entropy, temperature, reduction, grad_scale, true);
+    ctx->save_for_backward({logits, tokens, old_lp, adv, plain(mask), plain(ref), norm, rows});
+    ctx->saved_data["grad"] = grad;
+    ctx->saved_data["args"] =
+        std::vector<double>{clip_low, clip_high, dual_clip, kl_coef, entropy_coef, temperature, grad_scale};
+    ctx->saved_data["kl"] = kl;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->mark_non_differentiable({lp, ent, stats});
+    return {loss, lp, ent, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    static auto op = op_handle<decltype(op_policy_logits_backward_)>("rl_triton::_policy_loss_logits_backward_");
+    const auto s = ctx->get_saved_variables();
+    const auto a = ctx->saved_data["args"].toDoubleVector();
+    Tensor grad;
+    const auto made = ctx->saved_data.find("grad");
+    const bool fresh = made == ctx->saved_data.end();
+    if (fresh) {
+      grad = call_grad_buffer(s[0]);
+    } else {
+      grad = made->second.toTensor();
+      ctx->saved_data.erase(made);
+    }
+    op.call(grad, s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), s[6], s[7], g[0], a[0], a[1], a[2], a[3],
+            ctx->saved_data["kl"].toInt(), a[4], a[5], ctx->saved_data["reduction"].toInt(), a[6], fresh);
+    variable_list out(16);
+    out[0] = grad;
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss_logits_autograd(
+    const Tensor& logits, const Tensor& tokens, const Tensor& old_lp, const Tensor& adv, const OptT& mask,
+    const OptT& ref, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
+    double entropy_coef, bool entropy, double temperature, int64_t reduction, double grad_scale) {
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    auto o = PolicyLossLogits::apply(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef,
+                                     kl, entropy_coef, entropy, temperature, reduction, grad_scale);
+    return {o[0], o[1], o[2], o[3]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = op_handle<decltype(op_policy_logits)>("rl_triton::_policy_loss_logits");
+  auto r = op.call(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef,
+                   entropy, temperature, reduction, grad_scale, false);
+  return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r)};
+}
+
+struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& chosen, const OptT& rejected, const OptT& ref_c,
+                               const OptT& ref_r, const OptT& mask_c, const OptT& mask_r, double beta,
+                               double smoothing, int64_t kind, bool normalized) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = op_handle<decltype(op_preference)>("rl_triton::_preference_loss");
+    auto [loss, rewards, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
+                                         normalized);
+    ctx->save_for_backward({coef, plain(mask_c), plain(mask_r)});
+    ctx->saved_data["len"] = chosen.size(1);
+    ctx->saved_data["rejected_len"] = rejected ? rejected->size(1) : (int64_t)-1;
+    ctx->saved_data["types"] = std::vector<int64_t>{
+        (int64_t)chosen.scalar_type(), (int64_t)(rejected ? rejected->scalar_type() : chosen.scalar_type())};
+    ctx->mark_non_differentiable({rewards});
+    return {loss, rewards};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    static auto op = op_handle<decltype(op_preference_backward)>("rl_triton::_preference_loss_backward");
+    const auto s = ctx->get_saved_variables();
+    const int64_t other = ctx->saved_data["rejected_len"].toInt();
+    auto [gc, gr] = op.call(s[0], g[0], opt(s[1]), opt(s[2]), ctx->saved_data["len"].toInt(), other < 0 ? 0 : other,
+                            other < 0);
+    const auto types = ctx->saved_data["types"].toIntVector();
+    variable_list out(10);
+    out[0] = gc.to((at::ScalarType)types[0]);
+    if (other >= 0) out[1] = gr.to((at::ScalarType)types[1]);
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> preference_loss_autograd(const Tensor& chosen, const OptT& rejected, const OptT& ref_c,
+                                                    const OptT& ref_r, const OptT& mask_c, const OptT& mask_r,
+                                                    double beta, double smoothing, int64_t kind, bool normalized) {
+  if (at::GradMode::is_enabled() && (chosen.requires_grad() || (rejected && rejected->requires_grad()))) {
+    auto o = PreferenceLoss::apply(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind, normalized);
+    return {o[0], o[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = op_handle<decltype(op_preference)>("rl_triton::_preference_loss");
+  auto [loss, rewards, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
+                                       normalized);
+  return {loss, rewards};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(rl_triton, m) {
+  m.def("token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature, bool entropy) "
+        "-> (Tensor, Tensor)");
+  m.def("policy_loss(Tensor logprobs, Tensor old_logprobs, Tensor advantages, Tensor? mask, Tensor? ref_logprobs, "
+        "float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, int reduction, float grad_scale) "
+        "-> (Tensor, Tensor)");
+  m.def("policy_loss_logits(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? mask, "
+        "Tensor? ref_logprobs, float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, "
+        "float entropy_coef, bool entropy, float temperature, int reduction, float grad_scale) "
+        "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("preference_loss(Tensor chosen, Tensor? rejected, Tensor? ref_chosen, Tensor? ref_rejected, "
+        "Tensor? chosen_mask, Tensor? rejected_mask, float beta, float smoothing, int kind, bool normalized) "
+        "-> (Tensor, Tensor)");
+  m.def("_grad_buffer(Tensor logits) -> Tensor");
+  m.def("_token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature, bool entropy, bool keep) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("_token_logprobs_backward(Tensor logits, Tensor tokens, Tensor? mask, Tensor row_stats, Tensor? g_logprobs, "
+        "Tensor? g_entropy, float temperature) -> Tensor");
+  m.def("_policy_loss(Tensor logprobs, Tensor old_logprobs, Tensor advantages, Tensor? mask, Tensor? ref_logprobs, "
+        "float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, int reduction, float grad_scale, "
+        "bool need_grad) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("_policy_loss_backward_(Tensor(a!) grad, Tensor logprobs, Tensor old_logprobs, Tensor advantages, "
+        "Tensor? mask, Tensor? ref_logprobs, Tensor norm, Tensor grad_loss, float clip_low, float clip_high, "
+        "float dual_clip, float kl_coef, int kl, int reduction, float grad_scale, bool force) -> ()");
+  m.def("_policy_loss_logits(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? mask, "
+        "Tensor? ref_logprobs, float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, "
+        "float entropy_coef, bool entropy, float temperature, int reduction, float grad_scale, bool need_grad) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("_policy_loss_logits_backward_(Tensor(a!) grad, Tensor logits, Tensor tokens, Tensor old_logprobs, "
+        "Tensor advantages, Tensor? mask, Tensor? ref_logprobs, Tensor norm, Tensor row_stats, "
+        "Tensor grad_loss, float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, "
+        "float entropy_coef, float temperature, int reduction, float grad_scale, bool force) -> ()");
+  m.def("_preference_loss(Tensor chosen, Tensor? rejected, Tensor? ref_chosen, Tensor? ref_rejected, "
+        "Tensor? chosen_mask, Tensor? rejected_mask, float beta, float smoothing, int kind, bool normalized) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("_preference_loss_backward(Tensor coef, Tensor grad_loss, Tensor? chosen_mask, Tensor? rejected_mask, "
+        "int chosen_len, int rejected_len, bool halves) -> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(rl_triton, CUDA, m) {
+  m.impl("_grad_buffer", &op_grad_buffer);
+  m.impl("_token_logprobs", &op_logprobs);
+  m.impl("_token_logprobs_backward", &op_logprobs_backward);
+  m.impl("_policy_loss", &op_policy);
+  m.impl("_policy_loss_backward_", &op_policy_backward_);
+  m.impl("_policy_loss_logits", &op_policy_logits);
+  m.impl("_policy_loss_logits_backward_", &op_policy_logits_backward_);
+  m.impl("_preference_loss", &op_preference);
+  m.impl("_preference_loss_backward", &op_preference_backward);
+}
+
+TORCH_LIBRARY_IMPL(rl_triton, Autograd, m) {
+  m.impl("token_logprobs", &token_logprobs_autograd);
+  m.impl("policy_loss", &policy_loss_autograd);
+  m.impl("policy_loss_logits", &policy_loss_logits_autograd);
+  m.impl("preference_loss", &preference_loss_autograd);
+  // The kernels proper have no second derivative: differentiating them raises.
+  for (const char* name : {"_token_logprobs", "_token_logprobs_backward", "_policy_loss", "_policy_loss_logits",
+                           "_preference_loss", "_preference_loss_backward"})
+    m.impl(name, torch::autograd::autogradNotImplementedFallback());
+}

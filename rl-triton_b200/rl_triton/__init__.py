@@ -4,7 +4,10 @@ simonsays1980/rl-triton v0.1.3, computed by hand-written sm_100a CUDA kernels
 paths and error behaviour as the reference's src/rl_triton/__init__.py, plus
 fused PPO epilogues (compute_gae_normalized, compute_gae_value_loss) and the
 observation-skip masking mode (compute_gae_obs_skip) the reference does not
-have."""
+have, and the token-level policy operators around them: log-probabilities from
+logits (compute_token_logprobs), the clipped policy loss (compute_policy_loss,
+compute_policy_loss_from_logits) and the paired preference loss
+(compute_preference_loss), each with its gradient."""
 
 __version__ = "0.1.3"
 
@@ -18,6 +21,9 @@ from rl_triton.ops.fused import (  # additions: fused PPO epilogues and masking 
     compute_gae_obs_skip,
     compute_gae_value_loss,
 )
+from rl_triton.ops.token_logprobs import compute_token_logprobs  # additions: token-level policy operators
+from rl_triton.ops.policy_loss import compute_policy_loss, compute_policy_loss_from_logits
+from rl_triton.ops.preference_loss import compute_preference_loss
 
 __all__ = [
     "compute_discounted_returns",
@@ -28,6 +34,10 @@ __all__ = [
     "compute_gae_obs_skip",
     "compute_gae_value_loss",
     "compute_lambda_returns",
+    "compute_policy_loss",
+    "compute_policy_loss_from_logits",
+    "compute_preference_loss",
     "compute_retrace",
+    "compute_token_logprobs",
     "compute_vtrace",
 ]

@@ -37,12 +37,26 @@ ALG_SCAN_FWD = 6
 SEG_EXCLUSIVE = 2
 LOSS_MSE = 0
 LOSS_HUBER = 1
+ROW_STATS = 8
+SHORT_VOCAB = 1024
+MASK_NONE, MASK_U8, MASK_F32, MASK_BF16, MASK_I32, MASK_I64 = range(6)
+KL_K1, KL_K2, KL_K3 = 1, 2, 3
+REDUCE_TOKEN, REDUCE_SEQUENCE, REDUCE_SUM = 0, 1, 2
+PREFERENCE_SIGMOID, PREFERENCE_IPO, PREFERENCE_HINGE = 0, 1, 2
 
 
 class Segment(ctypes.Structure):
     """Mirror of rls_segment_t."""
 
     _fields_ = [("t0", ctypes.c_int64), ("total_len", ctypes.c_int64), ("halo", ctypes.c_void_p)]
+
+
+class Policy(ctypes.Structure):
+    """Mirror of rls_policy_t."""
+
+    _fields_ = [("clip_low", ctypes.c_float), ("clip_high", ctypes.c_float), ("dual_clip", ctypes.c_float),
+                ("kl_coef", ctypes.c_float), ("entropy_coef", ctypes.c_float), ("kl_kind", ctypes.c_int),
+                ("reduction", ctypes.c_int)]
 
 
 def _load() -> ctypes.CDLL:
@@ -126,12 +140,97 @@ def _(inputs, dones, seed_values, ends_at, t0=-1, total=-1, halo=None):
 def _(u, v, carry, direction, t0=-1, total=-1, halo=None):
     return _f32_like(u)
 
+
+# The token-level operators (csrc/torch_token_ops.cpp): the differentiable ones
+# are autograd functions over the ones with an underscore, which have the fakes.
+def _f32(like, *shape):
+    return torch.empty(shape, dtype=torch.float32, device=like.device)
+
+
+@torch.library.register_fake("rl_triton::_grad_buffer")
+def _grad_buffer_fake(logits):
+    # the strides op_grad_buffer gives (see there)
+    n, t, v = logits.shape
+    if logits.numel() == 0 or (v > 1 and logits.stride(2) != 1):
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    es, ss = logits.stride(0), logits.stride(1)
+    apart = (t == 1 or ss >= v) and (n == 1 or es >= (t - 1) * ss + v)
+    span = (n - 1) * es + (t - 1) * ss + v
+    if not apart or span > n * t * v + n * t * v // 4:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return torch.empty_strided(logits.shape, logits.stride(), dtype=logits.dtype, device=logits.device)
+
+
+def _row_stats_fake(logits, keep):
+    n, t, v = logits.shape
+    return _f32(logits, n, t, ROW_STATS) if keep and v > SHORT_VOCAB else _f32(logits, 0)
+
+
+@torch.library.register_fake("rl_triton::_token_logprobs")
+def _(logits, tokens, mask, temperature, entropy, keep):
+    n, t, _v = logits.shape
+    return (_f32(logits, n, t), _f32(logits, n, t) if entropy else _f32(logits, 0),
+            _row_stats_fake(logits, keep))
+
+
+@torch.library.register_fake("rl_triton::_token_logprobs_backward")
+def _(logits, tokens, mask, row_stats, g_logprobs, g_entropy, temperature):
+    return _grad_buffer_fake(logits)
+
+
+def _norm_fake(mask, like, n, reduction):
+    return _f32(like, n + 1 if mask is not None and mask.numel() and reduction != REDUCE_SUM else 0)
+
+
+@torch.library.register_fake("rl_triton::_policy_loss")
+def _(logprobs, old_logprobs, advantages, mask, ref_logprobs, clip_low, clip_high, dual_clip, kl_coef, kl, reduction,
+      grad_scale, need_grad):
+    n, t = logprobs.shape
+    return (_f32(logprobs), _f32(logprobs, 5), _norm_fake(mask, logprobs, n, reduction),
+            _f32(logprobs, n, t) if need_grad else _f32(logprobs, 0))
+
+
+@torch.library.register_fake("rl_triton::_policy_loss_backward_")
+def _(grad, *args):
+    return None
+
+
+@torch.library.register_fake("rl_triton::_policy_loss_logits")
+def _(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, clip_low, clip_high, dual_clip, kl_coef, kl,
+      entropy_coef, entropy, temperature, reduction, grad_scale, need_grad):
+    n, t, _v = logits.shape
+    return (_f32(logits), _f32(logits, n, t),
+            _f32(logits, n, t) if entropy or entropy_coef != 0.0 else _f32(logits, 0), _f32(logits, 5),
+            _norm_fake(mask, logits, n, reduction), _row_stats_fake(logits, True),
+            _grad_buffer_fake(logits) if need_grad else torch.empty((0,), dtype=logits.dtype, device=logits.device))
+
+
+@torch.library.register_fake("rl_triton::_policy_loss_logits_backward_")
+def _(grad, *args):
+    return None
+
+
+@torch.library.register_fake("rl_triton::_preference_loss")
+def _(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, smoothing, kind, normalized):
+    b = chosen.shape[0] if rejected is not None else chosen.shape[0] // 2
+    return _f32(chosen), _f32(chosen, 2, b), _f32(chosen, 2, b)
+
+
+@torch.library.register_fake("rl_triton::_preference_loss_backward")
+def _(coef, grad_loss, chosen_mask, rejected_mask, chosen_len, rejected_len, halves):
+    b = coef.shape[1]
+    if halves:
+        return _f32(coef, 2 * b, chosen_len), _f32(coef, 0)
+    return _f32(coef, b, chosen_len), _f32(coef, b, rejected_len)
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
 _SEG = ctypes.POINTER(Segment)
+_POL = ctypes.POINTER(Policy)
 
 _SIGS = {
     "rls_workspace_bytes": (_SZ, [_I64]),
@@ -154,6 +253,18 @@ _SIGS = {
     "rls_gae_value_loss": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I, _F, _I, _P, _SZ,
                                 _P]),
     "rls_gae_obs_skip": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I, _P]),
+    "rls_token_logprobs": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _F, _I, _P]),
+    "rls_token_logprobs_backward": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F,
+                                         _I, _P]),
+    "rls_policy_loss": (_I, [_P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _P, _P, _P, _I64, _I64, _P, _SZ, _P]),
+    "rls_policy_loss_backward": (_I, [_P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _I, _P, _P, _I64, _I64, _P]),
+    "rls_policy_loss_logits": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _P, _P, _P, _P, _P, _P,
+                                    _I64, _I64, _I64, _I64, _I64, _F, _I, _P, _SZ, _P]),
+    "rls_policy_loss_logits_backward": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _I, _P, _P,
+                                             _P, _I64, _I64, _I64, _I64, _I64, _F, _I, _P]),
+    "rls_preference_loss": (_I, [_P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _F, _F, _I, _I, _P, _P, _P, _P,
+                                 _SZ, _P]),
+    "rls_preference_loss_backward": (_I, [_P, _P, _P, _P, _I, _P, _P, _I64, _I64, _I64, _P]),
     "rls_gae_noalloc": (_I, [_P, _P, _P, _P, _P, _I, _P, _I64, _I64, _F, _F, _I, _SEG, _P]),
     "rls_gae_noalloc_error": (_I, [_P]),
 }
