@@ -68,7 +68,8 @@ struct Rows {
   int64_t V;
   const int64_t* tokens;
   Mask mask;
-  float c;             // log2(e) / temperature
+  float c;             // log2(e) / temperature, rounded
+  double c64;          // the same, not
   float inv_temp;
   bool flat;           // es == seq * ss
 
@@ -127,13 +128,18 @@ __device__ __forceinline__ double log2_of(float s0) {
 }
 
 // fp64, so that what follows from it (the ratio of the policy loss) does not
-// carry the rounding of the fp32 output.
-__device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c) {
+// carry the rounding of the fp32 output.  Two errors that S0 has in common over
+// all rows are taken out to first order, since sums of many log-probabilities
+// (the preference loss's) would add them up: c was rounded, which moves log S0 by
+// the mean of d times the relative error; and ex2.approx lies 5.0e-8 low on
+// average (measured over d in (-8, 0)), except at the maximum, where d is 0.
+__device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c, double c64) {
   const Shift sh = shift_of(r, c);
   if (ex2(sh(x_tok)) == r.s0) return 0.0;  // the others are below fp32's reach
-  const double d = sh.far ? ((double)x_tok - (double)sh.off) * (double)c
-                          : (double)x_tok * (double)c - (double)sh.off;
-  return (d - log2_of(r.s0)) * 0.693147180559945309417;
+  const double res = r.far ? 0.0 : (double)r.m * (double)c - (double)sh.off;  // d at the maximum
+  const double log_s0 = log2_of(r.s0) - res + (c64 / (double)c - 1.0) * ((double)r.t - res)
+                        + 7.2e-8 * (double)(1.f - __frcp_rn(r.s0));
+  return (((double)x_tok - (double)r.m) * c64 - log_s0) * 0.693147180559945309417;
 }
 __device__ __forceinline__ float entropy_of(const RowStats& r) {
   if (r.alone) return 0.f;
@@ -214,9 +220,10 @@ __device__ __forceinline__ Cut cut_row(const T* p, int64_t V) {
 
 // ---- running statistics --------------------------------------------------------
 // (m, s0, s1) of the elements seen: s0 = sum 2^d, s1 = sum 2^d d with d taken
-// from off = m c.  m starts at -kFar, not -inf, so that no difference of two
-// offsets is NaN; elements below it count as 0 (rows that have nothing above it
-// take the far form).
+// from off = m c; without an entropy to compute, s1 takes each vector's largest
+// d for all of its elements, which serves for logprob_of's small correction.
+// m starts at -kFar, not -inf, so that no difference of two offsets is NaN;
+// elements below it count as 0 (rows that have nothing above it take the far form).
 template <bool ENT>
 struct Run {
   float m = -kFar, off, s0 = 0.f, s1 = 0.f;
@@ -225,16 +232,10 @@ struct Run {
   __device__ __forceinline__ void raise(float mx, float c) {
     const float to = mx * c, by = off - to;
     const float k = ex2(by);
-    if constexpr (ENT) s1 = fmaf(s0, fmaxf(by, kDeep), s1) * k;
+    s1 = fmaf(s0, fmaxf(by, kDeep), s1) * k;
     s0 *= k;
     m = mx;
     off = to;
-  }
-  __device__ __forceinline__ void add(float x, float c) {
-    const float d = fmaf(x, c, -off);
-    const float e = ex2(d);
-    s0 += e;
-    if constexpr (ENT) s1 = fmaf(e, fmaxf(d, kDeep), s1);
   }
   template <int K>
   __device__ __forceinline__ void add(const float (&x)[K], float c) {
@@ -242,15 +243,26 @@ struct Run {
 #pragma unroll
     for (int k = 1; k < K; ++k) mx = fmaxf(mx, x[k]);
     if (mx > m) raise(mx, c);
+    float e[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) add(x[k], c);
+    for (int k = 0; k < K; ++k) {
+      const float d = fmaf(x[k], c, -off);
+      e[k] = ex2(d);
+      if constexpr (ENT) s1 = fmaf(e[k], fmaxf(d, kDeep), s1);
+    }
+#pragma unroll
+    for (int w = 1; w < K; w *= 2)
+#pragma unroll
+      for (int k = 0; k + w < K; k += 2 * w) e[k] += e[k + w];
+    s0 += e[0];
+    if constexpr (!ENT) s1 = fmaf(e[0], fmaxf(fmaf(mx, c, -off), kDeep), s1);
   }
   __device__ __forceinline__ void join(float om, float ooff, float os0, float os1) {
     const bool up = om > m;
     const float to = up ? ooff : off;
     const float d0 = off - to, d1 = ooff - to;
     const float k0 = ex2(d0), k1 = ex2(d1);
-    if constexpr (ENT) s1 = fmaf(s0, fmaxf(d0, kDeep), s1) * k0 + fmaf(os0, fmaxf(d1, kDeep), os1) * k1;
+    s1 = fmaf(s0, fmaxf(d0, kDeep), s1) * k0 + fmaf(os0, fmaxf(d1, kDeep), os1) * k1;
     s0 = s0 * k0 + os0 * k1;
     if (up) m = om;
     off = to;
@@ -263,7 +275,7 @@ __device__ __forceinline__ void warp_join(Run<ENT>& r, int width = 32) {
     const float om = __shfl_xor_sync(0xffffffffu, r.m, o);
     const float oo = __shfl_xor_sync(0xffffffffu, r.off, o);
     const float a = __shfl_xor_sync(0xffffffffu, r.s0, o);
-    const float b = ENT ? __shfl_xor_sync(0xffffffffu, r.s1, o) : 0.f;
+    const float b = __shfl_xor_sync(0xffffffffu, r.s1, o);
     r.join(om, oo, a, b);
   }
 }
@@ -434,7 +446,7 @@ __device__ __forceinline__ void block_join(Run<ENT>& r, float c) {
   r.m = __shfl_sync(0xffffffffu, z.m, 0);
   r.off = __shfl_sync(0xffffffffu, z.off, 0);
   r.s0 = __shfl_sync(0xffffffffu, z.s0, 0);
-  if constexpr (ENT) r.s1 = __shfl_sync(0xffffffffu, z.s1, 0);
+  r.s1 = __shfl_sync(0xffffffffu, z.s1, 0);
 }
 
 template <int NT>
@@ -473,10 +485,10 @@ __device__ __noinline__ RowStats far_stats(const T* x, int64_t V, float c) {
     const float d = (Vec<T>::get(x + v) - m) * c;
     const float e = ex2(d);
     s0 += e;
-    if constexpr (ENT) s1 = fmaf(e, fmaxf(d, kDeep), s1);
+    s1 = fmaf(e, fmaxf(d, kDeep), s1);
   }
   s0 = block_sum<NT>(s0);
-  if constexpr (ENT) s1 = block_sum<NT>(s1);
+  s1 = block_sum<NT>(s1);
   return RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f};
 }
 
@@ -510,7 +522,7 @@ __device__ __forceinline__ RowStats row_stats(const T* x, int64_t V, float c) {
   block_join<ENT, NT>(run, c);
   if (!(run.s0 >= kLeast && run.s0 <= kMost)) return far_stats<T, ENT, NT>(x, V, c);
   const float d = fmaf(run.m, c, -run.off), e = ex2(d);
-  return RowStats{run.m, run.s0, ENT ? run.s1 / run.s0 : 0.f, false, ENT && run.s0 == e && run.s1 == e * d};
+  return RowStats{run.m, run.s0, run.s1 / run.s0, false, ENT && run.s0 == e && run.s1 == e * d};
 }
 
 template <class T, int NT>
@@ -599,7 +611,7 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
     if constexpr (MODE != kBwd) {
       const float xt = ok ? Vec<T>::get(x + tok) : NAN;
       r = row_stats<T, ENT, NT, U>(x, in.V, in.c);
-      const double lp = logprob_of(xt, r, in.c);
+      const double lp = logprob_of(xt, r, in.c, in.c64);
       float ent = 0.f;
       if constexpr (ENT) ent = entropy_of(r);
       int flags = kFlagKept;
@@ -637,6 +649,392 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
       if (a == 0.f && b == 0.f) zero_row<T, NT>(g, in.V);
       else grad_row<T, ENT, NT, U>(x, g, in.V, tok, shift_of(r, in.c), row_grad(a, b, r, in.inv_temp));
     }
+  }
+}
+
+// ---- long rows: a pipeline over rows --------------------------------------------
+// C CTAs (a cluster) of NT threads share a row: each CTA takes one stretch of its 16-byte
+// vectors, each thread every NT-th vector of the stretch, at most K, in slots of
+// shared memory that no other thread reads.  So the copies (cp.async, all K of a
+// row in flight at once) need no barrier, only the thread's own wait; the one
+// barrier a row is the join of the statistics.  A slot is refilled from the next row as
+// soon as its last use is over: in the forward call when its elements are added
+// up, with a gradient when the gradient is stored, so that the next row's loads
+// are in flight during this row's stores and reductions.
+__device__ __forceinline__ void copy16(uint4* to, const uint4* from) {
+  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Stores to the same shared variable of another CTA of the cluster.
+__device__ __forceinline__ void store_remote(float4* p, unsigned rank, float4 v) {
+  unsigned at = (unsigned)__cvta_generic_to_shared(p), there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+
+constexpr int kMostCtas = 8;  // of a cluster (the portable limit)
+
+// Every thread's value to every warp of the row's CTAs: `mine` (one per warp, from
+// lane 0) goes to all CTAs' tables; the tables of two successive calls differ,
+// so that one barrier a call suffices.
+template <int NT, bool CL>
+struct Table {
+  static constexpr int kWarps = NT / 32;
+  static constexpr int kMost = CL ? kWarps * kMostCtas : kWarps;
+  float4 at[2][kMost];
+};
+template <int NT, bool CL>
+__device__ __forceinline__ const float4* exchange(Table<NT, CL>& t, unsigned& turn, float4 mine, unsigned rank,
+                                                  unsigned size) {
+  float4* tab = t.at[turn & 1];
+  ++turn;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (CL) {
+    if (lane < size) store_remote(tab + rank * (NT / 32) + warp, lane, mine);
+    cluster_barrier();
+  } else {
+    if (lane == 0) tab[warp] = mine;
+    __syncthreads();
+  }
+  return tab;
+}
+
+// Joins (m, s0, s1) over a warp: to the common maximum first, then plain sums.
+__device__ __forceinline__ void warp_gather(float& m, float& s0, float& s1, float c) {
+  float top = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float by = m * c - top * c;
+  const float k = ex2(by);
+  s1 = fmaf(s0, fmaxf(by, kDeep), s1) * k;
+  s0 *= k;
+  m = top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+  }
+}
+
+__device__ __forceinline__ float incoming_entropy(const PolicyGrad& s, float w, float) { return -w * s.p.ent_coef; }
+__device__ __forceinline__ float incoming_entropy(const GivenGrad&, float, float b) { return b; }
+
+template <class T, bool ENT, int MODE, class Src, int NT, int K, bool CL>
+__global__ void __launch_bounds__(NT, 768 / NT) pipe_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src) {
+  if constexpr (Src::kPolicy && MODE == kBwd) {
+    if (src.skip()) return;
+  }
+  constexpr int N = Vec<T>::N;
+  constexpr bool kGrad = MODE != kFwd;
+  extern __shared__ uint4 slots[];  // [K][NT]
+  __shared__ Table<NT, CL> table;
+  unsigned turn = 0;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const unsigned rank = CL ? cluster_rank() : 0, size = CL ? cluster_size() : 1;
+  const int64_t team = blockIdx.x / size, teams = gridDim.x / size;
+  uint4* mine = slots + tid;
+  const float c = in.c;
+
+  // The rows of this team in order: `window` says which of the next 32 are to be
+  // worked on; the others only get their zeros.
+  int64_t next_row = team;
+  unsigned window = 0;
+  int left = 0;
+  auto wanted = [&](int64_t row) -> bool {
+    if (row >= in.rows || !mask_at(in.mask, row)) return false;
+    if constexpr (MODE == kBwd && Src::kPolicy) return ENT || out.stats[2 * row + 1].x != 0.f;
+    if constexpr (MODE == kBwd && !Src::kPolicy) {
+      const float a = src.g_lp ? src.g_lp[row] : 0.f;
+      bool some = a != 0.f;
+      if constexpr (ENT) some = some || src.g_ent[row] != 0.f;
+      return some;
+    }
+    return true;
+  };
+  auto zeros = [&](int64_t row) {
+    T* g = gr.g + gr.at(row, in.seq);
+    const Cut cut = cut_row(g, in.V);
+    const int64_t per = (cut.nvec + size - 1) / size, v0 = per * rank;
+    const int64_t v1 = v0 + per < cut.nvec ? v0 + per : cut.nvec;
+    uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
+    for (int64_t v = v0 + tid; v < v1; v += NT) __stcs(gv + v, make_uint4(0, 0, 0, 0));
+    const int64_t ends = cut.head + cut.tail;
+    if (rank == 0 && tid < ends) g[tid < cut.head ? tid : in.V - ends + tid] = Vec<T>::put(0.f);
+  };
+  auto advance = [&]() -> int64_t {
+    for (;;) {
+      if (next_row >= in.rows) return -1;
+      if (left == 0) {
+        window = __ballot_sync(0xffffffffu, wanted(next_row + lane * teams));
+        left = 32;
+      }
+      const bool yes = window & 1u;
+      const int64_t row = next_row;
+      window >>= 1;
+      --left;
+      next_row += teams;
+      if (yes) return row;
+      if constexpr (MODE != kBwd) {
+        if (rank == 0 && tid == 0) {
+          out.logprob[row] = 0.f;
+          if (out.entropy) out.entropy[row] = 0.f;
+          if (out.stats) out.stats[2 * row] = out.stats[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      if (kGrad && gr.g) zeros(row);
+    }
+  };
+
+  // A row's place: its vectors from v0 on are this CTA's, `mid` of them.
+  struct Place {
+    int64_t row, tok;
+    const T* x;
+    int head, ends;   // elements before the first vector; those and the ones after the last
+    int64_t v0;
+    int mid;
+    bool ok;
+    float end, xt;    // the thread's end element; the token's logit
+    float old_lp, adv, ref, w;  // the policy loss's inputs
+    float a, b;       // incoming gradients of a backward call
+    float4 stats;
+  };
+  const int64_t V = in.V;
+  auto place = [&](int64_t row) -> Place {
+    Place p;
+    p.row = row;
+    p.x = in.x + in.at(row);
+    const Cut cut = cut_row(p.x, V);
+    p.head = (int)cut.head;
+    p.ends = rank == 0 ? (int)(cut.head + cut.tail) : 0;
+    const int64_t per = (cut.nvec + size - 1) / size;
+    p.v0 = per * rank;
+    const int64_t n = cut.nvec - p.v0;
+    p.mid = (int)(n < 0 ? 0 : n < per ? n : per);
+    p.tok = in.tokens[row];
+    p.ok = p.tok >= 0 && p.tok < V;
+    p.end = tid < p.ends ? Vec<T>::get(p.x + (tid < p.head ? tid : V - (cut.head + cut.tail) + tid)) : 0.f;
+    if constexpr (Src::kPolicy) {
+      const int64_t env = row / in.seq;
+      p.w = policy_weight(src.p, env);
+      if constexpr (MODE != kBwd) {
+        p.old_lp = src.p.old_lp[row];
+        p.adv = src.p.adv[src.p.adv_row ? env : row];
+        p.ref = src.p.ref ? src.p.ref[row] : 0.f;
+      }
+    }
+    if constexpr (MODE == kBwd) {
+      p.stats = out.stats[2 * row];
+      if constexpr (Src::kPolicy) p.a = out.stats[2 * row + 1].x;
+      else p.a = src.g_lp ? src.g_lp[row] : 0.f;
+      if constexpr (ENT && !Src::kPolicy) p.b = src.g_ent[row];
+    }
+    return p;
+  };
+  // The token's logit, asked for once the token itself is there.
+  auto token_logit = [&](Place& p) {
+    if constexpr (MODE != kBwd) p.xt = p.ok ? Vec<T>::get(p.x + p.tok) : NAN;
+  };
+  auto fetch = [&](const Place& p, int j) {
+    if (p.row >= 0 && tid + j * NT < p.mid)
+      copy16(mine + j * NT, reinterpret_cast<const uint4*>(p.x + p.head) + p.v0 + tid + j * NT);
+    copy_commit();
+  };
+
+  int64_t first = advance();
+  if (first < 0) return;  // the same for every CTA of the team
+  Place now = place(first);
+#pragma unroll
+  for (int j = 0; j < K; ++j) fetch(now, j);
+  token_logit(now);
+  if constexpr (CL && MODE != kBwd) cluster_barrier();  // the others' tables exist
+
+  for (;;) {
+    Place next;
+    next.row = -1;
+    // ---- statistics
+    RowStats r;
+    float a = 0.f, b = 0.f;
+    if constexpr (MODE != kBwd) {
+      if constexpr (MODE == kFwd) {
+        const int64_t row = advance();
+        if (row >= 0) next = place(row);
+      }
+      Run<ENT> run(c);
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if constexpr (MODE == kFwd) copy_wait<K - 1>();
+        else {
+          // slots j + 1 .. K - 1 may still be on their way
+          switch (K - 1 - j) {
+            case 0: copy_wait<0>(); break;   case 1: copy_wait<1>(); break;   case 2: copy_wait<2>(); break;
+            case 3: copy_wait<3>(); break;   case 4: copy_wait<4>(); break;   case 5: copy_wait<5>(); break;
+            case 6: copy_wait<6>(); break;   case 7: copy_wait<7>(); break;   case 8: copy_wait<8>(); break;
+            case 9: copy_wait<9>(); break;   case 10: copy_wait<10>(); break; case 11: copy_wait<11>(); break;
+            case 12: copy_wait<12>(); break; case 13: copy_wait<13>(); break; case 14: copy_wait<14>(); break;
+            default: copy_wait<15>(); break;
+          }
+        }
+        if (tid + j * NT < now.mid) {
+          float f[N];
+          Vec<T>::unpack(mine[j * NT], f);
+          run.add(f, c);
+        }
+        if constexpr (MODE == kFwd) fetch(next, j);
+      }
+      if (tid < now.ends) {
+        const float f[1] = {now.end};
+        run.add(f, c);
+      }
+      warp_gather(run.m, run.s0, run.s1, c);
+      {
+        const float4* tab = exchange(table, turn, make_float4(run.m, run.s0, run.s1, 0.f), rank, size);
+        const int n = size * (NT / 32);
+        float4 q = lane < n ? tab[lane] : make_float4(-kFar, 0.f, 0.f, 0.f);
+        if (CL && n > 32 && lane + 32 < n) {
+          const float4 q2 = tab[lane + 32];
+          const float top = fmaxf(q.x, q2.x);
+          const float d0 = q.x * c - top * c, d1 = q2.x * c - top * c;
+          const float k0 = ex2(d0), k1 = ex2(d1);
+          q.z = fmaf(q.y, fmaxf(d0, kDeep), q.z) * k0 + fmaf(q2.y, fmaxf(d1, kDeep), q2.z) * k1;
+          q.y = q.y * k0 + q2.y * k1;
+          q.x = top;
+        }
+        warp_gather(q.x, q.y, q.z, c);
+        run.m = q.x; run.s0 = q.y; run.s1 = q.z;
+      }
+      const float off = run.m * c, dm = fmaf(run.m, c, -off), em = ex2(dm);
+      r = RowStats{run.m, run.s0, run.s1 / run.s0, false, ENT && run.s0 == em && run.s1 == em * dm};
+      if (!(run.s0 >= kLeast && run.s0 <= kMost)) {  // the same in all threads of the team
+        // the far form, from global memory (the slots may hold the next row)
+        const T* xs = now.x + now.head + now.v0 * N;
+        const int64_t n = (int64_t)now.mid * N;
+        float m = tid < now.ends ? now.end : -INFINITY;
+        for (int64_t i = tid; i < n; i += NT) m = fmaxf(m, Vec<T>::get(xs + i));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float4* tab = exchange(table, turn, make_float4(m, 0.f, 0.f, 0.f), rank, size);
+        for (int w = 0; w < (int)size * (NT / 32); ++w) m = fmaxf(m, tab[w].x);
+        float s0 = 0.f, s1 = 0.f;
+        auto add = [&](float x) {
+          const float d = (x - m) * c;
+          const float e = ex2(d);
+          s0 += e;
+          s1 = fmaf(e, fmaxf(d, kDeep), s1);
+        };
+        for (int64_t i = tid; i < n; i += NT) add(Vec<T>::get(xs + i));
+        if (tid < now.ends) add(now.end);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+          s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+        }
+        tab = exchange(table, turn, make_float4(s0, s1, 0.f, 0.f), rank, size);
+        s0 = s1 = 0.f;
+        for (int w = 0; w < (int)size * (NT / 32); ++w) { s0 += tab[w].x; s1 += tab[w].y; }
+        r = RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f};
+      }
+      const double lp = logprob_of(now.xt, r, c, in.c64);
+      float ent = 0.f;
+      if constexpr (ENT) ent = entropy_of(r);
+      int flags = kFlagKept;
+      const bool writes = rank == 0 && tid == 0;
+      if constexpr (Src::kPolicy) {
+        const Policy& p = src.p;
+        const float w = now.w;
+        const PolicyTerm o = policy_term(p, lp, now.old_lp, now.adv, now.ref);
+        a = w * o.d;
+        if constexpr (ENT) b = -w * p.ent_coef;
+        if (o.clipped) flags |= kFlagClipped;
+        if (writes) {
+          const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
+          out.stats[2 * now.row + 1] = make_float4(a, w * term, o.kl, o.drift);
+        }
+      }
+      if (writes) {
+        out.logprob[now.row] = (float)lp;
+        if (out.entropy) out.entropy[now.row] = ent;
+        if (out.stats) out.stats[2 * now.row] = stats_word(r, flags);
+      }
+    } else {
+      r = stats_of(now.stats);
+      a = now.a;
+      if constexpr (ENT) b = incoming_entropy(src, now.w, now.b);
+    }
+    // ---- gradient
+    if constexpr (kGrad) {
+      const int64_t row = advance();
+      if (row >= 0) next = place(row);
+      if constexpr (Src::kPolicy) { a *= src.up(); b *= src.up(); }
+      if (!now.ok) a = NAN;
+      T* g = gr.g ? gr.g + gr.at(now.row, in.seq) : nullptr;
+      const bool none = a == 0.f && b == 0.f;
+      if (g && none) zeros(now.row);
+      const Shift sh = shift_of(r, c);
+      const RowGrad rg = row_grad(a, b, r, in.inv_temp);
+      const bool same = (((uintptr_t)now.x ^ (uintptr_t)g) & 15) == 0;
+      // the token's vector and its element there
+      const int64_t rel = now.tok - now.head - now.v0 * N;
+      const int tv = rel >= 0 && rel < (int64_t)now.mid * N ? (int)(rel / N) : -1;
+      const int te = (int)(rel - (int64_t)tv * N);
+      T* gs = g + now.head + now.v0 * N;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if constexpr (MODE == kBwd) copy_wait<K - 1>();
+        const int v = tid + j * NT;
+        if (g && !none && v < now.mid) {
+          float f[N];
+          Vec<T>::unpack(mine[j * NT], f);
+          if (sh.far) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = grad_at<ENT>(f[e], Shift{c, sh.off, true}, rg);
+          } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = grad_at<ENT>(f[e], Shift{c, sh.off, false}, rg);
+          }
+          if (v == tv) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (e == te) f[e] += rg.a;
+          }
+          if (same) {
+            __stcs(reinterpret_cast<uint4*>(gs) + v, Vec<T>::pack(f));
+          } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) gs[(int64_t)v * N + e] = Vec<T>::put(f[e]);
+          }
+        }
+        fetch(next, j);
+      }
+      if (g && !none && tid < now.ends) {
+        const int64_t i = tid < now.head ? tid : V - now.ends + tid;
+        float f = grad_at<ENT>(now.end, sh, rg);
+        if (i == now.tok) f += rg.a;
+        g[i] = Vec<T>::put(f);
+      }
+    }
+    if (next.row < 0) break;
+    token_logit(next);
+    now = next;
   }
 }
 
@@ -682,17 +1080,17 @@ __global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, 
       const float d = lane + k * G < V ? sh(f[k]) : -INFINITY;
       const float e = ex2(d);
       s0 += e;
-      if constexpr (ENT) s1 = fmaf(e, fmaxf(d, kDeep), s1);
+      s1 = fmaf(e, fmaxf(d, kDeep), s1);
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) {
       s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-      if constexpr (ENT) s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
     }
-    const RowStats r{m, s0, ENT ? s1 / s0 : 0.f, true, ENT && s0 == 1.f && s1 == 0.f};
+    const RowStats r{m, s0, s1 / s0, true, ENT && s0 == 1.f && s1 == 0.f};
     double lp = 0.0;
     float ent = 0.f;
-    if (Src::kPolicy || MODE != kBwd) lp = logprob_of(xt, r, in.c);
+    if (Src::kPolicy || MODE != kBwd) lp = logprob_of(xt, r, in.c, in.c64);
     if constexpr (ENT) ent = entropy_of(r);
     if (!kept) { lp = 0.0; ent = 0.f; }
     float a = 0.f, b = 0.f;

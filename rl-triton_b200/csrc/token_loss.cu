@@ -259,7 +259,8 @@ Rows<T> rows_of_call(const LogitsCall& c) {
   r.V = c.V;
   r.tokens = c.tokens;
   r.mask = c.mask;
-  r.c = (float)(1.4426950408889634074 / (double)c.temperature);
+  r.c64 = 1.4426950408889634074 / (double)c.temperature;
+  r.c = (float)r.c64;
   r.inv_temp = (float)(1.0 / (double)c.temperature);
   r.flat = c.N == 1 || (c.T == 1 ? false : c.es == c.T * c.ss);
   if (c.T == 1 && c.N > 1) { r.ss = c.es; r.flat = true; }

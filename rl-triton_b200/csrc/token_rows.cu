@@ -1,14 +1,59 @@
-// token_rows.cu -- the logits kernels for long rows: one CTA a row.
+// token_rows.cu -- the logits kernels for long rows: a pipeline over rows, and one CTA a row beyond
+// its reach.
 #include "token_launch.h"
 
 namespace rls {
 namespace tok {
 namespace {
 
-template <class T, bool ENT, int MODE, class Src, int NT>
-int go(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
+// The row pipeline with C CTAs a row.
+template <class T, bool ENT, int MODE, class Src, int NT, int K, bool CL>
+int pipe(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, int size, cudaStream_t s) {
+  auto kern = pipe_rows_kernel<T, ENT, MODE, Src, NT, K, CL>;
+  constexpr size_t smem = (size_t)NT * K * 16;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RLS_ECUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CL ? 1 : 0;
+  // Teams that fit on the device at once, asked once per device and cluster size
+  // (under the launch lock): a team that had to wait for another would double
+  // the time.
+  static int resident[64][4] = {{0}};
+  int& most = resident[dev][size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3];
+  if (!most) {
+    int n = 0;
+    if (smem > 32 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return RLS_ECUDA;
+    if (CL) {
+      cfg.gridDim = dim3((unsigned)size);
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) return RLS_ECUDA;
+    } else {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, NT, smem) != cudaSuccess || n < 1) return RLS_ECUDA;
+      n *= (int)(sum_blocks(1 << 30) / 8);
+    }
+    most = n;
+  }
+  int64_t teams = most;
+  if (teams > in.rows) teams = in.rows;
+  cfg.gridDim = dim3((unsigned)(teams * size));
+  return cudaLaunchKernelEx(&cfg, kern, in, out, gr, src) == cudaSuccess ? RLS_OK : RLS_ECUDA;
+}
+
+// Rows beyond the slots of a full cluster: one CTA a row, the second pass from L2.
+template <class T, bool ENT, int MODE, class Src>
+int plain(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
   const int64_t blocks = in.rows < 0x7fffffffLL ? in.rows : 0x7fffffffLL;
-  cta_rows_kernel<T, ENT, MODE, Src, NT, 4><<<(unsigned)blocks, NT, 0, s>>>(in, out, gr, src);
+  cta_rows_kernel<T, ENT, MODE, Src, 512, 4><<<(unsigned)blocks, 512, 0, s>>>(in, out, gr, src);
   return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
 }
 
@@ -17,8 +62,21 @@ int go(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& s
 template <class T, bool ENT, int MODE, class Src>
 int launch_cta_rows(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
   const int64_t nvec = in.V / Vec<T>::N;
-  if (nvec <= 512) return go<T, ENT, MODE, Src, 128>(in, out, gr, src, s);
-  return go<T, ENT, MODE, Src, 512>(in, out, gr, src, s);
+  int size = 1;
+  while (size < kMostCtas && nvec > (int64_t)size * 4096) size *= 2;
+  // few rows: more CTAs for each, down to 512 vectors a CTA
+  while (size < kMostCtas && in.rows * size < 2 * 148 && nvec > (int64_t)size * 1024) size *= 2;
+  const int64_t each = (nvec + size - 1) / size;
+  if (each > 4096) return plain<T, ENT, MODE, Src>(in, out, gr, src, s);
+  if (size > 1) {
+    if (each <= 1024) return pipe<T, ENT, MODE, Src, 256, 4, true>(in, out, gr, src, size, s);
+    return pipe<T, ENT, MODE, Src, 256, 16, true>(in, out, gr, src, size, s);
+  }
+  if (each <= 256) return pipe<T, ENT, MODE, Src, 64, 4, false>(in, out, gr, src, 1, s);
+  if (each <= 512) return pipe<T, ENT, MODE, Src, 64, 8, false>(in, out, gr, src, 1, s);
+  if (each <= 1024) return pipe<T, ENT, MODE, Src, 128, 8, false>(in, out, gr, src, 1, s);
+  if (each <= 2048) return pipe<T, ENT, MODE, Src, 256, 8, false>(in, out, gr, src, 1, s);
+  return pipe<T, ENT, MODE, Src, 256, 16, false>(in, out, gr, src, 1, s);
 }
 
 RLS_TOKEN_INSTANTIATE(launch_cta_rows)

@@ -393,10 +393,12 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
     ctx->saved_data["kl"] = kl;
     ctx->saved_data["reduction"] = reduction;
     ctx->mark_non_differentiable({stats});
+    ctx->set_materialize_grads(false);
     return {loss, stats};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     static auto op = op_handle<decltype(op_policy_backward_)>("rl_triton::_policy_loss_backward_");
+    if (!g[0].defined()) return variable_list(12);
     const auto s = ctx->get_saved_variables();
     const auto a = ctx->saved_data["args"].toDoubleVector();
     Tensor grad;
@@ -449,10 +451,12 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
     ctx->saved_data["kl"] = kl;
     ctx->saved_data["reduction"] = reduction;
     ctx->mark_non_differentiable({lp, ent, stats});
+    ctx->set_materialize_grads(false);
     return {loss, lp, ent, stats};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     static auto op = op_handle<decltype(op_policy_logits_backward_)>("rl_triton::_policy_loss_logits_backward_");
+    if (!g[0].defined()) return variable_list(16);
     const auto s = ctx->get_saved_variables();
     const auto a = ctx->saved_data["args"].toDoubleVector();
     Tensor grad;
@@ -502,10 +506,12 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
     ctx->saved_data["types"] = std::vector<int64_t>{
         (int64_t)chosen.scalar_type(), (int64_t)(rejected ? rejected->scalar_type() : chosen.scalar_type())};
     ctx->mark_non_differentiable({rewards});
+    ctx->set_materialize_grads(false);
     return {loss, rewards};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     static auto op = op_handle<decltype(op_preference_backward)>("rl_triton::_preference_loss_backward");
+    if (!g[0].defined()) return variable_list(10);
     const auto s = ctx->get_saved_variables();
     const int64_t other = ctx->saved_data["rejected_len"].toInt();
     auto [gc, gr] = op.call(s[0], g[0], opt(s[1]), opt(s[2]), ctx->saved_data["len"].toInt(), other < 0 ? 0 : other,
