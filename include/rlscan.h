@@ -295,7 +295,7 @@ int rls_segment_compose(const float* summaries, int rank, int world, int backwar
  * not zero.  A step that does not count has log-probability, entropy and
  * gradient 0, and its logits, token and other inputs are not used.  A token
  * outside [0, vocab) at a step that counts gives NaN there (and in the loss).
- * Logits may be -inf.  All other floating arrays are fp32, contiguous.       */
+ * Logits may be -inf; vocab is at most 2^31 - 256.  All other floating arrays are fp32, contiguous.       */
 #define RLS_MASK_NONE 0
 #define RLS_MASK_U8   1   /* bool or any 8-bit integer */
 #define RLS_MASK_F32  2
@@ -311,7 +311,7 @@ int rls_segment_compose(const float* summaries, int rank, int world, int backwar
 #define RLS_SHORT_VOCAB 1024
 int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
                        const void* mask, int mask_kind, float* logprobs, float* entropy, float* row_stats,
-                       int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature, int in_dtype,
+                       int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature, int in_dtype,
                        void* stream);
 
 /* grad_logits[n, t, v] = (grad_logprobs (1[v = token] - p_v)
@@ -323,7 +323,7 @@ int rls_token_logprobs_backward(const void* logits, int64_t env_stride, int64_t 
                                 const void* mask, int mask_kind, const float* row_stats,
                                 const float* grad_logprobs, const float* grad_entropy, void* grad_logits,
                                 int64_t grad_env_stride, int64_t grad_step_stride, int64_t num_envs,
-                                int64_t seq_len, int64_t vocab, float temperature, int in_dtype, void* stream);
+                                int64_t seq_len, int64_t vocab, double temperature, int in_dtype, void* stream);
 
 /* The clipped policy loss.  With r = exp(logprob - old_logprob):
  *   term = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A),
@@ -382,7 +382,7 @@ int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_
                            const float* ref_logprobs, const void* mask, int mask_kind, const rls_policy_t* policy,
                            float grad_scale, float* norm, float* logprobs, float* entropy, float* row_stats,
                            float* loss, float* stats, void* grad_logits, int64_t grad_env_stride,
-                           int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature, int in_dtype,
+                           int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature, int in_dtype,
                            void* ws, size_t ws_bytes, void* stream);
 int rls_policy_loss_logits_backward(const void* logits, int64_t env_stride, int64_t step_stride,
                                     const int64_t* tokens, const float* old_logprobs, const float* advantages,
@@ -391,7 +391,7 @@ int rls_policy_loss_logits_backward(const void* logits, int64_t env_stride, int6
                                     const float* grad_loss, int force, const float* norm,
                                     const float* row_stats, void* grad_logits, int64_t grad_env_stride,
                                     int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab,
-                                    float temperature, int in_dtype, void* stream);
+                                    double temperature, int in_dtype, void* stream);
 
 /* The paired preference loss over the log-probabilities of `pairs` responses
  * preferred (chosen [pairs, chosen_len]) and not (rejected [pairs,

@@ -7,7 +7,7 @@
 //   d logprob / d x_v = (1[v = tok] - p_v) / temperature,
 //   d H / d x_v       = -p_v (log p_v + H) / temperature.
 // Everything is computed in base 2: with c = log2(e) / temperature and an
-// offset M (the running maximum times c, rounded),
+// offset M (the running maximum times c, rounded to a whole number),
 //   d_v = x_v c - M,  S0 = sum 2^d_v,  S1 = sum 2^d_v d_v,  t = S1 / S0,
 //   logprob = ln2 (d_tok - log2 S0),   H = ln2 (log2 S0 - t),
 // one fused multiply-add and one ex2 an element, and the gradient for incoming
@@ -41,6 +41,39 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 lanes in one instruction.
+struct F2 {
+  unsigned long long u;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.u) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void split(F2 a, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.u));
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 ex2(F2 a) {
+  float x, y;
+  split(a, x, y);
+  return f2(ex2(x), ex2(y));
+}
+
 // ---- mask ------------------------------------------------------------------
 // One element a step, any of the types below; non-zero counts (NaN too).
 struct Mask {
@@ -60,23 +93,46 @@ __device__ __forceinline__ bool mask_at(const Mask& m, int64_t i) {
 }
 
 // ---- rows ------------------------------------------------------------------
+// row / seq by a multiplication, for rows below 2^31 (else by a division):
+// q = (umulhi(n, mul) + n) >> shift, shift = ceil(log2 seq),
+// mul = ceil(2^(32 + shift) / seq) - 2^32.
+struct Divide {
+  int64_t by;
+  unsigned mul, shift;
+  bool wide;
+  __host__ static Divide of(int64_t by, int64_t most) {
+    Divide d{by, 0, 0, most > 0x7fffffffLL || by > 0x7fffffffLL};
+    if (d.wide) return d;
+    while ((1LL << d.shift) < by) ++d.shift;
+    const unsigned long long two = 1ull << (32 + d.shift);
+    d.mul = (unsigned)((two + (unsigned long long)by - 1) / (unsigned long long)by - (1ull << 32));
+    return d;
+  }
+  __device__ __forceinline__ int64_t operator()(int64_t n) const {
+    if (wide) return n / by;
+    const unsigned m = (unsigned)n;
+    return (int64_t)((__umulhi(m, mul) + m) >> shift);
+  }
+};
+
 template <class T>
 struct Rows {
   const T* x;          // logits
   int64_t es, ss;      // strides of env and step in elements
   int64_t rows, seq;   // rows = envs * seq
-  int64_t V;
+  Divide env;          // a row's env
+  int V;
   const int64_t* tokens;
   Mask mask;
   float c;             // log2(e) / temperature, rounded
-  double c64;          // the same, not
+  double c64, c_off;   // the same, not rounded; c64 / c - 1
   float inv_temp;
   bool flat;           // es == seq * ss
 
   __device__ __forceinline__ int64_t at(int64_t row) const {
     if (flat) return row * ss;
-    const int64_t env = row / seq;
-    return env * es + (row - env * seq) * ss;
+    const int64_t e = env(row);
+    return e * es + (row - e * seq) * ss;
   }
 };
 
@@ -85,10 +141,10 @@ struct GradRows {
   T* g;
   int64_t es, ss;
   bool flat;
-  __device__ __forceinline__ int64_t at(int64_t row, int64_t seq) const {
+  __device__ __forceinline__ int64_t at(int64_t row, const Rows<T>& in) const {
     if (flat) return row * ss;
-    const int64_t env = row / seq;
-    return env * es + (row - env * seq) * ss;
+    const int64_t e = in.env(row);
+    return e * es + (row - e * in.seq) * ss;
   }
 };
 
@@ -117,8 +173,11 @@ struct Shift {
   bool far;
   __device__ __forceinline__ float operator()(float x) const { return far ? (x - off) * c : fmaf(x, c, -off); }
 };
+// What d is taken from: m c to a whole number.  Sums move to a larger offset by a
+// power of two then, exactly (ex2.approx of a whole number is one).
+__device__ __forceinline__ float offset_of(float m, float c) { return rintf(m * c); }
 __device__ __forceinline__ Shift shift_of(const RowStats& r, float c) {
-  return Shift{c, r.far ? r.m : r.m * c, r.far};
+  return Shift{c, r.far ? r.m : offset_of(r.m, c), r.far};
 }
 
 __device__ __forceinline__ double log2_of(float s0) {
@@ -132,13 +191,13 @@ __device__ __forceinline__ double log2_of(float s0) {
 // all rows are taken out to first order, since sums of many log-probabilities
 // (the preference loss's) would add them up: c was rounded, which moves log S0 by
 // the mean of d times the relative error; and ex2.approx lies 5.0e-8 low on
-// average (measured over d in (-8, 0)), except at the maximum, where d is 0.
-__device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c, double c64) {
+// average (measured over d in (-8, 0)), except at the far form's maximum, where d is 0.
+__device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c, double c64, double c_off) {
   const Shift sh = shift_of(r, c);
   if (ex2(sh(x_tok)) == r.s0) return 0.0;  // the others are below fp32's reach
   const double res = r.far ? 0.0 : (double)r.m * (double)c - (double)sh.off;  // d at the maximum
-  const double log_s0 = log2_of(r.s0) - res + (c64 / (double)c - 1.0) * ((double)r.t - res)
-                        + 7.2e-8 * (double)(1.f - __frcp_rn(r.s0));
+  const double low = r.far ? 7.2e-8 * (double)(1.f - __frcp_rn(r.s0)) : 7.2e-8;
+  const double log_s0 = log2_of(r.s0) - res + c_off * ((double)r.t - res) + low;
   return (((double)x_tok - (double)r.m) * c64 - log_s0) * 0.693147180559945309417;
 }
 __device__ __forceinline__ float entropy_of(const RowStats& r) {
@@ -148,12 +207,18 @@ __device__ __forceinline__ float entropy_of(const RowStats& r) {
 
 // The gradient's coefficients for incoming (a, b) of (logprob, entropy).
 struct RowGrad {
-  float a;     // added at the token
-  float A, B;  // 2^d (A + B d) is subtracted everywhere
+  float A, B;  // -2^d (A + B d), and at the token token_grad() instead
 };
 __device__ __forceinline__ RowGrad row_grad(float a, float b, const RowStats& r, float inv_temp) {
   const float k = inv_temp / r.s0, bl = b * kLn2;
-  return RowGrad{a * inv_temp, (a - bl * r.t) * k, bl * k};
+  return RowGrad{(a - bl * r.t) * k, bl * k};
+}
+// At the token, from 1 - p with a p that is 1 where the token is all there is.
+__device__ __forceinline__ float token_grad(float x, const Shift& sh, float a, float b, float s0, float t,
+                                            float inv_temp) {
+  const float d = sh(x);
+  const float p = ex2(d) / s0;
+  return inv_temp * (a * (1.f - p) - b * kLn2 * p * (fmaxf(d, kDeep) - t));
 }
 template <bool ENT>
 __device__ __forceinline__ float grad_at(float x, const Shift& sh, const RowGrad& g) {
@@ -175,6 +240,32 @@ struct Vec<float> {
   }
   __device__ __forceinline__ static uint4 pack(const float (&f)[4]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  // -inf becomes finite (and as good as -inf); NaN stays.
+  __device__ __forceinline__ static uint4 bound(const uint4& u) {
+    uint4 o;
+    constexpr unsigned low = 0xfb800000u;  // -2^120
+    asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.x) : "r"(u.x), "r"(low));
+    asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.y) : "r"(u.y), "r"(low));
+    asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.z) : "r"(u.z), "r"(low));
+    asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.w) : "r"(u.w), "r"(low));
+    return o;
+  }
+  __device__ __forceinline__ static float top(const uint4& u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  __device__ __forceinline__ static F2 pair(const uint4& u, int k) {
+    return k == 0 ? f2(__uint_as_float(u.x), __uint_as_float(u.y)) : f2(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  __device__ __forceinline__ static uint4 join(const F2 (&g)[2]) {
+    float f[4];
+    split(g[0], f[0], f[1]);
+    split(g[1], f[2], f[3]);
+    return pack(f);
+  }
+  // The vector's elements, one store each.
+  __device__ __forceinline__ static void scatter(float* p, const uint4& u) {
+    p[0] = __uint_as_float(u.x); p[1] = __uint_as_float(u.y); p[2] = __uint_as_float(u.z); p[3] = __uint_as_float(u.w);
   }
   __device__ __forceinline__ static float get(const float* p) { return *p; }
   __device__ __forceinline__ static float put(float v) { return v; }
@@ -201,20 +292,57 @@ struct Vec<__nv_bfloat16> {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  __device__ __forceinline__ static unsigned max2(unsigned a, unsigned b) {
+    unsigned o;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(o) : "r"(a), "r"(b));
+    return o;
+  }
+  __device__ __forceinline__ static uint4 bound(const uint4& u) {
+    uint4 o;
+    constexpr unsigned low = 0xfb80fb80u;  // -2^120
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.x) : "r"(u.x), "r"(low));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.y) : "r"(u.y), "r"(low));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.z) : "r"(u.z), "r"(low));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.w) : "r"(u.w), "r"(low));
+    return o;
+  }
+  __device__ __forceinline__ static float top(const uint4& u) {
+    const unsigned m = max2(max2(u.x, u.y), max2(u.z, u.w));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  __device__ __forceinline__ static F2 pair(const uint4& u, int k) {
+    const unsigned w = k == 0 ? u.x : k == 1 ? u.y : k == 2 ? u.z : u.w;
+    return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  __device__ __forceinline__ static uint4 join(const F2 (&g)[4]) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split(g[k], f[2 * k], f[2 * k + 1]);
+    return pack(f);
+  }
+  __device__ __forceinline__ static void scatter(__nv_bfloat16* p, const uint4& u) {
+    unsigned short* h = reinterpret_cast<unsigned short*>(p);
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[2 * k] = (unsigned short)(w[k] & 0xffffu);
+      h[2 * k + 1] = (unsigned short)(w[k] >> 16);
+    }
+  }
   __device__ __forceinline__ static float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   __device__ __forceinline__ static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 
 // A row cut at 16-byte boundaries: `head` elements, `nvec` vectors, `tail`.
 struct Cut {
-  int64_t head, nvec, tail;
+  int head, nvec, tail;
 };
 template <class T>
-__device__ __forceinline__ Cut cut_row(const T* p, int64_t V) {
+__device__ __forceinline__ Cut cut_row(const T* p, int V) {
   constexpr int N = Vec<T>::N;
-  int64_t head = (int64_t)((16 - ((uintptr_t)p & 15)) & 15) / (int64_t)sizeof(T);
+  int head = (int)((16u - (unsigned)((uintptr_t)p & 15)) & 15u) / (int)sizeof(T);
   if (head > V) head = V;
-  const int64_t nvec = (V - head) / N;
+  const int nvec = (int)((unsigned)(V - head) / (unsigned)N);
   return Cut{head, nvec, V - head - nvec * N};
 }
 
@@ -227,10 +355,10 @@ __device__ __forceinline__ Cut cut_row(const T* p, int64_t V) {
 template <bool ENT>
 struct Run {
   float m = -kFar, off, s0 = 0.f, s1 = 0.f;
-  __device__ __forceinline__ explicit Run(float c) : off(-kFar * c) {}
+  __device__ __forceinline__ explicit Run(float c) : off(offset_of(-kFar, c)) {}
   // Moves to a larger maximum.
   __device__ __forceinline__ void raise(float mx, float c) {
-    const float to = mx * c, by = off - to;
+    const float to = offset_of(mx, c), by = off - to;
     const float k = ex2(by);
     s1 = fmaf(s0, fmaxf(by, kDeep), s1) * k;
     s0 *= k;
@@ -256,6 +384,41 @@ struct Run {
       for (int k = 0; k + w < K; k += 2 * w) e[k] += e[k + w];
     s0 += e[0];
     if constexpr (!ENT) s1 = fmaf(e[0], fmaxf(fmaf(mx, c, -off), kDeep), s1);
+  }
+  // M whole vectors at once.
+  template <class T, int M>
+  __device__ __forceinline__ void add_vectors(uint4 (&u)[M], float c) {
+    constexpr int P = Vec<T>::N / 2;
+    if constexpr (ENT) {
+#pragma unroll
+      for (int k = 0; k < M; ++k) u[k] = Vec<T>::bound(u[k]);
+    }
+    float mx = Vec<T>::top(u[0]);
+#pragma unroll
+    for (int k = 1; k < M; ++k) mx = fmaxf(mx, Vec<T>::top(u[k]));
+    if (mx > m) raise(mx, c);
+    const F2 cc = f2(c, c), no = f2(-off, -off);
+    F2 sum, by;
+#pragma unroll
+    for (int k = 0; k < M; ++k)
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const F2 d = fma2(Vec<T>::pair(u[k], q), cc, no);
+        const F2 e = ex2(d);
+        const bool first = k == 0 && q == 0;
+        sum = first ? e : add2(sum, e);
+        if constexpr (ENT) by = first ? mul2(e, d) : fma2(e, d, by);
+      }
+    float x, y;
+    split(sum, x, y);
+    x += y;
+    s0 += x;
+    if constexpr (ENT) {
+      split(by, x, y);
+      s1 += x + y;
+    } else {
+      s1 = fmaf(x, fmaxf(fmaf(mx, c, -off), kDeep), s1);
+    }
   }
   __device__ __forceinline__ void join(float om, float ooff, float os0, float os1) {
     const bool up = om > m;
@@ -318,8 +481,10 @@ struct PolicyTerm {
 __device__ __forceinline__ PolicyTerm policy_term(const Policy& p, double lp, float old_lp, float adv, float ref) {
   PolicyTerm o;
   const double lr64 = lp - (double)old_lp;
-  const float lr = (float)lr64;
-  const float gain = expf(lr) * adv;
+  const float lr = (float)lr64, lr_low = (float)(lr64 - (double)lr);  // the part that fp32 drops
+  float gain = expf(lr);
+  if (gain < INFINITY) gain = fmaf(gain, lr_low, gain);
+  gain *= adv;
   o.loss = -gain;
   o.d = -gain;
   o.clipped = false;
@@ -333,11 +498,17 @@ __device__ __forceinline__ PolicyTerm policy_term(const Policy& p, double lp, fl
   o.drift = expm1f(lr) - lr;
   o.kl = 0.f;
   if (p.ref) {
-    const float x = (float)((double)ref - lp);
+    const double x64 = (double)ref - lp;
+    const float x = (float)x64, x_low = (float)(x64 - (double)x);
     float dk;
     if (p.kl_kind == RLS_KL_K1) { o.kl = -x; dk = 1.f; }
     else if (p.kl_kind == RLS_KL_K2) { o.kl = 0.5f * x * x; dk = -x; }
-    else { const float e = expm1f(x); o.kl = e - x; dk = -e; }
+    else {
+      float e = expm1f(x);
+      if (fabsf(x) < INFINITY) e = fmaf(e + 1.f, x_low, e);
+      o.kl = e - x;
+      dk = -e;
+    }
     if (p.kl_coef != 0.f) {
       o.loss = fmaf(p.kl_coef, o.kl, o.loss);
       o.d = fmaf(p.kl_coef, dk, o.d);
@@ -476,7 +647,7 @@ __device__ __forceinline__ float block_sum(float v) {
 
 // The far form: two plain passes, the true maximum first.
 template <class T, bool ENT, int NT>
-__device__ __noinline__ RowStats far_stats(const T* x, int64_t V, float c) {
+__device__ __noinline__ RowStats far_stats(const T* x, int V, float c) {
   float m = -INFINITY;
   for (int64_t v = threadIdx.x; v < V; v += NT) m = fmaxf(m, Vec<T>::get(x + v));
   m = block_max<NT>(m);
@@ -493,7 +664,7 @@ __device__ __noinline__ RowStats far_stats(const T* x, int64_t V, float c) {
 }
 
 template <class T, bool ENT, int NT, int U>
-__device__ __forceinline__ RowStats row_stats(const T* x, int64_t V, float c) {
+__device__ __forceinline__ RowStats row_stats(const T* x, int V, float c) {
   constexpr int N = Vec<T>::N;
   const Cut cut = cut_row(x, V);
   Run<ENT> run(c);
@@ -513,29 +684,34 @@ __device__ __forceinline__ RowStats row_stats(const T* x, int64_t V, float c) {
       run.add(f, c);
     }
   }
-  const int64_t ends = cut.head + cut.tail;
-  if (threadIdx.x < ends) {
-    const int64_t i = threadIdx.x < cut.head ? threadIdx.x : V - ends + threadIdx.x;
+  const int ends = cut.head + cut.tail;
+  if ((int)threadIdx.x < ends) {
+    const int64_t i = (int)threadIdx.x < cut.head ? (int)threadIdx.x : V - ends + (int)threadIdx.x;
     const float f[1] = {Vec<T>::get(x + i)};
     run.add(f, c);
   }
   block_join<ENT, NT>(run, c);
   if (!(run.s0 >= kLeast && run.s0 <= kMost)) return far_stats<T, ENT, NT>(x, V, c);
   const float d = fmaf(run.m, c, -run.off), e = ex2(d);
-  return RowStats{run.m, run.s0, run.s1 / run.s0, false, ENT && run.s0 == e && run.s1 == e * d};
+  const bool alone = ENT && run.s0 == e && run.s1 == e * d;
+  return RowStats{run.m, run.s0, alone ? d : run.s1 / run.s0, false, alone};
 }
 
 template <class T, int NT>
-__device__ __forceinline__ void zero_row(T* g, int64_t V) {
+__device__ __forceinline__ void zero_row(T* g, int V) {
   const Cut cut = cut_row(g, V);
   uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
   for (int64_t v = threadIdx.x; v < cut.nvec; v += NT) __stcs(gv + v, make_uint4(0, 0, 0, 0));
-  const int64_t ends = cut.head + cut.tail;
-  if (threadIdx.x < ends) g[threadIdx.x < cut.head ? threadIdx.x : V - ends + threadIdx.x] = Vec<T>::put(0.f);
+  const int ends = cut.head + cut.tail;
+  if ((int)threadIdx.x < ends) g[(int)threadIdx.x < cut.head ? (int)threadIdx.x : V - ends + (int)threadIdx.x] = Vec<T>::put(0.f);
 }
 
 template <class T, bool ENT, int NT, int U>
-__device__ __forceinline__ void grad_row(const T* x, T* g, int64_t V, int64_t tok, const Shift& sh, const RowGrad& rg) {
+__device__ __forceinline__ void grad_row(const T* x, T* g, int V, int64_t tok, const RowStats& r, float a, float b,
+                                         float c, float inv_temp) {
+  const Shift sh = shift_of(r, c);
+  const RowGrad rg = row_grad(a, b, r, inv_temp);
+  auto at_token = [&](float y) { return token_grad(y, sh, a, b, r.s0, r.t, inv_temp); };
   constexpr int N = Vec<T>::N;
   const Cut cut = cut_row(x, V);
   const bool same = (((uintptr_t)x ^ (uintptr_t)g) & 15) == 0;
@@ -555,12 +731,7 @@ __device__ __forceinline__ void grad_row(const T* x, T* g, int64_t V, int64_t to
       Vec<T>::unpack(u[k], f);
       const int64_t i0 = cut.head + v * N;
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = grad_at<ENT>(f[e], sh, rg);
-      if (tok >= i0 && tok < i0 + N) {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (tok == i0 + e) f[e] += rg.a;
-      }
+      for (int e = 0; e < N; ++e) f[e] = i0 + e == tok ? at_token(f[e]) : grad_at<ENT>(f[e], sh, rg);
       if (same) {
         __stcs(reinterpret_cast<uint4*>(g + i0), Vec<T>::pack(f));
       } else {
@@ -569,12 +740,11 @@ __device__ __forceinline__ void grad_row(const T* x, T* g, int64_t V, int64_t to
       }
     }
   }
-  const int64_t ends = cut.head + cut.tail;
-  if (threadIdx.x < ends) {
-    const int64_t i = threadIdx.x < cut.head ? threadIdx.x : V - ends + threadIdx.x;
-    float f = grad_at<ENT>(Vec<T>::get(x + i), sh, rg);
-    if (i == tok) f += rg.a;
-    g[i] = Vec<T>::put(f);
+  const int ends = cut.head + cut.tail;
+  if ((int)threadIdx.x < ends) {
+    const int64_t i = (int)threadIdx.x < cut.head ? (int)threadIdx.x : V - ends + (int)threadIdx.x;
+    const float f = Vec<T>::get(x + i);
+    g[i] = Vec<T>::put(i == tok ? at_token(f) : grad_at<ENT>(f, sh, rg));
   }
 }
 
@@ -592,7 +762,7 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
   }
   for (int64_t row = blockIdx.x; row < in.rows; row += gridDim.x) {
     const T* x = in.x + in.at(row);
-    T* g = MODE == kFwd || !gr.g ? nullptr : gr.g + gr.at(row, in.seq);
+    T* g = MODE == kFwd || !gr.g ? nullptr : gr.g + gr.at(row, in);
     if (!mask_at(in.mask, row)) {
       if constexpr (MODE != kBwd) {
         if (threadIdx.x == 0) {
@@ -611,12 +781,12 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
     if constexpr (MODE != kBwd) {
       const float xt = ok ? Vec<T>::get(x + tok) : NAN;
       r = row_stats<T, ENT, NT, U>(x, in.V, in.c);
-      const double lp = logprob_of(xt, r, in.c, in.c64);
+      const double lp = logprob_of(xt, r, in.c, in.c64, in.c_off);
       float ent = 0.f;
       if constexpr (ENT) ent = entropy_of(r);
       int flags = kFlagKept;
       if constexpr (Src::kPolicy) {
-        const int64_t env = row / in.seq;
+        const int64_t env = in.env(row);
         const Policy& p = src.p;
         const PolicyTerm o = policy_term(p, lp, p.old_lp[row], p.adv[p.adv_row ? env : row], p.ref ? p.ref[row] : 0.f);
         const float w = policy_weight(p, env);
@@ -637,7 +807,7 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
       r = stats_of(out.stats[2 * row]);
       if constexpr (Src::kPolicy) {
         a = out.stats[2 * row + 1].x;
-        if constexpr (ENT) b = -policy_weight(src.p, row / in.seq) * src.p.ent_coef;
+        if constexpr (ENT) b = -policy_weight(src.p, in.env(row)) * src.p.ent_coef;
       } else {
         a = src.g_lp ? src.g_lp[row] : 0.f;
         if constexpr (ENT) b = src.g_ent[row];
@@ -647,20 +817,18 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
       if constexpr (Src::kPolicy) { a *= src.up(); b *= src.up(); }
       if (!ok) a = NAN;
       if (a == 0.f && b == 0.f) zero_row<T, NT>(g, in.V);
-      else grad_row<T, ENT, NT, U>(x, g, in.V, tok, shift_of(r, in.c), row_grad(a, b, r, in.inv_temp));
+      else grad_row<T, ENT, NT, U>(x, g, in.V, tok, r, a, b, in.c, in.inv_temp);
     }
   }
 }
 
-// ---- long rows: a pipeline over rows --------------------------------------------
-// C CTAs (a cluster) of NT threads share a row: each CTA takes one stretch of its 16-byte
-// vectors, each thread every NT-th vector of the stretch, at most K, in slots of
-// shared memory that no other thread reads.  So the copies (cp.async, all K of a
-// row in flight at once) need no barrier, only the thread's own wait; the one
-// barrier a row is the join of the statistics.  A slot is refilled from the next row as
-// soon as its last use is over: in the forward call when its elements are added
-// up, with a gradient when the gradient is stored, so that the next row's loads
-// are in flight during this row's stores and reductions.
+// ---- long rows ------------------------------------------------------------------
+// A team of 1 to 8 CTAs (a cluster) of NT threads works on one row at a time; each
+// CTA takes one stretch of the row's 16-byte vectors, each thread every NT-th vector
+// of the stretch.  What a vector was read into (registers, or a slot of shared
+// memory that no other thread reads) is refilled with a later one, of the next row at
+// the end of a row, as soon as its last use is over: so loads are always in flight, across the
+// row's one barrier (the join of the statistics) too.
 __device__ __forceinline__ void copy16(uint4* to, const uint4* from) {
   const unsigned at = (unsigned)__cvta_generic_to_shared(to);
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
@@ -668,6 +836,13 @@ __device__ __forceinline__ void copy16(uint4* to, const uint4* from) {
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// The same for a number that unrolling makes constant, at most N.
+template <int N>
+__device__ __forceinline__ void copy_wait_upto(int n) {
+  if constexpr (N == 0) copy_wait<0>();
+  else if (n == N) copy_wait<N>();
+  else copy_wait_upto<N - 1>(n);
+}
 
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
@@ -719,18 +894,24 @@ __device__ __forceinline__ const float4* exchange(Table<NT, CL>& t, unsigned& tu
   return tab;
 }
 
-// Joins (m, s0, s1) over a warp: to the common maximum first, then plain sums.
-__device__ __forceinline__ void warp_gather(float& m, float& s0, float& s1, float c) {
+// Joins (m, s0, s1) over groups of WIDTH lanes: to the common maximum first, then
+// plain sums.
+template <int WIDTH>
+__device__ __forceinline__ void gather(float& m, float& s0, float& s1, float c) {
   float top = m;
+  if constexpr (WIDTH == 32) {
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(m));
+  } else {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float by = m * c - top * c;
+    for (int o = WIDTH / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  const float by = offset_of(m, c) - offset_of(top, c);
   const float k = ex2(by);
   s1 = fmaf(s0, fmaxf(by, kDeep), s1) * k;
   s0 *= k;
   m = top;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = WIDTH / 2; o > 0; o >>= 1) {
     s0 += __shfl_xor_sync(0xffffffffu, s0, o);
     s1 += __shfl_xor_sync(0xffffffffu, s1, o);
   }
@@ -739,53 +920,51 @@ __device__ __forceinline__ void warp_gather(float& m, float& s0, float& s1, floa
 __device__ __forceinline__ float incoming_entropy(const PolicyGrad& s, float w, float) { return -w * s.p.ent_coef; }
 __device__ __forceinline__ float incoming_entropy(const GivenGrad&, float, float b) { return b; }
 
-template <class T, bool ENT, int MODE, class Src, int NT, int K, bool CL>
-__global__ void __launch_bounds__(NT, 768 / NT) pipe_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src) {
-  if constexpr (Src::kPolicy && MODE == kBwd) {
-    if (src.skip()) return;
-  }
-  constexpr int N = Vec<T>::N;
-  constexpr bool kGrad = MODE != kFwd;
-  extern __shared__ uint4 slots[];  // [K][NT]
-  __shared__ Table<NT, CL> table;
-  unsigned turn = 0;
-  const int tid = threadIdx.x, lane = tid & 31;
+// The rows of a team, in order, and what its CTA and threads have of each.
+template <class T, bool ENT, int MODE, class Src, int NT, bool CL>
+struct Walk {
+  static constexpr int N = Vec<T>::N;
+  const Rows<T>& in;
+  const RowOut& out;
+  const GradRows<T>& gr;
+  const Src& src;
+  const int tid = threadIdx.x;
   const unsigned rank = CL ? cluster_rank() : 0, size = CL ? cluster_size() : 1;
-  const int64_t team = blockIdx.x / size, teams = gridDim.x / size;
-  uint4* mine = slots + tid;
-  const float c = in.c;
-
-  // The rows of this team in order: `window` says which of the next 32 are to be
-  // worked on; the others only get their zeros.
-  int64_t next_row = team;
-  unsigned window = 0;
+  const int log_size = !CL || size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3;  // sizes are powers of two
+  const int64_t teams = gridDim.x >> log_size;
+  int64_t next_row = blockIdx.x >> log_size;
+  unsigned window = 0;  // which of the next 32 rows are to be worked on; the others only get their zeros
   int left = 0;
-  auto wanted = [&](int64_t row) -> bool {
+
+  __device__ __forceinline__ Walk(const Rows<T>& i, const RowOut& o, const GradRows<T>& g, const Src& s)
+      : in(i), out(o), gr(g), src(s) {}
+
+  __device__ __forceinline__ bool wanted(int64_t row) const {
     if (row >= in.rows || !mask_at(in.mask, row)) return false;
     if constexpr (MODE == kBwd && Src::kPolicy) return ENT || out.stats[2 * row + 1].x != 0.f;
     if constexpr (MODE == kBwd && !Src::kPolicy) {
-      const float a = src.g_lp ? src.g_lp[row] : 0.f;
-      bool some = a != 0.f;
+      bool some = src.g_lp && src.g_lp[row] != 0.f;
       if constexpr (ENT) some = some || src.g_ent[row] != 0.f;
       return some;
     }
     return true;
-  };
-  auto zeros = [&](int64_t row) {
-    T* g = gr.g + gr.at(row, in.seq);
+  }
+  __device__ __forceinline__ void zeros(int64_t row) const {
+    T* g = gr.g + gr.at(row, in);
     const Cut cut = cut_row(g, in.V);
-    const int64_t per = (cut.nvec + size - 1) / size, v0 = per * rank;
-    const int64_t v1 = v0 + per < cut.nvec ? v0 + per : cut.nvec;
-    uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
-    for (int64_t v = v0 + tid; v < v1; v += NT) __stcs(gv + v, make_uint4(0, 0, 0, 0));
-    const int64_t ends = cut.head + cut.tail;
-    if (rank == 0 && tid < ends) g[tid < cut.head ? tid : in.V - ends + tid] = Vec<T>::put(0.f);
-  };
-  auto advance = [&]() -> int64_t {
+    int v0;
+    const int n = stretch(cut, v0);
+    uint4* gv = reinterpret_cast<uint4*>(g + cut.head) + v0;
+    for (int v = tid; v < n; v += NT) __stcs(gv + v, make_uint4(0, 0, 0, 0));
+    const int ends = ends_of(cut);
+    if (tid < ends) g[tid < cut.head ? tid : in.V - ends + tid] = Vec<T>::put(0.f);
+  }
+  // The next row to work on, or -1; the same in all threads of the team.
+  __device__ __forceinline__ int64_t advance() {
     for (;;) {
       if (next_row >= in.rows) return -1;
       if (left == 0) {
-        window = __ballot_sync(0xffffffffu, wanted(next_row + lane * teams));
+        window = __ballot_sync(0xffffffffu, wanted(next_row + (tid & 31) * teams));
         left = 32;
       }
       const bool yes = window & 1u;
@@ -801,40 +980,55 @@ __global__ void __launch_bounds__(NT, 768 / NT) pipe_rows_kernel(Rows<T> in, Row
           if (out.stats) out.stats[2 * row] = out.stats[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
-      if (kGrad && gr.g) zeros(row);
+      if (MODE != kFwd && gr.g) zeros(row);
     }
-  };
+  }
+  __device__ __forceinline__ const T* row_at(int64_t row) const { return in.x + in.at(row); }
+  // The CTA's stretch begins v0 vectors into the row and has as many.
+  __device__ __forceinline__ int stretch(const Cut& cut, int& v0) const {
+    if constexpr (!CL) {
+      v0 = 0;
+      return cut.nvec;
+    }
+    const int per = (cut.nvec + (int)size - 1) >> log_size;
+    v0 = per * (int)rank;
+    const int n = cut.nvec - v0;
+    return n < 0 ? 0 : n < per ? n : per;
+  }
+  // Vectors a CTA has of any row, at most.
+  __device__ __forceinline__ int most() const {
+    return ((in.V + N - 1) / N + (int)size - 1) >> log_size;
+  }
 
-  // A row's place: its vectors from v0 on are this CTA's, `mid` of them.
   struct Place {
-    int64_t row, tok;
-    const T* x;
-    int head, ends;   // elements before the first vector; those and the ones after the last
-    int64_t v0;
-    int mid;
-    bool ok;
-    float end, xt;    // the thread's end element; the token's logit
+    int64_t row;
+    const uint4* at;  // this thread's first vector
+    int mid;          // vectors from there to the end of the stretch (every NT-th is the thread's)
+  };
+  __device__ __forceinline__ Place place(int64_t row) const {
+    const T* x = row_at(row);
+    const Cut cut = cut_row(x, in.V);
+    int v0;
+    const int n = stretch(cut, v0);
+    return Place{row, reinterpret_cast<const uint4*>(x + cut.head) + v0 + tid, n - tid};
+  }
+  // What the row's one-off steps need, asked for a row ahead.
+  struct Extra {
+    int64_t tok;
+    float end, xt;              // the thread's end element; the token's logit
     float old_lp, adv, ref, w;  // the policy loss's inputs
-    float a, b;       // incoming gradients of a backward call
+    float a, b;                 // incoming gradients of a backward call
     float4 stats;
   };
-  const int64_t V = in.V;
-  auto place = [&](int64_t row) -> Place {
-    Place p;
-    p.row = row;
-    p.x = in.x + in.at(row);
-    const Cut cut = cut_row(p.x, V);
-    p.head = (int)cut.head;
-    p.ends = rank == 0 ? (int)(cut.head + cut.tail) : 0;
-    const int64_t per = (cut.nvec + size - 1) / size;
-    p.v0 = per * rank;
-    const int64_t n = cut.nvec - p.v0;
-    p.mid = (int)(n < 0 ? 0 : n < per ? n : per);
+  __device__ __forceinline__ Extra extra(int64_t row) const {
+    Extra p;
+    const T* x = row_at(row);
+    const Cut cut = cut_row(x, in.V);
+    const int ends = ends_of(cut);
     p.tok = in.tokens[row];
-    p.ok = p.tok >= 0 && p.tok < V;
-    p.end = tid < p.ends ? Vec<T>::get(p.x + (tid < p.head ? tid : V - (cut.head + cut.tail) + tid)) : 0.f;
+    p.end = tid < ends ? Vec<T>::get(x + (tid < cut.head ? tid : in.V - ends + tid)) : 0.f;
     if constexpr (Src::kPolicy) {
-      const int64_t env = row / in.seq;
+      const int64_t env = in.env(row);
       p.w = policy_weight(src.p, env);
       if constexpr (MODE != kBwd) {
         p.old_lp = src.p.old_lp[row];
@@ -849,192 +1043,342 @@ __global__ void __launch_bounds__(NT, 768 / NT) pipe_rows_kernel(Rows<T> in, Row
       if constexpr (ENT && !Src::kPolicy) p.b = src.g_ent[row];
     }
     return p;
-  };
+  }
   // The token's logit, asked for once the token itself is there.
-  auto token_logit = [&](Place& p) {
-    if constexpr (MODE != kBwd) p.xt = p.ok ? Vec<T>::get(p.x + p.tok) : NAN;
-  };
-  auto fetch = [&](const Place& p, int j) {
-    if (p.row >= 0 && tid + j * NT < p.mid)
-      copy16(mine + j * NT, reinterpret_cast<const uint4*>(p.x + p.head) + p.v0 + tid + j * NT);
-    copy_commit();
-  };
+  __device__ __forceinline__ void token_logit(int64_t row, Extra& p) const {
+    p.xt = p.tok >= 0 && p.tok < in.V ? Vec<T>::get(row_at(row) + p.tok) : NAN;
+  }
+  // Elements outside the row's vectors: the first CTA's threads take one each.
+  __device__ __forceinline__ int ends_of(const Cut& cut) const { return rank == 0 ? (int)(cut.head + cut.tail) : 0; }
 
-  int64_t first = advance();
-  if (first < 0) return;  // the same for every CTA of the team
-  Place now = place(first);
-#pragma unroll
-  for (int j = 0; j < K; ++j) fetch(now, j);
-  token_logit(now);
-  if constexpr (CL && MODE != kBwd) cluster_barrier();  // the others' tables exist
-
-  for (;;) {
-    Place next;
-    next.row = -1;
-    // ---- statistics
-    RowStats r;
-    float a = 0.f, b = 0.f;
-    if constexpr (MODE != kBwd) {
-      if constexpr (MODE == kFwd) {
-        const int64_t row = advance();
-        if (row >= 0) next = place(row);
-      }
-      Run<ENT> run(c);
-#pragma unroll
-      for (int j = 0; j < K; ++j) {
-        if constexpr (MODE == kFwd) copy_wait<K - 1>();
-        else {
-          // slots j + 1 .. K - 1 may still be on their way
-          switch (K - 1 - j) {
-            case 0: copy_wait<0>(); break;   case 1: copy_wait<1>(); break;   case 2: copy_wait<2>(); break;
-            case 3: copy_wait<3>(); break;   case 4: copy_wait<4>(); break;   case 5: copy_wait<5>(); break;
-            case 6: copy_wait<6>(); break;   case 7: copy_wait<7>(); break;   case 8: copy_wait<8>(); break;
-            case 9: copy_wait<9>(); break;   case 10: copy_wait<10>(); break; case 11: copy_wait<11>(); break;
-            case 12: copy_wait<12>(); break; case 13: copy_wait<13>(); break; case 14: copy_wait<14>(); break;
-            default: copy_wait<15>(); break;
-          }
-        }
-        if (tid + j * NT < now.mid) {
-          float f[N];
-          Vec<T>::unpack(mine[j * NT], f);
-          run.add(f, c);
-        }
-        if constexpr (MODE == kFwd) fetch(next, j);
-      }
-      if (tid < now.ends) {
-        const float f[1] = {now.end};
-        run.add(f, c);
-      }
-      warp_gather(run.m, run.s0, run.s1, c);
-      {
-        const float4* tab = exchange(table, turn, make_float4(run.m, run.s0, run.s1, 0.f), rank, size);
-        const int n = size * (NT / 32);
+  // The statistics of the row from every thread's share (the vectors; the ends
+  // are added here); the same in all threads of the team.
+  __device__ __forceinline__ RowStats join(Run<ENT>& run, int64_t row, const Extra& ex, Table<NT, CL>& table,
+                                           unsigned& turn) const {
+    const int lane = tid & 31;
+    const float c = in.c;
+    const T* x = row_at(row);
+    const Cut cut = cut_row(x, in.V);
+    const int ends = ends_of(cut);
+    if (tid < ends) {
+      const float f[1] = {ex.end};
+      run.add(f, c);
+    }
+    gather<32>(run.m, run.s0, run.s1, c);
+    {
+      const float4* tab = exchange(table, turn, make_float4(run.m, run.s0, run.s1, 0.f), rank, size);
+      // every group of lanes reads all of the table
+      constexpr int kWarps = NT / 32;
+      if constexpr (!CL) {
+        const float4 q = tab[lane & (kWarps - 1)];
+        run.m = q.x; run.s0 = q.y; run.s1 = q.z;
+        gather<kWarps>(run.m, run.s0, run.s1, c);
+      } else {
+        const int n = (int)size * kWarps;
         float4 q = lane < n ? tab[lane] : make_float4(-kFar, 0.f, 0.f, 0.f);
-        if (CL && n > 32 && lane + 32 < n) {
+        if (lane + 32 < n) {
           const float4 q2 = tab[lane + 32];
           const float top = fmaxf(q.x, q2.x);
-          const float d0 = q.x * c - top * c, d1 = q2.x * c - top * c;
+          const float to = offset_of(top, c), d0 = offset_of(q.x, c) - to, d1 = offset_of(q2.x, c) - to;
           const float k0 = ex2(d0), k1 = ex2(d1);
           q.z = fmaf(q.y, fmaxf(d0, kDeep), q.z) * k0 + fmaf(q2.y, fmaxf(d1, kDeep), q2.z) * k1;
           q.y = q.y * k0 + q2.y * k1;
           q.x = top;
         }
-        warp_gather(q.x, q.y, q.z, c);
         run.m = q.x; run.s0 = q.y; run.s1 = q.z;
+        gather<32>(run.m, run.s0, run.s1, c);
       }
-      const float off = run.m * c, dm = fmaf(run.m, c, -off), em = ex2(dm);
-      r = RowStats{run.m, run.s0, run.s1 / run.s0, false, ENT && run.s0 == em && run.s1 == em * dm};
-      if (!(run.s0 >= kLeast && run.s0 <= kMost)) {  // the same in all threads of the team
-        // the far form, from global memory (the slots may hold the next row)
-        const T* xs = now.x + now.head + now.v0 * N;
-        const int64_t n = (int64_t)now.mid * N;
-        float m = tid < now.ends ? now.end : -INFINITY;
-        for (int64_t i = tid; i < n; i += NT) m = fmaxf(m, Vec<T>::get(xs + i));
+    }
+    if (run.s0 >= kLeast && run.s0 <= kMost) {
+      const float off = offset_of(run.m, c), dm = fmaf(run.m, c, -off), em = ex2(dm);
+      const bool alone = ENT && run.s0 == em && run.s1 == em * dm;
+      return RowStats{run.m, run.s0, alone ? dm : run.s1 / run.s0, false, alone};
+    }
+    // The far form, from global memory (what the row was read into may hold the
+    // next one).  All threads of the team come here or none.
+    int v0;
+    const int64_t n = (int64_t)stretch(cut, v0) * N;
+    const T* xs = x + cut.head + (int64_t)v0 * N;
+    float m = tid < ends ? ex.end : -INFINITY;
+    for (int64_t i = tid; i < n; i += NT) m = fmaxf(m, Vec<T>::get(xs + i));
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float4* tab = exchange(table, turn, make_float4(m, 0.f, 0.f, 0.f), rank, size);
-        for (int w = 0; w < (int)size * (NT / 32); ++w) m = fmaxf(m, tab[w].x);
-        float s0 = 0.f, s1 = 0.f;
-        auto add = [&](float x) {
-          const float d = (x - m) * c;
-          const float e = ex2(d);
-          s0 += e;
-          s1 = fmaf(e, fmaxf(d, kDeep), s1);
-        };
-        for (int64_t i = tid; i < n; i += NT) add(Vec<T>::get(xs + i));
-        if (tid < now.ends) add(now.end);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float4* tab = exchange(table, turn, make_float4(m, 0.f, 0.f, 0.f), rank, size);
+    for (int w = 0; w < (int)size * (NT / 32); ++w) m = fmaxf(m, tab[w].x);
+    float s0 = 0.f, s1 = 0.f;
+    auto add = [&](float y) {
+      const float d = (y - m) * c;
+      const float e = ex2(d);
+      s0 += e;
+      s1 = fmaf(e, fmaxf(d, kDeep), s1);
+    };
+    for (int64_t i = tid; i < n; i += NT) add(Vec<T>::get(xs + i));
+    if (tid < ends) add(ex.end);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-          s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-        }
-        tab = exchange(table, turn, make_float4(s0, s1, 0.f, 0.f), rank, size);
-        s0 = s1 = 0.f;
-        for (int w = 0; w < (int)size * (NT / 32); ++w) { s0 += tab[w].x; s1 += tab[w].y; }
-        r = RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f};
-      }
-      const double lp = logprob_of(now.xt, r, c, in.c64);
-      float ent = 0.f;
-      if constexpr (ENT) ent = entropy_of(r);
-      int flags = kFlagKept;
-      const bool writes = rank == 0 && tid == 0;
-      if constexpr (Src::kPolicy) {
-        const Policy& p = src.p;
-        const float w = now.w;
-        const PolicyTerm o = policy_term(p, lp, now.old_lp, now.adv, now.ref);
-        a = w * o.d;
-        if constexpr (ENT) b = -w * p.ent_coef;
-        if (o.clipped) flags |= kFlagClipped;
-        if (writes) {
-          const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
-          out.stats[2 * now.row + 1] = make_float4(a, w * term, o.kl, o.drift);
-        }
-      }
+    for (int o = 16; o > 0; o >>= 1) {
+      s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+    }
+    tab = exchange(table, turn, make_float4(s0, s1, 0.f, 0.f), rank, size);
+    s0 = s1 = 0.f;
+    for (int w = 0; w < (int)size * (NT / 32); ++w) { s0 += tab[w].x; s1 += tab[w].y; }
+    return RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f};
+  }
+
+  // Log-probability, entropy and, with the policy loss, the term and the row's
+  // incoming gradients before the scale; one warp of a CTA calls it.
+  __device__ __forceinline__ void outputs(int64_t row, const RowStats& r, const Extra& ex, float& a, float& b) const {
+    const double lp = logprob_of(ex.xt, r, in.c, in.c64, in.c_off);
+    float ent = 0.f;
+    if constexpr (ENT) ent = entropy_of(r);
+    int flags = kFlagKept;
+    const bool writes = rank == 0 && tid == 0;
+    if constexpr (Src::kPolicy) {
+      const Policy& p = src.p;
+      const PolicyTerm o = policy_term(p, lp, ex.old_lp, ex.adv, ex.ref);
+      a = ex.w * o.d;
+      b = ENT ? -ex.w * p.ent_coef : 0.f;
+      if (o.clipped) flags |= kFlagClipped;
       if (writes) {
-        out.logprob[now.row] = (float)lp;
-        if (out.entropy) out.entropy[now.row] = ent;
-        if (out.stats) out.stats[2 * now.row] = stats_word(r, flags);
+        const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
+        out.stats[2 * row + 1] = make_float4(a, ex.w * term, o.kl, o.drift);
+      }
+    }
+    if (writes) {
+      out.logprob[row] = (float)lp;
+      if (out.entropy) out.entropy[row] = ent;
+      if (out.stats) out.stats[2 * row] = stats_word(r, flags);
+    }
+  }
+
+  // Writing a row's gradient.
+  struct Writer {
+    T* g;             // null: nothing to write
+    T* gs;            // this thread's first vector's place
+    bool same;        // the gradient's rows lie as the logits' do within 16 bytes
+    Shift sh;
+    RowGrad rg;
+  };
+  // (a, b) as the loss's scale and a token outside the vocabulary leave them.
+  __device__ __forceinline__ void scaled(const Extra& ex, float& a, float& b) const {
+    if constexpr (Src::kPolicy) { a *= src.up(); b *= src.up(); }
+    if (ex.tok < 0 || ex.tok >= in.V) a = NAN;
+  }
+  __device__ __forceinline__ Writer writer(int64_t row, const RowStats& r, float a, float b) const {
+    Writer w;
+    w.g = gr.g ? gr.g + gr.at(row, in) : nullptr;
+    if (w.g && a == 0.f && b == 0.f) {
+      zeros(row);
+      w.g = nullptr;
+    }
+    w.sh = shift_of(r, in.c);
+    w.rg = row_grad(a, b, r, in.inv_temp);
+    const T* x = row_at(row);
+    const Cut cut = cut_row(x, in.V);
+    w.same = (((uintptr_t)x ^ (uintptr_t)w.g) & 15) == 0;
+    int v0;
+    stretch(cut, v0);
+    w.gs = w.g + cut.head + (int64_t)(v0 + tid) * N;
+    return w;
+  }
+  // The gradient of the vector v places after the thread's first (the token's
+  // element is put right by finish()).
+  __device__ __forceinline__ void write(const Writer& w, int v, uint4 u) const {
+    constexpr int P = N / 2;
+    F2 f[P];
+    if (!w.sh.far) {
+      const F2 cc = f2(in.c, in.c), no = f2(-w.sh.off, -w.sh.off), nA = f2(-w.rg.A, -w.rg.A);
+      if constexpr (ENT) u = Vec<T>::bound(u);
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        const F2 d = fma2(Vec<T>::pair(u, q), cc, no);
+        f[q] = mul2(ex2(d), ENT ? fma2(f2(-w.rg.B, -w.rg.B), d, nA) : nA);
       }
     } else {
-      r = stats_of(now.stats);
-      a = now.a;
-      if constexpr (ENT) b = incoming_entropy(src, now.w, now.b);
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        float y, z;
+        split(Vec<T>::pair(u, q), y, z);
+        f[q] = f2(grad_at<ENT>(y, w.sh, w.rg), grad_at<ENT>(z, w.sh, w.rg));
+      }
     }
-    // ---- gradient
-    if constexpr (kGrad) {
-      const int64_t row = advance();
-      if (row >= 0) next = place(row);
-      if constexpr (Src::kPolicy) { a *= src.up(); b *= src.up(); }
-      if (!now.ok) a = NAN;
-      T* g = gr.g ? gr.g + gr.at(now.row, in.seq) : nullptr;
-      const bool none = a == 0.f && b == 0.f;
-      if (g && none) zeros(now.row);
-      const Shift sh = shift_of(r, c);
-      const RowGrad rg = row_grad(a, b, r, in.inv_temp);
-      const bool same = (((uintptr_t)now.x ^ (uintptr_t)g) & 15) == 0;
-      // the token's vector and its element there
-      const int64_t rel = now.tok - now.head - now.v0 * N;
-      const int tv = rel >= 0 && rel < (int64_t)now.mid * N ? (int)(rel / N) : -1;
-      const int te = (int)(rel - (int64_t)tv * N);
-      T* gs = g + now.head + now.v0 * N;
+    const uint4 o = Vec<T>::join(f);
+    if (w.same) __stcs(reinterpret_cast<uint4*>(w.gs) + v, o);
+    else Vec<T>::scatter(w.gs + (int64_t)v * N, o);
+  }
+  // The row's end elements, and the token's by the thread that wrote its place;
+  // incoming() gives (a, b, S0, t) to that one.
+  template <class F>
+  __device__ __forceinline__ void finish(const Writer& w, int64_t row, const Extra& ex, F&& incoming) const {
+    const Cut cut = cut_row(row_at(row), in.V);
+    const int ends = ends_of(cut);
+    const int end = tid < ends ? (tid < cut.head ? tid : in.V - ends + tid) : -1;
+    if (end >= 0) w.g[end] = Vec<T>::put(grad_at<ENT>(ex.end, w.sh, w.rg));
+    if (ex.tok < 0 || ex.tok >= in.V) return;
+    int v0;
+    const int n = stretch(cut, v0);
+    const int tok = (int)ex.tok, rel = tok - cut.head - v0 * N;
+    if (rel >= 0 && rel < n * N ? rel / N % NT == tid : tok == end) {
+      const float4 q = incoming();
+      w.g[tok] = Vec<T>::put(token_grad(ex.xt, w.sh, q.x, q.y, q.z, q.w, in.inv_temp));
+    }
+  }
+};
+
+// ---- forward alone, and gradient alone: rows stream through registers --------------
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+
+template <class T, bool ENT, int MODE, class Src, int NT, int U, bool CL>
+__global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
+    stream_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src) {
+  if constexpr (Src::kPolicy && MODE == kBwd) {
+    if (src.skip()) return;
+  }
+  constexpr int M = 2;  // vectors taken at a time
+  static_assert(MODE != kBoth && U % M == 0, "streams");
+  __shared__ Table<NT, CL> table;
+  unsigned turn = 0;
+  using W = Walk<T, ENT, MODE, Src, NT, CL>;
+  W walk(in, out, gr, src);
+  const unsigned low = Vec<T>::kLowest;
+  uint4 u[U];
+  auto fetch = [&](const typename W::Place& p, int base, int j) {
+    if (base + (j + M - 1) * NT < p.mid) {
 #pragma unroll
-      for (int j = 0; j < K; ++j) {
-        if constexpr (MODE == kBwd) copy_wait<K - 1>();
-        const int v = tid + j * NT;
-        if (g && !none && v < now.mid) {
-          float f[N];
-          Vec<T>::unpack(mine[j * NT], f);
-          if (sh.far) {
+      for (int k = j; k < j + M; ++k) u[k] = load_once(p.at + base + k * NT);
+    } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = grad_at<ENT>(f[e], Shift{c, sh.off, true}, rg);
-          } else {
+      for (int k = j; k < j + M; ++k)
+        u[k] = base + k * NT < p.mid ? load_once(p.at + base + k * NT) : make_uint4(low, low, low, low);
+    }
+  };
+  const int rounds = (walk.most() + NT * U - 1) / (NT * U);
+  const int64_t first = walk.advance();
+  if (first < 0) return;  // the same for every CTA of the team
+  typename W::Place now = walk.place(first);
+  typename W::Extra ex = walk.extra(first);
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = grad_at<ENT>(f[e], Shift{c, sh.off, false}, rg);
-          }
-          if (v == tv) {
+  for (int j = 0; j < U; j += M) fetch(now, 0, j);
+  walk.token_logit(first, ex);
+  if constexpr (CL && MODE == kFwd) cluster_barrier();  // the others' tables exist
+  for (;;) {
+    typename W::Place next{-1, nullptr, 0};
+    typename W::Extra nx{};
+    const int64_t row = walk.advance();
+    if (row >= 0) {
+      next = walk.place(row);
+      nx = walk.extra(row);
+    }
+    Run<ENT> run(in.c);
+    typename W::Writer wr;
+    float a = 0.f, b = 0.f;
+    if constexpr (MODE == kBwd) {
+      a = ex.a;
+      b = ENT ? incoming_entropy(src, ex.w, ex.b) : 0.f;
+      walk.scaled(ex, a, b);
+      wr = walk.writer(now.row, stats_of(ex.stats), a, b);
+    }
+    for (int round = 0; round < rounds; ++round) {
+      const int base = round * (NT * U);
+      const bool over = round + 1 == rounds;
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (e == te) f[e] += rg.a;
-          }
-          if (same) {
-            __stcs(reinterpret_cast<uint4*>(gs) + v, Vec<T>::pack(f));
-          } else {
+      for (int j = 0; j < U; j += M) {
+        if constexpr (MODE == kFwd) {
+          uint4 t[M];
 #pragma unroll
-            for (int e = 0; e < N; ++e) gs[(int64_t)v * N + e] = Vec<T>::put(f[e]);
-          }
+          for (int k = 0; k < M; ++k) t[k] = u[j + k];
+          run.template add_vectors<T, M>(t, in.c);
+        } else if (wr.g) {
+#pragma unroll
+          for (int k = 0; k < M; ++k)
+            if (base + (j + k) * NT < now.mid) walk.write(wr, base + (j + k) * NT, u[j + k]);
         }
-        fetch(next, j);
+        if (over) fetch(next, 0, j);
+        else fetch(now, base + NT * U, j);
       }
-      if (g && !none && tid < now.ends) {
-        const int64_t i = tid < now.head ? tid : V - now.ends + tid;
-        float f = grad_at<ENT>(now.end, sh, rg);
-        if (i == now.tok) f += rg.a;
-        g[i] = Vec<T>::put(f);
-      }
+    }
+    if constexpr (MODE == kFwd) {
+      const RowStats r = walk.join(run, now.row, ex, table, turn);
+      if (walk.rank == 0 && threadIdx.x < 32) walk.outputs(now.row, r, ex, a, b);
+    } else if (wr.g) {
+      walk.finish(wr, now.row, ex, [&] { return make_float4(a, b, ex.stats.y, ex.stats.z); });
     }
     if (next.row < 0) break;
-    token_logit(next);
+    walk.token_logit(next.row, nx);
     now = next;
+    ex = nx;
+  }
+}
+
+// ---- both in one pass: a row waits in shared memory for its gradient ---------------
+// Each thread's vectors of the row, at most K, have slots of its own, filled by
+// cp.async (all K in flight at once): no barrier, only the thread's own wait.
+template <class T, bool ENT, class Src, int NT, int K, bool CL>
+__global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src) {
+  constexpr int M = 2;
+  static_assert(K % M == 0, "whole groups");
+  extern __shared__ uint4 slots[];  // [K][NT]
+  __shared__ Table<NT, CL> table;
+  __shared__ float4 incoming;       // (a, b, S0, t) of the row, from the warp that formed them
+  unsigned turn = 0;
+  using W = Walk<T, ENT, kBoth, Src, NT, CL>;
+  W walk(in, out, gr, src);
+  uint4* mine = slots + threadIdx.x;
+  const unsigned low = Vec<T>::kLowest;
+  auto fetch = [&](const typename W::Place& p, int j) {
+    if (j * NT < p.mid) copy16(mine + j * NT, p.at + j * NT);
+    copy_commit();
+  };
+  const int64_t first = walk.advance();
+  if (first < 0) return;  // the same for every CTA of the team
+  typename W::Place now = walk.place(first);
+  typename W::Extra ex = walk.extra(first);
+#pragma unroll
+  for (int j = 0; j < K; ++j) fetch(now, j);
+  walk.token_logit(first, ex);
+  if constexpr (CL) cluster_barrier();  // the others' tables exist
+  for (;;) {
+    Run<ENT> run(in.c);
+#pragma unroll
+    for (int j = 0; j < K; j += M) {
+      copy_wait_upto<K - M>(K - M - j);
+      uint4 u[M];
+#pragma unroll
+      for (int k = 0; k < M; ++k) u[k] = (j + k) * NT < now.mid ? mine[(j + k) * NT] : make_uint4(low, low, low, low);
+      run.template add_vectors<T, M>(u, in.c);
+    }
+    const RowStats r = walk.join(run, now.row, ex, table, turn);
+    if (threadIdx.x < 32) {
+      float a = 0.f, b = 0.f;
+      walk.outputs(now.row, r, ex, a, b);
+      walk.scaled(ex, a, b);
+      if (threadIdx.x == 0) incoming = make_float4(a, b, r.s0, r.t);
+    }
+    typename W::Place next{-1, nullptr, 0};
+    typename W::Extra nx{};
+    const int64_t row = walk.advance();
+    if (row >= 0) {
+      next = walk.place(row);
+      nx = walk.extra(row);
+    }
+    __syncthreads();
+    const typename W::Writer wr = walk.writer(now.row, r, incoming.x, incoming.y);
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      if (wr.g && j * NT < now.mid) walk.write(wr, j * NT, mine[j * NT]);
+      fetch(next, j);
+    }
+    if (wr.g) walk.finish(wr, now.row, ex, [&] { return incoming; });
+    if (next.row < 0) break;
+    walk.token_logit(next.row, nx);
+    now = next;
+    ex = nx;
   }
 }
 
@@ -1057,7 +1401,7 @@ __global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, 
     const bool live = row_raw < in.rows;
     const int64_t row = live ? row_raw : in.rows - 1;  // idle lanes shuffle along on the last row
     const T* x = in.x + in.at(row);
-    T* g = MODE == kFwd || !gr.g ? nullptr : gr.g + gr.at(row, in.seq);
+    T* g = MODE == kFwd || !gr.g ? nullptr : gr.g + gr.at(row, in);
     const bool kept = mask_at(in.mask, row);
     const int64_t tok = kept ? in.tokens[row] : 0;
     const bool ok = tok >= 0 && tok < V;
@@ -1090,13 +1434,13 @@ __global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, 
     const RowStats r{m, s0, s1 / s0, true, ENT && s0 == 1.f && s1 == 0.f};
     double lp = 0.0;
     float ent = 0.f;
-    if (Src::kPolicy || MODE != kBwd) lp = logprob_of(xt, r, in.c, in.c64);
+    if (Src::kPolicy || MODE != kBwd) lp = logprob_of(xt, r, in.c, in.c64, in.c_off);
     if constexpr (ENT) ent = entropy_of(r);
     if (!kept) { lp = 0.0; ent = 0.f; }
     float a = 0.f, b = 0.f;
     if (kept) {
       if constexpr (Src::kPolicy) {
-        const int64_t env = row / in.seq;
+        const int64_t env = in.env(row);
         const Policy& p = src.p;
         const PolicyTerm o = policy_term(p, lp, p.old_lp[row], p.adv[p.adv_row ? env : row], p.ref ? p.ref[row] : 0.f);
         const float w = policy_weight(p, env);
@@ -1130,8 +1474,7 @@ __global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, 
       for (int k = 0; k < E; ++k) {
         const int i = lane + k * G;
         if (i < V) {
-          float o = grad_at<ENT>(f[k], sh, rg);
-          if (i == tok) o += rg.a;
+          const float o = i == tok ? token_grad(f[k], sh, a, b, r.s0, r.t, in.inv_temp) : grad_at<ENT>(f[k], sh, rg);
           g[i] = Vec<T>::put(none ? 0.f : o);
         }
       }

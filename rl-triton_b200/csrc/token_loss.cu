@@ -223,14 +223,16 @@ struct LogitsCall {
   void* g;
   int64_t ges, gss;
   int64_t N, T, V;
-  float temperature;
+  double temperature;
   int dtype;
 };
 
+constexpr int64_t kMostVocab = 0x7fffff00;  // a row's elements are counted in 32 bits
+
 int check_logits(const LogitsCall& c) {
-  if (c.N < 0 || c.T < 0 || c.V < 1) return RLS_EINVAL;
+  if (c.N < 0 || c.T < 0 || c.V < 1 || c.V > kMostVocab) return RLS_EINVAL;
   if (c.dtype != RLS_F32 && c.dtype != RLS_BF16) return RLS_EINVAL;
-  if (!(c.temperature > 0.f) || !std::isfinite(c.temperature)) return RLS_EINVAL;
+  if (!(c.temperature > 0.0) || !std::isfinite(c.temperature)) return RLS_EINVAL;
   if (!mask_ok(c.mask.p, c.mask.kind)) return RLS_EINVAL;
   if (c.T > 0 && c.N > INT64_MAX / c.T) return RLS_EINVAL;
   if (c.N == 0 || c.T == 0) return RLS_OK;
@@ -256,12 +258,14 @@ Rows<T> rows_of_call(const LogitsCall& c) {
   r.ss = c.ss;
   r.rows = c.N * c.T;
   r.seq = c.T;
-  r.V = c.V;
+  r.env = Divide::of(c.T, c.N * c.T);
+  r.V = (int)c.V;
   r.tokens = c.tokens;
   r.mask = c.mask;
-  r.c64 = 1.4426950408889634074 / (double)c.temperature;
+  r.c64 = 1.4426950408889634074 / c.temperature;
   r.c = (float)r.c64;
-  r.inv_temp = (float)(1.0 / (double)c.temperature);
+  r.c_off = r.c64 / (double)r.c - 1.0;
+  r.inv_temp = (float)(1.0 / c.temperature);
   r.flat = c.N == 1 || (c.T == 1 ? false : c.es == c.T * c.ss);
   if (c.T == 1 && c.N > 1) { r.ss = c.es; r.flat = true; }
   return r;
@@ -301,7 +305,7 @@ int64_t rls::tok::sum_blocks(int64_t need) {
 
 extern "C" int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
                                   const void* mask, int mask_kind, float* logprobs, float* entropy, float* row_stats,
-                                  int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature, int in_dtype,
+                                  int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature, int in_dtype,
                                   void* stream) {
   LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, nullptr, 0, 0, num_envs, seq_len,
                vocab, temperature, in_dtype};
@@ -321,7 +325,7 @@ extern "C" int rls_token_logprobs_backward(const void* logits, int64_t env_strid
                                            const float* row_stats, const float* grad_logprobs,
                                            const float* grad_entropy, void* grad_logits, int64_t grad_env_stride,
                                            int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab,
-                                           float temperature, int in_dtype, void* stream) {
+                                           double temperature, int in_dtype, void* stream) {
   LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
                grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
   if (int st = check_logits(c)) return st;
@@ -404,7 +408,7 @@ extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, in
                                       int mask_kind, const rls_policy_t* policy, float grad_scale, float* norm,
                                       float* logprobs, float* entropy, float* row_stats, float* loss, float* stats,
                                       void* grad_logits, int64_t grad_env_stride, int64_t grad_step_stride,
-                                      int64_t num_envs, int64_t seq_len, int64_t vocab, float temperature,
+                                      int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature,
                                       int in_dtype, void* ws, size_t ws_bytes, void* stream) {
   LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
                grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
@@ -446,7 +450,7 @@ extern "C" int rls_policy_loss_logits_backward(const void* logits, int64_t env_s
                                                int force, const float* norm,
                                                const float* row_stats, void* grad_logits, int64_t grad_env_stride,
                                                int64_t grad_step_stride, int64_t num_envs, int64_t seq_len,
-                                               int64_t vocab, float temperature, int in_dtype, void* stream) {
+                                               int64_t vocab, double temperature, int in_dtype, void* stream) {
   LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
                grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
   if (!policy_ok(policy)) return RLS_EINVAL;

@@ -6,11 +6,10 @@ namespace rls {
 namespace tok {
 namespace {
 
-// The row pipeline with C CTAs a row.
-template <class T, bool ENT, int MODE, class Src, int NT, int K, bool CL>
-int pipe(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, int size, cudaStream_t s) {
-  auto kern = pipe_rows_kernel<T, ENT, MODE, Src, NT, K, CL>;
-  constexpr size_t smem = (size_t)NT * K * 16;
+// A kernel over teams of `size` CTAs.
+template <class T, class Src, int NT, size_t smem, bool CL>
+int launch(void (*kern)(Rows<T>, RowOut, GradRows<T>, Src), const Rows<T>& in, const RowOut& out,
+           const GradRows<T>& gr, const Src& src, int size, int (&resident)[64][4], cudaStream_t s) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RLS_ECUDA;
   cudaLaunchConfig_t cfg = {};
@@ -27,7 +26,6 @@ int pipe(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src&
   // Teams that fit on the device at once, asked once per device and cluster size
   // (under the launch lock): a team that had to wait for another would double
   // the time.
-  static int resident[64][4] = {{0}};
   int& most = resident[dev][size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3];
   if (!most) {
     int n = 0;
@@ -49,6 +47,19 @@ int pipe(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src&
   return cudaLaunchKernelEx(&cfg, kern, in, out, gr, src) == cudaSuccess ? RLS_OK : RLS_ECUDA;
 }
 
+template <class T, bool ENT, int MODE, class Src, int NT, int U, bool CL>
+int stream(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, int size, cudaStream_t s) {
+  static int resident[64][4] = {{0}};
+  return launch<T, Src, NT, 0, CL>(stream_rows_kernel<T, ENT, MODE, Src, NT, U, CL>, in, out, gr, src, size, resident,
+                                   s);
+}
+template <class T, bool ENT, class Src, int NT, int K, bool CL>
+int both(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, int size, cudaStream_t s) {
+  static int resident[64][4] = {{0}};
+  return launch<T, Src, NT, (size_t)NT * K * 16, CL>(both_rows_kernel<T, ENT, Src, NT, K, CL>, in, out, gr, src, size,
+                                                     resident, s);
+}
+
 // Rows beyond the slots of a full cluster: one CTA a row, the second pass from L2.
 template <class T, bool ENT, int MODE, class Src>
 int plain(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
@@ -63,20 +74,29 @@ template <class T, bool ENT, int MODE, class Src>
 int launch_cta_rows(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
   const int64_t nvec = in.V / Vec<T>::N;
   int size = 1;
-  while (size < kMostCtas && nvec > (int64_t)size * 4096) size *= 2;
-  // few rows: more CTAs for each, down to 512 vectors a CTA
+  // With the gradient a row stays in the slots (64 KB a CTA).
+  if (MODE == kBoth)
+    while (size < kMostCtas && nvec > (int64_t)size * 4096) size *= 2;
+  // few rows: more CTAs for each, down to 1024 vectors a CTA
   while (size < kMostCtas && in.rows * size < 2 * 148 && nvec > (int64_t)size * 1024) size *= 2;
   const int64_t each = (nvec + size - 1) / size;
-  if (each > 4096) return plain<T, ENT, MODE, Src>(in, out, gr, src, s);
-  if (size > 1) {
-    if (each <= 1024) return pipe<T, ENT, MODE, Src, 256, 4, true>(in, out, gr, src, size, s);
-    return pipe<T, ENT, MODE, Src, 256, 16, true>(in, out, gr, src, size, s);
+  if constexpr (MODE == kBoth) {
+    if (each > 4096) return plain<T, ENT, MODE, Src>(in, out, gr, src, s);
+    if (size > 1) {
+      if (each <= 1024) return both<T, ENT, Src, 256, 4, true>(in, out, gr, src, size, s);
+      return both<T, ENT, Src, 256, 16, true>(in, out, gr, src, size, s);
+    }
+    if (each <= 256) return both<T, ENT, Src, 64, 4, false>(in, out, gr, src, 1, s);
+    if (each <= 512) return both<T, ENT, Src, 64, 8, false>(in, out, gr, src, 1, s);
+    if (each <= 1024) return both<T, ENT, Src, 128, 8, false>(in, out, gr, src, 1, s);
+    if (each <= 2048) return both<T, ENT, Src, 256, 8, false>(in, out, gr, src, 1, s);
+    return both<T, ENT, Src, 256, 16, false>(in, out, gr, src, 1, s);
+  } else {
+    if (size > 1) return stream<T, ENT, MODE, Src, 256, 4, true>(in, out, gr, src, size, s);
+    if (each <= 512) return stream<T, ENT, MODE, Src, 64, 4, false>(in, out, gr, src, 1, s);
+    if (each <= 1024) return stream<T, ENT, MODE, Src, 128, 8, false>(in, out, gr, src, 1, s);
+    return stream<T, ENT, MODE, Src, 256, 8, false>(in, out, gr, src, 1, s);
   }
-  if (each <= 256) return pipe<T, ENT, MODE, Src, 64, 4, false>(in, out, gr, src, 1, s);
-  if (each <= 512) return pipe<T, ENT, MODE, Src, 64, 8, false>(in, out, gr, src, 1, s);
-  if (each <= 1024) return pipe<T, ENT, MODE, Src, 128, 8, false>(in, out, gr, src, 1, s);
-  if (each <= 2048) return pipe<T, ENT, MODE, Src, 256, 8, false>(in, out, gr, src, 1, s);
-  return pipe<T, ENT, MODE, Src, 256, 16, false>(in, out, gr, src, 1, s);
 }
 
 RLS_TOKEN_INSTANTIATE(launch_cta_rows)

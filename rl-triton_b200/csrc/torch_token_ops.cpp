@@ -118,7 +118,7 @@ std::tuple<Tensor, Tensor, Tensor> op_logprobs(const Tensor& logits, const Tenso
   Tensor ent = like(a.x, entropy ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
   Tensor stats = row_stats(a, keep);
   check(rls_token_logprobs(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), a.mask.ptr(),
-                           a.mask.kind, W(lp), W(ent), W(stats), a.n, a.t, a.v, (float)temperature, dtype_of(a.x),
+                           a.mask.kind, W(lp), W(ent), W(stats), a.n, a.t, a.v, temperature, dtype_of(a.x),
                            stream_of(a.x)),
         "rls_token_logprobs");
   return {lp, ent, stats};
@@ -131,7 +131,7 @@ Tensor op_logprobs_backward(const Tensor& logits, const Tensor& tokens, const Op
   Tensor g = op_grad_buffer(a.x);
   check(rls_token_logprobs_backward(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(),
                                     a.mask.ptr(), a.mask.kind, W(stats), F(gl), F(ge), g.data_ptr(), g.stride(0),
-                                    g.stride(1), a.n, a.t, a.v, (float)temperature, dtype_of(a.x), stream_of(a.x)),
+                                    g.stride(1), a.n, a.t, a.v, temperature, dtype_of(a.x), stream_of(a.x)),
         "rls_token_logprobs_backward");
   return g;
 }
@@ -209,7 +209,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_policy_log
                                F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, &p, (float)grad_scale,
                                W(norm), W(lp), W(ent), W(rows), loss.data_ptr<float>(), stats.data_ptr<float>(),
                                need_grad ? g.data_ptr() : nullptr, need_grad ? g.stride(0) : 0,
-                               need_grad ? g.stride(1) : 0, a.n, a.t, a.v, (float)temperature, dtype_of(a.x),
+                               need_grad ? g.stride(1) : 0, a.n, a.t, a.v, temperature, dtype_of(a.x),
                                ws.data_ptr(), (size_t)ws.numel(), stream_of(a.x)),
         "rls_policy_loss_logits");
   return {loss, lp, ent, stats, norm, rows, g};
@@ -228,7 +228,7 @@ void op_policy_logits_backward_(Tensor& grad, const Tensor& logits, const Tensor
                                         F(old_lp), F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, &p,
                                         (float)grad_scale, F(up), force, W(norm), W(rows),
                                         grad.data_ptr(), grad.stride(0), grad.stride(1), a.n, a.t, a.v,
-                                        (float)temperature, dtype_of(a.x), stream_of(a.x)),
+                                        temperature, dtype_of(a.x), stream_of(a.x)),
         "rls_policy_loss_logits_backward");
 }
 

@@ -227,6 +227,7 @@ def _(coef, grad_loss, chosen_mask, rejected_mask, chosen_len, rejected_len, hal
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
 _SEG = ctypes.POINTER(Segment)
@@ -253,15 +254,15 @@ _SIGS = {
     "rls_gae_value_loss": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I, _F, _I, _P, _SZ,
                                 _P]),
     "rls_gae_obs_skip": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I, _P]),
-    "rls_token_logprobs": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _F, _I, _P]),
-    "rls_token_logprobs_backward": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F,
+    "rls_token_logprobs": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _D, _I, _P]),
+    "rls_token_logprobs_backward": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _D,
                                          _I, _P]),
     "rls_policy_loss": (_I, [_P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _P, _P, _P, _I64, _I64, _P, _SZ, _P]),
     "rls_policy_loss_backward": (_I, [_P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _I, _P, _P, _I64, _I64, _P]),
     "rls_policy_loss_logits": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _P, _P, _P, _P, _P, _P,
-                                    _I64, _I64, _I64, _I64, _I64, _F, _I, _P, _SZ, _P]),
+                                    _I64, _I64, _I64, _I64, _I64, _D, _I, _P, _SZ, _P]),
     "rls_policy_loss_logits_backward": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _I, _P, _P,
-                                             _P, _I64, _I64, _I64, _I64, _I64, _F, _I, _P]),
+                                             _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _P]),
     "rls_preference_loss": (_I, [_P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _F, _F, _I, _I, _P, _P, _P, _P,
                                  _SZ, _P]),
     "rls_preference_loss_backward": (_I, [_P, _P, _P, _P, _I, _P, _P, _I64, _I64, _I64, _P]),
