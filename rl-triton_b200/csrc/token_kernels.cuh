@@ -7,7 +7,7 @@
 //   d logprob / d x_v = (1[v = tok] - p_v) / temperature,
 //   d H / d x_v       = -p_v (log p_v + H) / temperature.
 // Everything is computed in base 2: with c = log2(e) / temperature and an
-// offset M (the running maximum times c, rounded to a whole number),
+// offset M (an element near the maximum, times c, rounded to a whole number),
 //   d_v = x_v c - M,  S0 = sum 2^d_v,  S1 = sum 2^d_v d_v,  t = S1 / S0,
 //   logprob = ln2 (d_tok - log2 S0),   H = ln2 (log2 S0 - t),
 // one fused multiply-add and one ex2 an element, and the gradient for incoming
@@ -32,7 +32,11 @@ constexpr float kLn2 = 0.693147180559945309f;
 // useless and S0 leaves [kLeast, kMost]; such rows, and rows with NaN, are
 // summed again with d = (x - m) c, the far form.
 constexpr float kFar = 1e30f;
-constexpr float kLeast = 0.25f, kMost = 1e15f;
+constexpr float kLeast = 0.25f, kMost = 1e18f;
+// An offset stays until an element lies this far (in powers of two) above it: any offset
+// near the maximum serves, and a warp whose lanes each kept their own maximum
+// would move one of them at almost every step.
+constexpr float kSlack = 24.f;
 constexpr float kDeep = -16384.f;  // 2^kDeep is 0: keeps 2^d * d finite at d = -inf
 
 __device__ __forceinline__ float ex2(float x) {
@@ -141,6 +145,7 @@ struct GradRows {
   T* g;
   int64_t es, ss;
   bool flat;
+  bool alike;  // every row lies within 16 bytes as its logits do
   __device__ __forceinline__ int64_t at(int64_t row, const Rows<T>& in) const {
     if (flat) return row * ss;
     const int64_t e = in.env(row);
@@ -347,16 +352,17 @@ __device__ __forceinline__ Cut cut_row(const T* p, int V) {
 }
 
 // ---- running statistics --------------------------------------------------------
-// (m, s0, s1) of the elements seen: s0 = sum 2^d, s1 = sum 2^d d with d taken
-// from off = m c; without an entropy to compute, s1 takes each vector's largest
-// d for all of its elements, which serves for logprob_of's small correction.
-// m starts at -kFar, not -inf, so that no difference of two offsets is NaN;
-// elements below it count as 0 (rows that have nothing above it take the far form).
+// s0 = sum 2^d and s1 = sum 2^d d of the elements seen, with d taken from off, the
+// offset of one of them, m, that no other exceeds by kSlack; without an entropy
+// to compute, s1 takes each group's largest d for all of its elements, which serves for
+// logprob_of's small correction.  m starts at -kFar, not -inf, so that no
+// difference of two offsets is NaN; elements below it count as 0 (rows that have
+// nothing above it take the far form).
 template <bool ENT>
 struct Run {
   float m = -kFar, off, s0 = 0.f, s1 = 0.f;
   __device__ __forceinline__ explicit Run(float c) : off(offset_of(-kFar, c)) {}
-  // Moves to a larger maximum.
+  // Moves to a larger element's offset.
   __device__ __forceinline__ void raise(float mx, float c) {
     const float to = offset_of(mx, c), by = off - to;
     const float k = ex2(by);
@@ -370,7 +376,7 @@ struct Run {
     float mx = x[0];
 #pragma unroll
     for (int k = 1; k < K; ++k) mx = fmaxf(mx, x[k]);
-    if (mx > m) raise(mx, c);
+    if (fmaf(mx, c, -off) > kSlack) raise(mx, c);
     float e[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -396,7 +402,11 @@ struct Run {
     float mx = Vec<T>::top(u[0]);
 #pragma unroll
     for (int k = 1; k < M; ++k) mx = fmaxf(mx, Vec<T>::top(u[k]));
-    if (mx > m) raise(mx, c);
+    float dm = fmaf(mx, c, -off);
+    if (dm > kSlack) {
+      raise(mx, c);
+      dm = fmaf(mx, c, -off);
+    }
     const F2 cc = f2(c, c), no = f2(-off, -off);
     F2 sum, by;
 #pragma unroll
@@ -417,7 +427,7 @@ struct Run {
       split(by, x, y);
       s1 += x + y;
     } else {
-      s1 = fmaf(x, fmaxf(fmaf(mx, c, -off), kDeep), s1);
+      s1 = fmaf(x, fmaxf(dm, kDeep), s1);
     }
   }
   __device__ __forceinline__ void join(float om, float ooff, float os0, float os1) {
@@ -1003,14 +1013,14 @@ struct Walk {
   struct Place {
     int64_t row;
     const uint4* at;  // this thread's first vector
-    int mid;          // vectors from there to the end of the stretch (every NT-th is the thread's)
+    int n, mid;       // vectors of the stretch, and from the thread's first to its end
   };
   __device__ __forceinline__ Place place(int64_t row) const {
     const T* x = row_at(row);
     const Cut cut = cut_row(x, in.V);
     int v0;
     const int n = stretch(cut, v0);
-    return Place{row, reinterpret_cast<const uint4*>(x + cut.head) + v0 + tid, n - tid};
+    return Place{row, reinterpret_cast<const uint4*>(x + cut.head) + v0 + tid, n, n - tid};
   }
   // What the row's one-off steps need, asked for a row ahead.
   struct Extra {
@@ -1155,7 +1165,6 @@ struct Walk {
   struct Writer {
     T* g;             // null: nothing to write
     T* gs;            // this thread's first vector's place
-    bool same;        // the gradient's rows lie as the logits' do within 16 bytes
     Shift sh;
     RowGrad rg;
   };
@@ -1175,36 +1184,33 @@ struct Walk {
     w.rg = row_grad(a, b, r, in.inv_temp);
     const T* x = row_at(row);
     const Cut cut = cut_row(x, in.V);
-    w.same = (((uintptr_t)x ^ (uintptr_t)w.g) & 15) == 0;
     int v0;
     stretch(cut, v0);
     w.gs = w.g + cut.head + (int64_t)(v0 + tid) * N;
     return w;
   }
-  // The gradient of the vector v places after the thread's first (the token's
-  // element is put right by finish()).
-  __device__ __forceinline__ void write(const Writer& w, int v, uint4 u) const {
+  // The gradient of the vector v places after the thread's first, stored where
+  // `inside` (the token's element is put right by finish()).
+  __device__ __forceinline__ void write(const Writer& w, int v, uint4 u, bool inside) const {
     constexpr int P = N / 2;
     F2 f[P];
-    if (!w.sh.far) {
-      const F2 cc = f2(in.c, in.c), no = f2(-w.sh.off, -w.sh.off), nA = f2(-w.rg.A, -w.rg.A);
-      if constexpr (ENT) u = Vec<T>::bound(u);
+    const F2 cc = f2(in.c, in.c), no = f2(-w.sh.off, -w.sh.off), nA = f2(-w.rg.A, -w.rg.A);
+    if constexpr (ENT) u = Vec<T>::bound(u);
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const F2 d = fma2(Vec<T>::pair(u, q), cc, no);
-        f[q] = mul2(ex2(d), ENT ? fma2(f2(-w.rg.B, -w.rg.B), d, nA) : nA);
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < P; ++q) {
-        float y, z;
-        split(Vec<T>::pair(u, q), y, z);
-        f[q] = f2(grad_at<ENT>(y, w.sh, w.rg), grad_at<ENT>(z, w.sh, w.rg));
-      }
+    for (int q = 0; q < P; ++q) {
+      const F2 d = fma2(Vec<T>::pair(u, q), cc, no);
+      f[q] = mul2(ex2(d), ENT ? fma2(f2(-w.rg.B, -w.rg.B), d, nA) : nA);
     }
     const uint4 o = Vec<T>::join(f);
-    if (w.same) __stcs(reinterpret_cast<uint4*>(w.gs) + v, o);
-    else Vec<T>::scatter(w.gs + (int64_t)v * N, o);
+    if (inside) __stcs(reinterpret_cast<uint4*>(w.gs) + v, o);
+  }
+  // The same for all of the thread's vectors of a row in the far form, read again.
+  __device__ __forceinline__ void write_far(const Writer& w, const Place& p) const {
+    const T* x = reinterpret_cast<const T*>(p.at);
+#pragma unroll 1
+    for (int v = 0; v < p.mid; v += NT)
+#pragma unroll 1
+      for (int e = v * N; e < v * N + N; ++e) w.gs[e] = Vec<T>::put(grad_at<ENT>(Vec<T>::get(x + e), w.sh, w.rg));
   }
   // The row's end elements, and the token's by the thread that wrote its place;
   // incoming() gives (a, b, S0, t) to that one.
@@ -1248,14 +1254,17 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
   W walk(in, out, gr, src);
   const unsigned low = Vec<T>::kLowest;
   uint4 u[U];
-  auto fetch = [&](const typename W::Place& p, int base, int j) {
-    if (base + (j + M - 1) * NT < p.mid) {
+  // Vectors j .. j + M - 1 of the round that begins at `base`; `full`: all threads have them.
+  auto fetch = [&](const typename W::Place& p, int base, bool full, int j) {
+    if (full) {
 #pragma unroll
       for (int k = j; k < j + M; ++k) u[k] = load_once(p.at + base + k * NT);
     } else {
 #pragma unroll
-      for (int k = j; k < j + M; ++k)
-        u[k] = base + k * NT < p.mid ? load_once(p.at + base + k * NT) : make_uint4(low, low, low, low);
+      for (int k = j; k < j + M; ++k) {
+        u[k] = make_uint4(low, low, low, low);
+        if (base + k * NT < p.mid) u[k] = load_once(p.at + base + k * NT);
+      }
     }
   };
   const int rounds = (walk.most() + NT * U - 1) / (NT * U);
@@ -1264,11 +1273,11 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
   typename W::Place now = walk.place(first);
   typename W::Extra ex = walk.extra(first);
 #pragma unroll
-  for (int j = 0; j < U; j += M) fetch(now, 0, j);
+  for (int j = 0; j < U; j += M) fetch(now, 0, NT * U <= now.n, j);
   walk.token_logit(first, ex);
   if constexpr (CL && MODE == kFwd) cluster_barrier();  // the others' tables exist
   for (;;) {
-    typename W::Place next{-1, nullptr, 0};
+    typename W::Place next{-1, nullptr, 0, 0};
     typename W::Extra nx{};
     const int64_t row = walk.advance();
     if (row >= 0) {
@@ -1284,9 +1293,14 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
       walk.scaled(ex, a, b);
       wr = walk.writer(now.row, stats_of(ex.stats), a, b);
     }
+    const bool near = MODE == kBwd && wr.g && !wr.sh.far;
+    if (MODE == kBwd && wr.g && !near) walk.write_far(wr, now);
     for (int round = 0; round < rounds; ++round) {
       const int base = round * (NT * U);
       const bool over = round + 1 == rounds;
+      const typename W::Place& then = over ? next : now;
+      const int from = over ? 0 : base + NT * U;
+      const bool then_full = from + NT * U <= then.n;
 #pragma unroll
       for (int j = 0; j < U; j += M) {
         if constexpr (MODE == kFwd) {
@@ -1294,13 +1308,14 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
 #pragma unroll
           for (int k = 0; k < M; ++k) t[k] = u[j + k];
           run.template add_vectors<T, M>(t, in.c);
-        } else if (wr.g) {
+        } else if (near) {
 #pragma unroll
-          for (int k = 0; k < M; ++k)
-            if (base + (j + k) * NT < now.mid) walk.write(wr, base + (j + k) * NT, u[j + k]);
+          for (int k = 0; k < M; ++k) {
+            const int v = base + (j + k) * NT;
+            walk.write(wr, v, u[j + k], v < now.mid);
+          }
         }
-        if (over) fetch(next, 0, j);
-        else fetch(now, base + NT * U, j);
+        fetch(then, from, then_full, j);
       }
     }
     if constexpr (MODE == kFwd) {
@@ -1350,7 +1365,10 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
       copy_wait_upto<K - M>(K - M - j);
       uint4 u[M];
 #pragma unroll
-      for (int k = 0; k < M; ++k) u[k] = (j + k) * NT < now.mid ? mine[(j + k) * NT] : make_uint4(low, low, low, low);
+      for (int k = 0; k < M; ++k) {
+        u[k] = make_uint4(low, low, low, low);
+        if ((j + k) * NT < now.mid) u[k] = mine[(j + k) * NT];
+      }
       run.template add_vectors<T, M>(u, in.c);
     }
     const RowStats r = walk.join(run, now.row, ex, table, turn);
@@ -1360,7 +1378,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
       walk.scaled(ex, a, b);
       if (threadIdx.x == 0) incoming = make_float4(a, b, r.s0, r.t);
     }
-    typename W::Place next{-1, nullptr, 0};
+    typename W::Place next{-1, nullptr, 0, 0};
     typename W::Extra nx{};
     const int64_t row = walk.advance();
     if (row >= 0) {
@@ -1369,10 +1387,16 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
     }
     __syncthreads();
     const typename W::Writer wr = walk.writer(now.row, r, incoming.x, incoming.y);
+    if (wr.g && !wr.sh.far) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      if (wr.g && j * NT < now.mid) walk.write(wr, j * NT, mine[j * NT]);
-      fetch(next, j);
+      for (int j = 0; j < K; ++j) {
+        walk.write(wr, j * NT, mine[j * NT], j * NT < now.mid);
+        fetch(next, j);
+      }
+    } else {
+      if (wr.g) walk.write_far(wr, now);
+#pragma unroll
+      for (int j = 0; j < K; ++j) fetch(next, j);
     }
     if (wr.g) walk.finish(wr, now.row, ex, [&] { return incoming; });
     if (next.row < 0) break;

@@ -277,6 +277,9 @@ GradRows<T> grad_of_call(const LogitsCall& c) {
   r.es = c.ges;
   r.ss = c.gss;
   r.flat = c.N == 1 || c.ges == c.T * c.gss;
+  auto off = [](int64_t elements) { return (elements * (int64_t)sizeof(T)) & 15; };
+  r.alike = (((uintptr_t)c.x ^ (uintptr_t)c.g) & 15) == 0 && (c.N == 1 || off(c.es) == off(c.ges)) &&
+            (c.T == 1 || off(c.ss) == off(c.gss));
   if (c.T == 1 && c.N > 1) { r.ss = c.ges; r.flat = true; }
   return r;
 }

@@ -73,6 +73,8 @@ int plain(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src
 template <class T, bool ENT, int MODE, class Src>
 int launch_cta_rows(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
   const int64_t nvec = in.V / Vec<T>::N;
+  // Vector stores need rows that lie alike (the operators see to it where they can).
+  if (MODE != kFwd && gr.g && !gr.alike) return plain<T, ENT, MODE, Src>(in, out, gr, src, s);
   int size = 1;
   // With the gradient a row stays in the slots (64 KB a CTA).
   if (MODE == kBoth)
@@ -86,15 +88,15 @@ int launch_cta_rows(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr,
       if (each <= 1024) return both<T, ENT, Src, 256, 4, true>(in, out, gr, src, size, s);
       return both<T, ENT, Src, 256, 16, true>(in, out, gr, src, size, s);
     }
-    if (each <= 256) return both<T, ENT, Src, 64, 4, false>(in, out, gr, src, 1, s);
-    if (each <= 512) return both<T, ENT, Src, 64, 8, false>(in, out, gr, src, 1, s);
-    if (each <= 1024) return both<T, ENT, Src, 128, 8, false>(in, out, gr, src, 1, s);
-    if (each <= 2048) return both<T, ENT, Src, 256, 8, false>(in, out, gr, src, 1, s);
+    if (each <= 256) return both<T, ENT, Src, 32, 8, false>(in, out, gr, src, 1, s);
+    if (each <= 512) return both<T, ENT, Src, 32, 16, false>(in, out, gr, src, 1, s);
+    if (each <= 1024) return both<T, ENT, Src, 64, 16, false>(in, out, gr, src, 1, s);
+    if (each <= 2048) return both<T, ENT, Src, 128, 16, false>(in, out, gr, src, 1, s);
     return both<T, ENT, Src, 256, 16, false>(in, out, gr, src, 1, s);
   } else {
     if (size > 1) return stream<T, ENT, MODE, Src, 256, 4, true>(in, out, gr, src, size, s);
-    if (each <= 512) return stream<T, ENT, MODE, Src, 64, 4, false>(in, out, gr, src, 1, s);
-    if (each <= 1024) return stream<T, ENT, MODE, Src, 128, 8, false>(in, out, gr, src, 1, s);
+    if (each <= 1024) return stream<T, ENT, MODE, Src, 32, 8, false>(in, out, gr, src, 1, s);
+    if (each <= 4096) return stream<T, ENT, MODE, Src, 128, 8, false>(in, out, gr, src, 1, s);
     return stream<T, ENT, MODE, Src, 256, 8, false>(in, out, gr, src, 1, s);
   }
 }
