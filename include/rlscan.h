@@ -29,7 +29,7 @@
  *  - Return value: RLS_OK (0) or an RLS_E* status; rls_status_string() names
  *    it.  Launches are asynchronous; device-side failures (a bounded wait that
  *    ran out) are latched in the workspace and read with rls_workspace_error()
- *    (bits: 1 tile look-back, 2 bulk copy, 4 grid barrier).
+ *    (bits: 1 tile look-back, 2 bulk copy, 4 grid barrier, 8 cluster exchange).
  */
 #ifndef RLSCAN_H
 #define RLSCAN_H

@@ -268,6 +268,10 @@ struct Vec<float> {
     split(g[1], f[2], f[3]);
     return pack(f);
   }
+  __device__ __forceinline__ static F2 two(const float* p) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    return f2(v.x, v.y);
+  }
   // The vector's elements, one store each.
   __device__ __forceinline__ static void scatter(float* p, const uint4& u) {
     p[0] = __uint_as_float(u.x); p[1] = __uint_as_float(u.y); p[2] = __uint_as_float(u.z); p[3] = __uint_as_float(u.w);
@@ -324,6 +328,10 @@ struct Vec<__nv_bfloat16> {
 #pragma unroll
     for (int k = 0; k < 4; ++k) split(g[k], f[2 * k], f[2 * k + 1]);
     return pack(f);
+  }
+  __device__ __forceinline__ static F2 two(const __nv_bfloat16* p) {
+    const unsigned w = *reinterpret_cast<const unsigned*>(p);
+    return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
   __device__ __forceinline__ static void scatter(__nv_bfloat16* p, const uint4& u) {
     unsigned short* h = reinterpret_cast<unsigned short*>(p);
@@ -479,9 +487,15 @@ __device__ __forceinline__ float policy_weight(const Policy& p, int64_t env) {
 
 struct PolicyTerm {
   float loss, d;         // the step's term and its derivative by the logprob
-  float kl, drift;
+  float kl;
   bool clipped;
 };
+
+// r - 1 - log r
+__device__ __forceinline__ float drift_of(double lp, float old_lp) {
+  const float lr = (float)(lp - (double)old_lp);
+  return expm1f(lr) - lr;
+}
 
 // -min(r A, clip(r) A), at most -dual A where A < 0, plus the KL estimate:
 // k1 = lp - ref, k2 = (lp - ref)^2 / 2, k3 = exp(ref - lp) - (ref - lp) - 1.
@@ -505,7 +519,6 @@ __device__ __forceinline__ PolicyTerm policy_term(const Policy& p, double lp, fl
     else if (lr64 > p.log_dual) { o.loss = -p.dual * adv; o.clipped = true; }
   }
   if (o.clipped) o.d = 0.f;
-  o.drift = expm1f(lr) - lr;
   o.kl = 0.f;
   if (p.ref) {
     const double x64 = (double)ref - lp;
@@ -598,6 +611,7 @@ struct PolicyGrad {
   const float* g;
   bool force;
   SumOut sums;
+  unsigned* error;  // the workspace's error word
   // the gradient at hand was made for that very scale
   __device__ __forceinline__ bool skip() const { return g && !force && *g == scale; }
   __device__ __forceinline__ float up() const { return g ? *g : scale; }
@@ -805,7 +819,7 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
         if (o.clipped) flags |= kFlagClipped;
         if (threadIdx.x == 0) {
           const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
-          out.stats[2 * row + 1] = make_float4(a, w * term, o.kl, o.drift);
+          out.stats[2 * row + 1] = make_float4(a, w * term, o.kl, drift_of(lp, p.old_lp[row]));
         }
       }
       if (threadIdx.x == 0) {
@@ -879,22 +893,90 @@ __device__ __forceinline__ void store_remote(float4* p, unsigned rank, float4 v)
 
 constexpr int kMostCtas = 8;  // of a cluster (the portable limit)
 
-// Every thread's value to every warp of the row's CTAs: `mine` (one per warp, from
-// lane 0) goes to all CTAs' tables; the tables of two successive calls differ,
-// so that one barrier a call suffices.
-template <int NT, bool CL>
+// Every warp's value to every warp of the row's CTAs: `mine` (one per warp) goes to all
+// CTAs' tables, of which two take turns, so that one barrier a call suffices.
+//
+// Across CTAs there are two ways.  A cluster barrier with release and acquire
+// waits for all of the thread's earlier stores, gradients on their way to memory among
+// them (measured at 131072 bf16 logits: 462 us with it, KASYNC us without, for 4081 rows of
+// loss and gradient); so where there are such stores the values travel as
+// asynchronous stores that count down an mbarrier of the CTA they go to.
+template <int NT, bool CL, bool ASYNC>
 struct Table {
   static constexpr int kWarps = NT / 32;
   static constexpr int kMost = CL ? kWarps * kMostCtas : kWarps;
   float4 at[2][kMost];
+  unsigned long long bar[CL && ASYNC ? 2 : 1];
 };
-template <int NT, bool CL>
-__device__ __forceinline__ const float4* exchange(Table<NT, CL>& t, unsigned& turn, float4 mine, unsigned rank,
+
+__device__ __forceinline__ void bar_init(unsigned long long* bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((unsigned)__cvta_generic_to_shared(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(unsigned long long* bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"((unsigned)__cvta_generic_to_shared(bar)),
+               "r"(bytes) : "memory");
+}
+// Polled without ordering (an acquire at each try would invalidate L1 each time);
+// bar_acquire orders what follows a wait that succeeded.
+__device__ __forceinline__ bool bar_try(unsigned long long* bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"((unsigned)__cvta_generic_to_shared(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void bar_acquire(unsigned long long* bar, unsigned parity) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], %1;\n\t}"
+      ::"r"((unsigned)__cvta_generic_to_shared(bar)), "r"(parity) : "memory");
+}
+__device__ __forceinline__ void store_async(float4* p, unsigned long long* bar, unsigned rank, float4 v) {
+  const unsigned at = (unsigned)__cvta_generic_to_shared(p), b = (unsigned)__cvta_generic_to_shared(bar);
+  unsigned there, its;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(its) : "r"(b), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(there),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(its) : "memory");
+}
+
+constexpr unsigned kTeamWait = 1u << 16;  // tries of a wait on the team, each suspended for a while
+
+// What a thread keeps of its exchanges.
+struct Turns {
+  unsigned n = 0;
+  unsigned* error;      // where a wait that ran out is noted
+  bool broken = false;  // one did: no wait any more (the results are not valid)
+};
+
+template <int NT, bool CL, bool ASYNC>
+__device__ __forceinline__ const float4* exchange(Table<NT, CL, ASYNC>& t, Turns& turn, float4 mine, unsigned rank,
                                                   unsigned size) {
-  float4* tab = t.at[turn & 1];
-  ++turn;
+  const unsigned which = turn.n & 1, parity = (turn.n >> 1) & 1;
+  float4* tab = t.at[which];
+  ++turn.n;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if constexpr (CL) {
+  if constexpr (CL && ASYNC) {
+    // Each warp of the team sends size x 16 bytes; this CTA's barrier gets 16 from each.
+    // A barrier is used again two exchanges on: whoever sends then has had this CTA's
+    // values of the exchange between, which its warps send after this wait.
+    unsigned long long* bar = &t.bar[which];
+    if (threadIdx.x == 0) bar_expect(bar, size * (NT / 32) * 16);
+    if (lane < size) store_async(tab + rank * (NT / 32) + warp, bar, lane, mine);
+    if (!turn.broken) {
+      unsigned tries = 0;
+      while (!bar_try(bar, parity))
+        if (++tries == kTeamWait) {
+          turn.broken = true;
+          if (turn.error) atomicOr(turn.error, 8u);
+          break;
+        }
+      bar_acquire(bar, parity);
+    }
+    turn.broken = __any_sync(0xffffffffu, turn.broken);
+  } else if constexpr (CL) {
     if (lane < size) store_remote(tab + rank * (NT / 32) + warp, lane, mine);
     cluster_barrier();
   } else {
@@ -1063,8 +1145,9 @@ struct Walk {
 
   // The statistics of the row from every thread's share (the vectors; the ends
   // are added here); the same in all threads of the team.
-  __device__ __forceinline__ RowStats join(Run<ENT>& run, int64_t row, const Extra& ex, Table<NT, CL>& table,
-                                           unsigned& turn) const {
+  template <bool ASYNC>
+  __device__ __forceinline__ RowStats join(Run<ENT>& run, int64_t row, const Extra& ex, Table<NT, CL, ASYNC>& table,
+                                           Turns& turn) const {
     const int lane = tid & 31;
     const float c = in.c;
     const T* x = row_at(row);
@@ -1135,30 +1218,36 @@ struct Walk {
     return RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f};
   }
 
-  // Log-probability, entropy and, with the policy loss, the term and the row's
-  // incoming gradients before the scale; one warp of a CTA calls it.
-  __device__ __forceinline__ void outputs(int64_t row, const RowStats& r, const Extra& ex, float& a, float& b) const {
-    const double lp = logprob_of(ex.xt, r, in.c, in.c64, in.c_off);
+  // What a row gives besides its gradient; one warp of a CTA calls these.  The
+  // incoming gradients come first: the other warps wait for them.
+  struct Result {
+    double lp;
+    float ent;
+    PolicyTerm o;
+  };
+  __device__ __forceinline__ Result result(const RowStats& r, const Extra& ex, float& a, float& b) const {
+    Result q{};
+    q.lp = logprob_of(ex.xt, r, in.c, in.c64, in.c_off);
+    if constexpr (Src::kPolicy) {
+      q.o = policy_term(src.p, q.lp, ex.old_lp, ex.adv, ex.ref);
+      a = ex.w * q.o.d;
+      b = ENT ? -ex.w * src.p.ent_coef : 0.f;
+    }
+    return q;
+  }
+  __device__ __forceinline__ void outputs(int64_t row, const RowStats& r, const Extra& ex, const Result& q, float a) const {
+    if (rank != 0 || tid != 0) return;
     float ent = 0.f;
     if constexpr (ENT) ent = entropy_of(r);
     int flags = kFlagKept;
-    const bool writes = rank == 0 && tid == 0;
     if constexpr (Src::kPolicy) {
-      const Policy& p = src.p;
-      const PolicyTerm o = policy_term(p, lp, ex.old_lp, ex.adv, ex.ref);
-      a = ex.w * o.d;
-      b = ENT ? -ex.w * p.ent_coef : 0.f;
-      if (o.clipped) flags |= kFlagClipped;
-      if (writes) {
-        const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
-        out.stats[2 * row + 1] = make_float4(a, ex.w * term, o.kl, o.drift);
-      }
+      const float term = ENT && src.p.ent_coef != 0.f ? q.o.loss - src.p.ent_coef * ent : q.o.loss;
+      if (q.o.clipped) flags |= kFlagClipped;
+      out.stats[2 * row + 1] = make_float4(a, ex.w * term, q.o.kl, drift_of(q.lp, ex.old_lp));
     }
-    if (writes) {
-      out.logprob[row] = (float)lp;
-      if (out.entropy) out.entropy[row] = ent;
-      if (out.stats) out.stats[2 * row] = stats_word(r, flags);
-    }
+    out.logprob[row] = (float)q.lp;
+    if (out.entropy) out.entropy[row] = ent;
+    if (out.stats) out.stats[2 * row] = stats_word(r, flags);
   }
 
   // Writing a row's gradient.
@@ -1248,8 +1337,8 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
   }
   constexpr int M = 2;  // vectors taken at a time
   static_assert(MODE != kBoth && U % M == 0, "streams");
-  __shared__ Table<NT, CL> table;
-  unsigned turn = 0;
+  __shared__ Table<NT, CL, false> table;
+  Turns turn{0, nullptr, false};
   using W = Walk<T, ENT, MODE, Src, NT, CL>;
   W walk(in, out, gr, src);
   const unsigned low = Vec<T>::kLowest;
@@ -1320,7 +1409,10 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
     }
     if constexpr (MODE == kFwd) {
       const RowStats r = walk.join(run, now.row, ex, table, turn);
-      if (walk.rank == 0 && threadIdx.x < 32) walk.outputs(now.row, r, ex, a, b);
+      if (walk.rank == 0 && threadIdx.x < 32) {
+        const typename W::Result q = walk.result(r, ex, a, b);
+        walk.outputs(now.row, r, ex, q, a);
+      }
     } else if (wr.g) {
       walk.finish(wr, now.row, ex, [&] { return make_float4(a, b, ex.stats.y, ex.stats.z); });
     }
@@ -1339,9 +1431,9 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
   constexpr int M = 2;
   static_assert(K % M == 0, "whole groups");
   extern __shared__ uint4 slots[];  // [K][NT]
-  __shared__ Table<NT, CL> table;
+  __shared__ Table<NT, CL, true> table;
   __shared__ float4 incoming;       // (a, b, S0, t) of the row, from the warp that formed them
-  unsigned turn = 0;
+  Turns turn{0, src.error, false};
   using W = Walk<T, ENT, kBoth, Src, NT, CL>;
   W walk(in, out, gr, src);
   uint4* mine = slots + threadIdx.x;
@@ -1357,7 +1449,14 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
 #pragma unroll
   for (int j = 0; j < K; ++j) fetch(now, j);
   walk.token_logit(first, ex);
-  if constexpr (CL) cluster_barrier();  // the others' tables exist
+  if constexpr (CL) {  // the others' tables exist, their barriers are set
+    if (threadIdx.x == 0) {
+      bar_init(&table.bar[0]);
+      bar_init(&table.bar[1]);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    cluster_barrier();
+  }
   for (;;) {
     Run<ENT> run(in.c);
 #pragma unroll
@@ -1372,9 +1471,12 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
       run.template add_vectors<T, M>(u, in.c);
     }
     const RowStats r = walk.join(run, now.row, ex, table, turn);
+    typename W::Result q;
+    float own = 0.f;
     if (threadIdx.x < 32) {
-      float a = 0.f, b = 0.f;
-      walk.outputs(now.row, r, ex, a, b);
+      float b = 0.f;
+      q = walk.result(r, ex, own, b);
+      float a = own;
       walk.scaled(ex, a, b);
       if (threadIdx.x == 0) incoming = make_float4(a, b, r.s0, r.t);
     }
@@ -1386,6 +1488,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
       nx = walk.extra(row);
     }
     __syncthreads();
+    if (threadIdx.x < 32) walk.outputs(now.row, r, ex, q, own);
     const typename W::Writer wr = walk.writer(now.row, r, incoming.x, incoming.y);
     if (wr.g && !wr.sh.far) {
 #pragma unroll
@@ -1404,9 +1507,225 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
     now = next;
     ex = nx;
   }
+  // No CTA leaves while another might still store to it (after a wait that ran out).
+  if constexpr (CL) cluster_barrier();
 }
 
-// ---- short rows: G lanes a row, E elements a lane, the row in registers ------------
+// ---- short rows in tiles ---------------------------------------------------------
+// Rows that lie one after the other, each of few logits: a CTA copies a tile of R whole rows
+// (R a power of two, the tile 16-byte aligned) to shared memory as one
+// stretch, G = 256 / R lanes (at most 32) sum up each row, one thread a row then forms its
+// log-probability, loss term and coefficients -- the fp64 and the transcendental steps
+// that would cost a whole warp's time with a warp a row -- and the gradient is
+// written over the stretch again, by vectors that need not respect the rows.
+// ACC: how a lane reads a row: 0 one element, 1 two (V even), 2 a 16-byte vector (rows are whole vectors).
+constexpr int kTileThreads = 256;
+constexpr int kTileCtas = 5;  // an SM: 48 registers a thread
+
+struct TileShape {
+  int rows, log_lanes; // R, log2 G
+  int turn;            // a row's lanes start `turn` rounds further than the last row's do (bank conflicts), ...
+  int rounds;          // ... of so many whole ones
+  Divide by_vocab;     // an element's row
+};
+
+template <class T, bool ENT, int MODE, class Src, int ACC>
+__global__ void __launch_bounds__(kTileThreads, kTileCtas) tile_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src,
+                                                                    TileShape shape) {
+  if constexpr (Src::kPolicy && MODE == kBwd) {
+    if (src.skip()) return;
+  }
+  constexpr int N = Vec<T>::N;
+  constexpr bool kTerms = Src::kPolicy && MODE != kBwd;
+  extern __shared__ uint4 tile[];
+  __shared__ float4 found[kTileThreads];  // a row's m, S0, S1; then its m, A, B and whether it has a gradient
+  const T* elems = reinterpret_cast<const T*>(tile);
+  const int tid = threadIdx.x, V = in.V, R = shape.rows, G = 1 << shape.log_lanes;
+  const float c = in.c;
+  double sum[kTerms ? kSums : 1] = {};
+  const int r = tid >> shape.log_lanes, lane = tid & (G - 1);
+  const int first = lane + (shape.turn ? r % shape.rounds * G : 0);
+  const int64_t tiles = (in.rows + R - 1) / R;
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int64_t row0 = t * R;
+    const int rows = (int)(in.rows - row0 < R ? in.rows - row0 : R);
+    const int count = rows * V, vecs = count / N;
+    const T* x = in.x + row0 * V;
+    for (int v = tid; v < vecs; v += kTileThreads) copy16(tile + v, reinterpret_cast<const uint4*>(x) + v);
+    copy_commit();
+    for (int i = vecs * N + tid; i < count; i += kTileThreads) reinterpret_cast<T*>(tile)[i] = x[i];
+    // what the row's thread needs, asked for meanwhile
+    const int64_t row = row0 + tid;
+    const bool own = tid < rows;
+    bool kept = false;
+    int64_t tok = 0;
+    float old_lp = 0.f, adv = 0.f, ref = 0.f, w = 0.f, a = 0.f, b = 0.f;
+    if (own) {
+      kept = mask_at(in.mask, row);
+      if (kept) tok = in.tokens[row];
+      if constexpr (Src::kPolicy) {
+        const int64_t env = in.env(row);
+        old_lp = src.p.old_lp[row];
+        adv = src.p.adv[src.p.adv_row ? env : row];
+        if (src.p.ref) ref = src.p.ref[row];
+        if (kept) w = policy_weight(src.p, env);
+      } else if constexpr (MODE == kBwd) {
+        if (src.g_lp) a = src.g_lp[row];
+        if constexpr (ENT) b = src.g_ent[row];
+      }
+    }
+    copy_wait<0>();
+    __syncthreads();
+    // ---- a row's sums, by its lanes
+    if (r < R) {  // whole warps
+      const bool there = r < rows;
+      const T* line = elems + r * V;
+      constexpr int W = ACC == 2 ? N : ACC == 1 ? 2 : 1;
+      const int n = there ? V / W : 0;         // accesses of the row, lane, lane + G, ... of which are this lane's
+      auto load = [&](int k, F2 (&f)[ACC == 2 ? N / 2 : 1]) {
+        if constexpr (ACC == 2) {
+          const uint4 u = reinterpret_cast<const uint4*>(line)[k];
+#pragma unroll
+          for (int q = 0; q < N / 2; ++q) f[q] = Vec<T>::pair(u, q);
+        } else if constexpr (ACC == 1) {
+          f[0] = Vec<T>::two(line + 2 * k);
+        } else {
+          f[0] = f2(Vec<T>::get(line + k), -INFINITY);
+        }
+      };
+      // the lane's accesses from `first` on, then those before it
+      auto each = [&](auto&& f) {
+        for (int k = first; k < n; k += G) f(k);
+        for (int k = lane; k < first && k < n; k += G) f(k);
+      };
+      float m = -INFINITY;
+      each([&](int k) {
+        F2 f[ACC == 2 ? N / 2 : 1];
+        load(k, f);
+#pragma unroll
+        for (int q = 0; q < (ACC == 2 ? N / 2 : 1); ++q) {
+          float y, z;
+          split(f[q], y, z);
+          m = fmaxf(m, fmaxf(y, z));
+        }
+      });
+      for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      F2 s0 = f2(0.f, 0.f), s1 = s0;
+      const F2 nm = f2(-m, -m), cc = f2(c, c);
+      each([&](int k) {
+        F2 f[ACC == 2 ? N / 2 : 1];
+        load(k, f);
+#pragma unroll
+        for (int q = 0; q < (ACC == 2 ? N / 2 : 1); ++q) {
+          const F2 d = mul2(add2(f[q], nm), cc);
+          float y, z;
+          split(d, y, z);
+          const F2 e = f2(ex2(y), ex2(z));
+          s0 = add2(s0, e);
+          s1 = fma2(e, f2(fmaxf(y, kDeep), fmaxf(z, kDeep)), s1);
+        }
+      });
+      float p0, p1, y;
+      split(s0, p0, y);
+      p0 += y;
+      split(s1, p1, y);
+      p1 += y;
+      for (int o = G / 2; o > 0; o >>= 1) {
+        p0 += __shfl_xor_sync(0xffffffffu, p0, o);
+        p1 += __shfl_xor_sync(0xffffffffu, p1, o);
+      }
+      if (lane == 0) found[r] = make_float4(m, p0, p1, 0.f);
+    }
+    __syncthreads();
+    // ---- a row's results, by its thread
+    float at_token = 0.f;
+    bool has = false;
+    if (own) {
+      const float4 q = found[tid];
+      const RowStats st{q.x, q.y, q.z / q.y, true, q.y == 1.f && q.z == 0.f};
+      const bool ok = tok >= 0 && tok < V;
+      const float xt = ok ? Vec<T>::get(elems + tid * V + (int)tok) : NAN;
+      double lp = 0.0;
+      float ent = 0.f;
+      if (kept) {
+        if constexpr (Src::kPolicy || MODE != kBwd) lp = logprob_of(xt, st, c, in.c64, in.c_off);
+        if constexpr (ENT && MODE != kBwd) ent = entropy_of(st);
+        if constexpr (Src::kPolicy) {
+          const Policy& p = src.p;
+          const PolicyTerm o = policy_term(p, lp, old_lp, adv, ref);
+          a = w * o.d;
+          if constexpr (ENT) b = -w * p.ent_coef;
+          if constexpr (kTerms) {
+            const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
+            sum[0] += (double)w * (double)term;
+            sum[1] += o.kl; sum[2] += drift_of(lp, old_lp); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent;
+            sum[5] += 1.0;
+          }
+          a *= src.up();
+          b *= src.up();
+        }
+        if (!ok) a = NAN;
+      } else {
+        a = b = 0.f;
+      }
+      if constexpr (MODE != kBwd) {
+        out.logprob[row] = (float)lp;
+        if (out.entropy) out.entropy[row] = ent;
+      }
+      if constexpr (MODE != kFwd) {
+        has = a != 0.f || b != 0.f;
+        const RowGrad rg = row_grad(a, b, st, in.inv_temp);
+        found[tid] = make_float4(st.m, -rg.A, -rg.B, has ? 1.f : 0.f);
+        has = has && ok;
+        if (has) at_token = token_grad(xt, Shift{c, st.m, true}, a, b, st.s0, st.t, in.inv_temp);
+      }
+    }
+    // ---- the gradient over the stretch
+    if constexpr (MODE != kFwd) {
+      __syncthreads();
+      T* g = gr.g;
+      if (g) {
+        g += row0 * V;
+        auto at = [&](float y, const float4& q) {
+          const float d = (y - q.x) * c, e = ex2(d);
+          const float v = ENT ? e * fmaf(q.z, fmaxf(d, kDeep), q.y) : e * q.y;
+          return q.w != 0.f ? v : 0.f;
+        };
+        for (int v = tid; v < vecs; v += kTileThreads) {
+          const uint4 u = tile[v];
+          float f[N];
+          Vec<T>::unpack(u, f);
+          int line = (int)shape.by_vocab(v * N);
+          float4 q = found[line];
+          if constexpr (ACC == 2) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = at(f[e], q);
+          } else {
+            int left = (line + 1) * V - v * N;  // elements to the end of the row
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              if (left == 0) {
+                q = found[++line];
+                left = V;
+              }
+              f[e] = at(f[e], q);
+              --left;
+            }
+          }
+          __stcs(reinterpret_cast<uint4*>(g) + v, Vec<T>::pack(f));
+        }
+        for (int i = vecs * N + tid; i < count; i += kTileThreads)
+          g[i] = Vec<T>::put(at(Vec<T>::get(elems + i), found[(int)shape.by_vocab(i)]));
+        __syncthreads();  // the token's element goes over what its vector holds
+        if (has) g[(int64_t)tid * V + tok] = Vec<T>::put(at_token);
+      }
+    }
+    __syncthreads();  // the tile is read
+  }
+  if constexpr (kTerms) finish_sums<kTileThreads>(sum, src.sums);
+}
+
+// ---- short rows anywhere: G lanes a row, E elements a lane, the row in registers -----
 // Each CTA takes tiles of 256 / G rows in strides of the grid; with the policy
 // loss it adds up its own rows' terms on the way.
 template <class T, bool ENT, int MODE, class Src, int G, int E>
@@ -1474,7 +1793,7 @@ __global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, 
           if (live && lane == 0) {
             const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
             sum[0] += (double)w * (double)term;
-            sum[1] += o.kl; sum[2] += o.drift; sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent; sum[5] += 1.0;
+            sum[1] += o.kl; sum[2] += drift_of(lp, p.old_lp[row]); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent; sum[5] += 1.0;
           }
         }
         a *= src.up();

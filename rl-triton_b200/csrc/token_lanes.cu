@@ -1,6 +1,7 @@
 // token_lanes.cu -- the logits kernels for short rows (discrete actions, small
-// vocabularies): a group of lanes holds a row in registers, so the gradient
-// pass needs no second read and no statistics from an earlier call.
+// vocabularies): tiles of rows in shared memory, or, where the rows do not lie one after the
+// other, a group of lanes holds a row in registers.  Either way the gradient
+// needs no statistics from an earlier call.
 #include "token_launch.h"
 
 namespace rls {
@@ -17,11 +18,51 @@ int go(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& s
   return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
 }
 
+// The most lanes of a warp that a row's accesses bring to one bank (4-byte words).
+int conflicts(int lanes, int words, int pitch, int turn) {
+  int bank[32] = {0}, most = 0;
+  for (int l = 0; l < 32; ++l) {
+    const int at = (l / lanes) * pitch + (l % lanes + (l / lanes) * turn * lanes) * words;
+    const int n = ++bank[at & 31];
+    if (n > most) most = n;
+  }
+  return most;
+}
+
+template <class T, bool ENT, int MODE, class Src, int ACC>
+int tiles(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
+  const int line = in.V * (int)sizeof(T);
+  // About 20 KB a tile, so that a dozen tiles fit on an SM; at least 8 rows, which
+  // are whole vectors for any V.
+  TileShape sh{};
+  sh.rows = 8;
+  while (sh.rows < kTileThreads && 2 * sh.rows * line <= 20 * 1024) sh.rows *= 2;
+  const int lanes = kTileThreads / sh.rows < 32 ? kTileThreads / sh.rows : 32;
+  while ((1 << sh.log_lanes) < lanes) ++sh.log_lanes;
+  const int words = ACC == 2 ? 4 : ACC == 1 ? (int)sizeof(T) / 2 : 1;
+  sh.turn = ACC != 2 && sizeof(T) == 4 && conflicts(lanes, words, in.V, 1) < conflicts(lanes, words, in.V, 0);
+  sh.rounds = in.V / (words * lanes) > 0 ? in.V / (words * lanes) : 1;
+  sh.by_vocab = Divide::of(in.V, 0);
+  const size_t smem = ((size_t)sh.rows * line + 15) / 16 * 16;  // at most 32 KB (8 rows of 1024 fp32)
+  auto kern = tile_rows_kernel<T, ENT, MODE, Src, ACC>;
+  const int64_t all = (in.rows + sh.rows - 1) / sh.rows, fit = sum_blocks(1 << 30) / 8 * kTileCtas;
+  const int64_t blocks = all < fit ? all : fit;
+  kern<<<(unsigned)blocks, kTileThreads, smem, s>>>(in, out, gr, src, sh);
+  return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
+}
+
 }  // namespace
 
 template <class T, bool ENT, int MODE, class Src>
 int launch_lane_rows(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src& src, cudaStream_t s) {
   const int64_t V = in.V;
+  // Rows (and their gradients) one after the other from a 16-byte boundary on.
+  const bool whole = in.flat && in.ss == V && ((uintptr_t)in.x & 15) == 0;
+  if (whole && (MODE == kFwd || !gr.g || (gr.flat && gr.ss == V && ((uintptr_t)gr.g & 15) == 0))) {
+    if (V * sizeof(T) % 16 == 0) return tiles<T, ENT, MODE, Src, 2>(in, out, gr, src, s);
+    if (V % 2 == 0) return tiles<T, ENT, MODE, Src, 1>(in, out, gr, src, s);
+    return tiles<T, ENT, MODE, Src, 0>(in, out, gr, src, s);
+  }
   if (V <= 4) return go<T, ENT, MODE, Src, 1, 4>(in, out, gr, src, s);
   if (V <= 8) return go<T, ENT, MODE, Src, 2, 4>(in, out, gr, src, s);
   if (V <= 16) return go<T, ENT, MODE, Src, 4, 4>(in, out, gr, src, s);

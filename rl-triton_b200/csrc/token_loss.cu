@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Terms t, float scale, 
         d[e] = w * o.d * up;
         if constexpr (SUMS) {
           sum[0] += (double)w * (double)o.loss;
-          sum[1] += o.kl; sum[2] += o.drift; sum[3] += o.clipped ? 1.0 : 0.0; sum[5] += 1.0;
+          sum[1] += o.kl; sum[2] += drift_of((double)lp[e], old_lp[e]); sum[3] += o.clipped ? 1.0 : 0.0; sum[5] += 1.0;
         }
       }
       if (++col == t.T) { col = 0; ++env; }
@@ -434,7 +434,7 @@ extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, in
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   const Policy p = make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm,
                                mask != nullptr, num_envs, seq_len);
-  PolicyGrad src{p, grad_scale, nullptr, false, SumOut{}};
+  PolicyGrad src{p, grad_scale, nullptr, false, SumOut{}, &static_cast<WsHeader*>(ws)->error};
   const int64_t blocks = sum_blocks((M + kThreads - 1) / kThreads);
   if (int st = sums_in(ws, ws_bytes, sum_blocks(M), loss, stats, s, &src.sums)) return st;
   if (int st = launch_count(p, c.mask, norm, num_envs, seq_len, ws, s)) return st;
@@ -471,6 +471,6 @@ extern "C" int rls_policy_loss_logits_backward(const void* logits, int64_t env_s
   const Policy p = make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm,
                                mask != nullptr, num_envs, seq_len);
   const RowOut ro{nullptr, nullptr, reinterpret_cast<float4*>(const_cast<float*>(row_stats))};
-  return launch_logits<kBwd>(c, policy->entropy_coef != 0.f, ro, PolicyGrad{p, grad_scale, grad_loss, force != 0, SumOut{}},
+  return launch_logits<kBwd>(c, policy->entropy_coef != 0.f, ro, PolicyGrad{p, grad_scale, grad_loss, force != 0, SumOut{}, nullptr},
                              reinterpret_cast<cudaStream_t>(stream));
 }
