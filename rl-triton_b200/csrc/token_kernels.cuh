@@ -7,7 +7,7 @@
 //   d logprob / d x_v = (1[v = tok] - p_v) / temperature,
 //   d H / d x_v       = -p_v (log p_v + H) / temperature.
 // Everything is computed in base 2: with c = log2(e) / temperature and an
-// offset M (an element near the maximum, times c, rounded to a whole number),
+// offset M (an element near the maximum, times c, rounded to a whole number, and 9),
 //   d_v = x_v c - M,  S0 = sum 2^d_v,  S1 = sum 2^d_v d_v,  t = S1 / S0,
 //   logprob = ln2 (d_tok - log2 S0),   H = ln2 (log2 S0 - t),
 // one fused multiply-add and one ex2 an element, and the gradient for incoming
@@ -31,12 +31,14 @@ constexpr float kLn2 = 0.693147180559945309f;
 // (logits at the type's lowest value in a whole row, infinities), x c - M is
 // useless and S0 leaves [kLeast, kMost]; such rows, and rows with NaN, are
 // summed again with d = (x - m) c, the far form.
-constexpr float kFar = 1e30f;
-constexpr float kLeast = 0.25f, kMost = 1e18f;
-// An offset stays until an element lies this far (in powers of two) above it: any offset
-// near the maximum serves, and a warp whose lanes each kept their own maximum
-// would move one of them at almost every step.
-constexpr float kSlack = 24.f;
+constexpr float kFar = 1e15f;
+constexpr float kLeast = 2e-4f, kMost = 1e12f;
+// An offset stays until an element lies this far (in powers of two) above where
+// it put its own: any offset near the maximum serves, and a warp whose lanes each kept
+// their own maximum would move one of them at almost every step.  Offsets lie kLift above the
+// element, so that every d is below 0: ex2.approx is off to one side there, to
+// the other above 0 (see logprob_of).
+constexpr float kSlack = 8.f, kLift = 9.f;
 constexpr float kDeep = -16384.f;  // 2^kDeep is 0: keeps 2^d * d finite at d = -inf
 
 __device__ __forceinline__ float ex2(float x) {
@@ -178,9 +180,9 @@ struct Shift {
   bool far;
   __device__ __forceinline__ float operator()(float x) const { return far ? (x - off) * c : fmaf(x, c, -off); }
 };
-// What d is taken from: m c to a whole number.  Sums move to a larger offset by a
+// What d is taken from: m c to a whole number, and kLift.  Sums move to a larger offset by a
 // power of two then, exactly (ex2.approx of a whole number is one).
-__device__ __forceinline__ float offset_of(float m, float c) { return rintf(m * c); }
+__device__ __forceinline__ float offset_of(float m, float c) { return rintf(m * c) + kLift; }
 __device__ __forceinline__ Shift shift_of(const RowStats& r, float c) {
   return Shift{c, r.far ? r.m : offset_of(r.m, c), r.far};
 }
@@ -196,7 +198,8 @@ __device__ __forceinline__ double log2_of(float s0) {
 // all rows are taken out to first order, since sums of many log-probabilities
 // (the preference loss's) would add them up: c was rounded, which moves log S0 by
 // the mean of d times the relative error; and ex2.approx lies 5.0e-8 low on
-// average (measured over d in (-8, 0)), except at the far form's maximum, where d is 0.
+// average for d below 0 (measured; 3.4e-8 high above), except at the far form's
+// maximum, where d is 0.
 __device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c, double c64, double c_off) {
   const Shift sh = shift_of(r, c);
   if (ex2(sh(x_tok)) == r.s0) return 0.0;  // the others are below fp32's reach
@@ -246,10 +249,10 @@ struct Vec<float> {
   __device__ __forceinline__ static uint4 pack(const float (&f)[4]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
-  // -inf becomes finite (and as good as -inf); NaN stays.
+  // -inf becomes finite (and as good as -inf: 2^d is 0, and the products with d stay finite); NaN stays.
   __device__ __forceinline__ static uint4 bound(const uint4& u) {
     uint4 o;
-    constexpr unsigned low = 0xfb800000u;  // -2^120
+    constexpr unsigned low = 0xdd800000u;  // -2^60, below -kFar
     asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.x) : "r"(u.x), "r"(low));
     asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.y) : "r"(u.y), "r"(low));
     asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.z) : "r"(u.z), "r"(low));
@@ -308,7 +311,7 @@ struct Vec<__nv_bfloat16> {
   }
   __device__ __forceinline__ static uint4 bound(const uint4& u) {
     uint4 o;
-    constexpr unsigned low = 0xfb80fb80u;  // -2^120
+    constexpr unsigned low = 0xdd80dd80u;  // -2^60, below -kFar
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.x) : "r"(u.x), "r"(low));
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.y) : "r"(u.y), "r"(low));
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.z) : "r"(u.z), "r"(low));
@@ -384,7 +387,7 @@ struct Run {
     float mx = x[0];
 #pragma unroll
     for (int k = 1; k < K; ++k) mx = fmaxf(mx, x[k]);
-    if (fmaf(mx, c, -off) > kSlack) raise(mx, c);
+    if (fmaf(mx, c, -off) > kSlack - kLift) raise(mx, c);
     float e[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -411,7 +414,7 @@ struct Run {
 #pragma unroll
     for (int k = 1; k < M; ++k) mx = fmaxf(mx, Vec<T>::top(u[k]));
     float dm = fmaf(mx, c, -off);
-    if (dm > kSlack) {
+    if (dm > kSlack - kLift) {
       raise(mx, c);
       dm = fmaf(mx, c, -off);
     }
@@ -1658,8 +1661,10 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) tile_rows_kernel(Rows
           if constexpr (kTerms) {
             const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
             sum[0] += (double)w * (double)term;
-            sum[1] += o.kl; sum[2] += drift_of(lp, old_lp); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent;
-            sum[5] += 1.0;
+            if (src.sums.stats) {
+              sum[1] += o.kl; sum[2] += drift_of(lp, old_lp); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent;
+              sum[5] += 1.0;
+            }
           }
           a *= src.up();
           b *= src.up();

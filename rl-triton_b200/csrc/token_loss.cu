@@ -77,6 +77,7 @@ struct Terms {
   Policy p;
   Mask mask;
   int64_t M, T;
+  Divide env;
 };
 
 __device__ __forceinline__ void load4(const float* p, int64_t i, int64_t M, float (&o)[4]) {
@@ -90,23 +91,52 @@ __device__ __forceinline__ void load4(const float* p, int64_t i, int64_t M, floa
 }
 
 // One pass over the steps: the sums of the loss and the statistics (SUMS) and
-// the gradient (GRAD).
-template <bool SUMS, bool GRAD>
-__global__ void __launch_bounds__(kThreads) policy_kernel(Terms t, float scale, const float* g, int force, float* grad,
-                                                          SumOut out) {
+// the gradient (GRAD).  A batch of at most kAlone steps is one CTA's, which then counts
+// the steps itself first (COUNT; norm is written as count_kernel does): one launch instead of two, where
+// the launches are most of the time.
+constexpr int kAlone = 8192, kAloneThreads = 1024;
+
+template <int NT>
+__device__ __forceinline__ void count_alone(const Mask& mask, int N, int T, int reduction, float* norm) {
+  __shared__ unsigned total, some;
+  if (threadIdx.x == 0) total = some = 0u;
+  __syncthreads();
+  // a warp a row
+  for (int n = threadIdx.x >> 5; n < N; n += NT / 32) {
+    unsigned c = 0;
+    for (int t = threadIdx.x & 31; t < T; t += 32) c += mask_at(mask, (int64_t)n * T + t) ? 1u : 0u;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if ((threadIdx.x & 31) == 0) {
+      norm[1 + n] = (float)c;
+      atomicAdd(&total, c);
+      if (c) atomicAdd(&some, 1u);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const double by = reduction == RLS_REDUCE_SEQUENCE ? (double)some : (double)total;
+    norm[0] = by > 0.0 ? (float)(1.0 / by) : 0.f;
+  }
+  __syncthreads();
+}
+
+template <bool SUMS, bool GRAD, bool COUNT, int NT>
+__global__ void __launch_bounds__(NT) policy_kernel(Terms t, float scale, const float* g, int force, float* grad,
+                                                    float* norm, SumOut out) {
   if constexpr (!SUMS) {
     if (g && !force && *g == scale) return;
   }
+  if constexpr (COUNT) count_alone<NT>(t.mask, (int)(t.M / t.T), (int)t.T, t.p.reduction, norm);
   const float up = g ? *g : scale;
   double sum[kSums] = {0, 0, 0, 0, 0, 0};
-  const int64_t step = (int64_t)gridDim.x * kThreads * 4;
-  for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; i < t.M; i += step) {
+  const int64_t step = (int64_t)gridDim.x * NT * 4;
+  for (int64_t i = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4; i < t.M; i += step) {
     float lp[4], old_lp[4], adv[4], ref[4], d[4];
     load4(t.lp, i, t.M, lp);
     load4(t.p.old_lp, i, t.M, old_lp);
     if (!t.p.adv_row) load4(t.p.adv, i, t.M, adv);
     if (t.p.ref) load4(t.p.ref, i, t.M, ref);
-    int64_t env = i / t.T, col = i - env * t.T;
+    int64_t env = t.env(i), col = i - env * t.T;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       d[e] = 0.f;
@@ -117,7 +147,10 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Terms t, float scale, 
         d[e] = w * o.d * up;
         if constexpr (SUMS) {
           sum[0] += (double)w * (double)o.loss;
-          sum[1] += o.kl; sum[2] += drift_of((double)lp[e], old_lp[e]); sum[3] += o.clipped ? 1.0 : 0.0; sum[5] += 1.0;
+          if (out.stats) {
+            sum[1] += o.kl; sum[2] += drift_of((double)lp[e], old_lp[e]); sum[3] += o.clipped ? 1.0 : 0.0;
+            sum[5] += 1.0;
+          }
         }
       }
       if (++col == t.T) { col = 0; ++env; }
@@ -132,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) policy_kernel(Terms t, float scale, 
       }
     }
   }
-  if constexpr (SUMS) finish_sums<kThreads>(sum, out);
+  if constexpr (SUMS) finish_sums<NT>(sum, out);
 }
 
 // The policy loss over long rows: their records' terms.
@@ -367,15 +400,23 @@ extern "C" int rls_policy_loss(const float* logprobs, const float* old_logprobs,
   Terms t{logprobs,
           make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm, mask != nullptr,
                       num_envs, seq_len),
-          Mask{mask, mask_kind}, M, seq_len};
+          Mask{mask, mask_kind}, M, seq_len, Divide::of(seq_len, M)};
   SumOut sums;
-  const int64_t blocks = policy_blocks(M);
+  const bool alone = M <= kAlone;
+  const int64_t blocks = alone ? 1 : policy_blocks(M);
   if (int st = sums_in(ws, ws_bytes, blocks, loss, stats, s, &sums)) return st;
-  if (int st = launch_count(t.p, t.mask, norm, num_envs, seq_len, ws, s)) return st;
-  if (grad_logprobs)
-    policy_kernel<true, true><<<(unsigned)blocks, kThreads, 0, s>>>(t, grad_scale, nullptr, 0, grad_logprobs, sums);
-  else
-    policy_kernel<true, false><<<(unsigned)blocks, kThreads, 0, s>>>(t, grad_scale, nullptr, 0, nullptr, sums);
+  if (alone) {
+    const bool count = t.p.norm != nullptr;
+    auto kern = grad_logprobs ? (count ? policy_kernel<true, true, true, kAloneThreads>
+                                       : policy_kernel<true, true, false, kAloneThreads>)
+                              : (count ? policy_kernel<true, false, true, kAloneThreads>
+                                       : policy_kernel<true, false, false, kAloneThreads>);
+    kern<<<1, kAloneThreads, 0, s>>>(t, grad_scale, nullptr, 0, grad_logprobs, norm, sums);
+  } else {
+    if (int st = launch_count(t.p, t.mask, norm, num_envs, seq_len, ws, s)) return st;
+    auto kern = grad_logprobs ? policy_kernel<true, true, false, kThreads> : policy_kernel<true, false, false, kThreads>;
+    kern<<<(unsigned)blocks, kThreads, 0, s>>>(t, grad_scale, nullptr, 0, grad_logprobs, nullptr, sums);
+  }
   return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
 }
 
@@ -399,9 +440,10 @@ extern "C" int rls_policy_loss_backward(const float* logprobs, const float* old_
   Terms t{logprobs,
           make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm, mask != nullptr,
                       num_envs, seq_len),
-          Mask{mask, mask_kind}, M, seq_len};
-  policy_kernel<false, true><<<(unsigned)policy_blocks(M), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      t, grad_scale, grad_loss, force, grad_logprobs, SumOut{});
+          Mask{mask, mask_kind}, M, seq_len, Divide::of(seq_len, M)};
+  policy_kernel<false, true, false, kThreads>
+      <<<(unsigned)policy_blocks(M), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+          t, grad_scale, grad_loss, force, grad_logprobs, nullptr, SumOut{});
   return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
 }
 

@@ -19,8 +19,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/custom_class.h>
 #include <torch/library.h>
 
+#include <mutex>
 #include <tuple>
 #include <utility>
 
@@ -161,17 +163,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_policy(const Tensor& logprobs, con
                                                      const Tensor& advantages, const OptT& mask, const OptT& ref,
                                                      double clip_low, double clip_high, double dual_clip,
                                                      double kl_coef, int64_t kl, int64_t reduction, double grad_scale,
-                                                     bool need_grad) {
+                                                     bool need_stats, bool need_grad) {
   const Tensor lp = f32(logprobs), old_lp = f32(old_logprobs), adv = f32(advantages);
   const OptT rf = f32(ref);
   const MaskArg m = mask_arg(mask);
   const int64_t n = lp.size(0), t = lp.size(1);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, 0.0, reduction);
-  Tensor loss = like(lp, {}), stats = like(lp, {5}), norm = norm_for(m, lp, n, reduction);
+  Tensor loss = like(lp, {}), stats = like(lp, {need_stats ? 5 : 0}), norm = norm_for(m, lp, n, reduction);
   Tensor grad = like(lp, need_grad ? at::IntArrayRef({n, t}) : at::IntArrayRef({0}));
   Tensor ws = policy_workspace(lp);
   check(rls_policy_loss(F(lp), F(old_lp), F(adv), adv.dim() == 1, F(rf), m.ptr(), m.kind, &p, (float)grad_scale,
-                        W(norm), loss.data_ptr<float>(), stats.data_ptr<float>(), W(grad), n, t, ws.data_ptr(),
+                        W(norm), loss.data_ptr<float>(), W(stats), W(grad), n, t, ws.data_ptr(),
                         (size_t)ws.numel(), stream_of(lp)),
         "rls_policy_loss");
   return {loss, stats, norm, grad};
@@ -195,19 +197,19 @@ void op_policy_backward_(Tensor& grad, const Tensor& logprobs, const Tensor& old
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_policy_logits(
     const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
     const OptT& mask, const OptT& ref, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
-    double entropy_coef, bool entropy, double temperature, int64_t reduction, double grad_scale, bool need_grad) {
+    double entropy_coef, bool need_stats, double temperature, int64_t reduction, double grad_scale, bool need_grad) {
   const LogitsArgs a(logits, tokens, mask);
   const Tensor old_lp = f32(old_logprobs), adv = f32(advantages);
   const OptT rf = f32(ref);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
-  Tensor loss = like(a.x, {}), stats = like(a.x, {5}), norm = norm_for(a.mask, a.x, a.n, reduction);
+  Tensor loss = like(a.x, {}), stats = like(a.x, {need_stats ? 5 : 0}), norm = norm_for(a.mask, a.x, a.n, reduction);
   Tensor lp = like(a.x, {a.n, a.t}), rows = row_stats(a, true);
-  Tensor ent = like(a.x, entropy || entropy_coef != 0.0 ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
+  Tensor ent = like(a.x, need_stats || entropy_coef != 0.0 ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
   Tensor g = need_grad ? op_grad_buffer(a.x) : at::empty({0}, a.x.options());
   Tensor ws = policy_workspace(a.x);
   check(rls_policy_loss_logits(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), F(old_lp),
                                F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, &p, (float)grad_scale,
-                               W(norm), W(lp), W(ent), W(rows), loss.data_ptr<float>(), stats.data_ptr<float>(),
+                               W(norm), W(lp), W(ent), W(rows), loss.data_ptr<float>(), W(stats),
                                need_grad ? g.data_ptr() : nullptr, need_grad ? g.stride(0) : 0,
                                need_grad ? g.stride(1) : 0, a.n, a.t, a.v, temperature, dtype_of(a.x),
                                ws.data_ptr(), (size_t)ws.numel(), stream_of(a.x)),
@@ -340,6 +342,23 @@ auto op_handle(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
 }
 
+// What a policy loss keeps for its backward call besides tensors: the
+// arguments, and the gradient written by the forward call until it is handed out.
+struct Kept : public torch::CustomClassHolder {
+  double clip_low, clip_high, dual_clip, kl_coef, entropy_coef = 0.0, temperature = 1.0, grad_scale;
+  int64_t kl, reduction;
+  Tensor grad;
+  // The gradient's buffer, once; an undefined tensor after that.
+  Tensor take() {
+    std::lock_guard<std::mutex> lock(mu);
+    return std::exchange(grad, Tensor());
+  }
+  std::mutex mu;
+};
+Kept& kept_of(AutogradContext* ctx) {
+  return *static_cast<Kept*>(ctx->saved_data.begin()->second.toCapsule().get());
+}
+
 Tensor call_grad_buffer(const Tensor& logits) {
   static auto op = op_handle<Tensor(const Tensor&)>("rl_triton::_grad_buffer");
   return op.call(logits);
@@ -382,37 +401,32 @@ std::tuple<Tensor, Tensor> token_logprobs_autograd(const Tensor& logits, const T
 struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
   static variable_list forward(AutogradContext* ctx, const Tensor& lp, const Tensor& old_lp, const Tensor& adv,
                                const OptT& mask, const OptT& ref, double clip_low, double clip_high, double dual_clip,
-                               double kl_coef, int64_t kl, int64_t reduction, double grad_scale) {
+                               double kl_coef, int64_t kl, int64_t reduction, double grad_scale, bool need_stats) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = op_handle<decltype(op_policy)>("rl_triton::_policy_loss");
     auto [loss, stats, norm, grad] = op.call(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl,
-                                             reduction, grad_scale, true);
+                                             reduction, grad_scale, need_stats, true);
     ctx->save_for_backward({lp, old_lp, adv, plain(mask), plain(ref), norm});
-    ctx->saved_data["grad"] = grad;
-    ctx->saved_data["args"] = std::vector<double>{clip_low, clip_high, dual_clip, kl_coef, grad_scale};
-    ctx->saved_data["kl"] = kl;
-    ctx->saved_data["reduction"] = reduction;
+    auto k = c10::make_intrusive<Kept>();
+    k->clip_low = clip_low; k->clip_high = clip_high; k->dual_clip = dual_clip; k->kl_coef = kl_coef;
+    k->grad_scale = grad_scale; k->kl = kl; k->reduction = reduction;
+    k->grad = grad;
+    ctx->saved_data["kept"] = c10::IValue::make_capsule(std::move(k));
     ctx->mark_non_differentiable({stats});
     ctx->set_materialize_grads(false);
     return {loss, stats};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     static auto op = op_handle<decltype(op_policy_backward_)>("rl_triton::_policy_loss_backward_");
-    if (!g[0].defined()) return variable_list(12);
+    if (!g[0].defined()) return variable_list(13);
     const auto s = ctx->get_saved_variables();
-    const auto a = ctx->saved_data["args"].toDoubleVector();
-    Tensor grad;
-    const auto made = ctx->saved_data.find("grad");
-    const bool fresh = made == ctx->saved_data.end();
-    if (fresh) {
-      grad = at::empty(s[0].sizes(), s[0].options().dtype(at::kFloat));
-    } else {
-      grad = made->second.toTensor();
-      ctx->saved_data.erase(made);
-    }
-    op.call(grad, s[0], s[1], s[2], opt(s[3]), opt(s[4]), s[5], g[0], a[0], a[1], a[2], a[3],
-            ctx->saved_data["kl"].toInt(), ctx->saved_data["reduction"].toInt(), a[4], fresh);
-    variable_list out(12);
+    Kept& k = kept_of(ctx);
+    Tensor grad = k.take();
+    const bool fresh = !grad.defined();
+    if (fresh) grad = at::empty(s[0].sizes(), s[0].options().dtype(at::kFloat));
+    op.call(grad, s[0], s[1], s[2], opt(s[3]), opt(s[4]), s[5], g[0], k.clip_low, k.clip_high, k.dual_clip, k.kl_coef,
+            k.kl, k.reduction, k.grad_scale, fresh);
+    variable_list out(13);
     out[0] = s[0].scalar_type() == at::kFloat ? grad : grad.to(s[0].scalar_type());
     return out;
   }
@@ -421,35 +435,36 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
 std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& lp, const Tensor& old_lp, const Tensor& adv,
                                                 const OptT& mask, const OptT& ref, double clip_low, double clip_high,
                                                 double dual_clip, double kl_coef, int64_t kl, int64_t reduction,
-                                                double grad_scale) {
+                                                double grad_scale, bool need_stats) {
   if (at::GradMode::is_enabled() && lp.requires_grad()) {
     auto o = PolicyLoss::apply(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, reduction,
-                               grad_scale);
+                               grad_scale, need_stats);
     return {o[0], o[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_handle<decltype(op_policy)>("rl_triton::_policy_loss");
   auto [loss, stats, norm, grad] = op.call(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl,
-                                           reduction, grad_scale, false);
+                                           reduction, grad_scale, need_stats, false);
   return {loss, stats};
 }
 
 struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const Tensor& old_lp,
                                const Tensor& adv, const OptT& mask, const OptT& ref, double clip_low, double clip_high,
-                               double dual_clip, double kl_coef, int64_t kl, double entropy_coef, bool entropy,
+                               double dual_clip, double kl_coef, int64_t kl, double entropy_coef, bool need_stats,
                                double temperature, int64_t reduction, double grad_scale) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = op_handle<decltype(op_policy_logits)>("rl_triton::_policy_loss_logits");
     auto [loss, lp, ent, stats, norm, rows, grad] =
         op.call(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef,
-                entropy, temperature, reduction, grad_scale, true);
+                need_stats, temperature, reduction, grad_scale, true);
     ctx->save_for_backward({logits, tokens, old_lp, adv, plain(mask), plain(ref), norm, rows});
-    ctx->saved_data["grad"] = grad;
-    ctx->saved_data["args"] =
-        std::vector<double>{clip_low, clip_high, dual_clip, kl_coef, entropy_coef, temperature, grad_scale};
-    ctx->saved_data["kl"] = kl;
-    ctx->saved_data["reduction"] = reduction;
+    auto k = c10::make_intrusive<Kept>();
+    k->clip_low = clip_low; k->clip_high = clip_high; k->dual_clip = dual_clip; k->kl_coef = kl_coef;
+    k->entropy_coef = entropy_coef; k->temperature = temperature; k->grad_scale = grad_scale;
+    k->kl = kl; k->reduction = reduction;
+    k->grad = grad;
+    ctx->saved_data["kept"] = c10::IValue::make_capsule(std::move(k));
     ctx->mark_non_differentiable({lp, ent, stats});
     ctx->set_materialize_grads(false);
     return {loss, lp, ent, stats};
@@ -458,18 +473,12 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
     static auto op = op_handle<decltype(op_policy_logits_backward_)>("rl_triton::_policy_loss_logits_backward_");
     if (!g[0].defined()) return variable_list(16);
     const auto s = ctx->get_saved_variables();
-    const auto a = ctx->saved_data["args"].toDoubleVector();
-    Tensor grad;
-    const auto made = ctx->saved_data.find("grad");
-    const bool fresh = made == ctx->saved_data.end();
-    if (fresh) {
-      grad = call_grad_buffer(s[0]);
-    } else {
-      grad = made->second.toTensor();
-      ctx->saved_data.erase(made);
-    }
-    op.call(grad, s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), s[6], s[7], g[0], a[0], a[1], a[2], a[3],
-            ctx->saved_data["kl"].toInt(), a[4], a[5], ctx->saved_data["reduction"].toInt(), a[6], fresh);
+    Kept& k = kept_of(ctx);
+    Tensor grad = k.take();
+    const bool fresh = !grad.defined();
+    if (fresh) grad = call_grad_buffer(s[0]);
+    op.call(grad, s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), s[6], s[7], g[0], k.clip_low, k.clip_high, k.dual_clip,
+            k.kl_coef, k.kl, k.entropy_coef, k.temperature, k.reduction, k.grad_scale, fresh);
     variable_list out(16);
     out[0] = grad;
     return out;
@@ -479,16 +488,16 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
 std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss_logits_autograd(
     const Tensor& logits, const Tensor& tokens, const Tensor& old_lp, const Tensor& adv, const OptT& mask,
     const OptT& ref, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
-    double entropy_coef, bool entropy, double temperature, int64_t reduction, double grad_scale) {
+    double entropy_coef, bool need_stats, double temperature, int64_t reduction, double grad_scale) {
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     auto o = PolicyLossLogits::apply(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef,
-                                     kl, entropy_coef, entropy, temperature, reduction, grad_scale);
+                                     kl, entropy_coef, need_stats, temperature, reduction, grad_scale);
     return {o[0], o[1], o[2], o[3]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_handle<decltype(op_policy_logits)>("rl_triton::_policy_loss_logits");
   auto r = op.call(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef,
-                   entropy, temperature, reduction, grad_scale, false);
+                   need_stats, temperature, reduction, grad_scale, false);
   return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r)};
 }
 
@@ -544,11 +553,11 @@ TORCH_LIBRARY_FRAGMENT(rl_triton, m) {
   m.def("token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature, bool entropy) "
         "-> (Tensor, Tensor)");
   m.def("policy_loss(Tensor logprobs, Tensor old_logprobs, Tensor advantages, Tensor? mask, Tensor? ref_logprobs, "
-        "float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, int reduction, float grad_scale) "
-        "-> (Tensor, Tensor)");
+        "float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, int reduction, float grad_scale, "
+        "bool need_stats) -> (Tensor, Tensor)");
   m.def("policy_loss_logits(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? mask, "
         "Tensor? ref_logprobs, float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, "
-        "float entropy_coef, bool entropy, float temperature, int reduction, float grad_scale) "
+        "float entropy_coef, bool need_stats, float temperature, int reduction, float grad_scale) "
         "-> (Tensor, Tensor, Tensor, Tensor)");
   m.def("preference_loss(Tensor chosen, Tensor? rejected, Tensor? ref_chosen, Tensor? ref_rejected, "
         "Tensor? chosen_mask, Tensor? rejected_mask, float beta, float smoothing, int kind, bool normalized) "
@@ -560,13 +569,13 @@ TORCH_LIBRARY_FRAGMENT(rl_triton, m) {
         "Tensor? g_entropy, float temperature) -> Tensor");
   m.def("_policy_loss(Tensor logprobs, Tensor old_logprobs, Tensor advantages, Tensor? mask, Tensor? ref_logprobs, "
         "float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, int reduction, float grad_scale, "
-        "bool need_grad) -> (Tensor, Tensor, Tensor, Tensor)");
+        "bool need_stats, bool need_grad) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("_policy_loss_backward_(Tensor(a!) grad, Tensor logprobs, Tensor old_logprobs, Tensor advantages, "
         "Tensor? mask, Tensor? ref_logprobs, Tensor norm, Tensor grad_loss, float clip_low, float clip_high, "
         "float dual_clip, float kl_coef, int kl, int reduction, float grad_scale, bool force) -> ()");
   m.def("_policy_loss_logits(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? mask, "
         "Tensor? ref_logprobs, float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, "
-        "float entropy_coef, bool entropy, float temperature, int reduction, float grad_scale, bool need_grad) "
+        "float entropy_coef, bool need_stats, float temperature, int reduction, float grad_scale, bool need_grad) "
         "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("_policy_loss_logits_backward_(Tensor(a!) grad, Tensor logits, Tensor tokens, Tensor old_logprobs, "
         "Tensor advantages, Tensor? mask, Tensor? ref_logprobs, Tensor norm, Tensor row_stats, "

@@ -184,9 +184,9 @@ def _norm_fake(mask, like, n, reduction):
 
 @torch.library.register_fake("rl_triton::_policy_loss")
 def _(logprobs, old_logprobs, advantages, mask, ref_logprobs, clip_low, clip_high, dual_clip, kl_coef, kl, reduction,
-      grad_scale, need_grad):
+      grad_scale, need_stats, need_grad):
     n, t = logprobs.shape
-    return (_f32(logprobs), _f32(logprobs, 5), _norm_fake(mask, logprobs, n, reduction),
+    return (_f32(logprobs), _f32(logprobs, 5 if need_stats else 0), _norm_fake(mask, logprobs, n, reduction),
             _f32(logprobs, n, t) if need_grad else _f32(logprobs, 0))
 
 
@@ -197,10 +197,11 @@ def _(grad, *args):
 
 @torch.library.register_fake("rl_triton::_policy_loss_logits")
 def _(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, clip_low, clip_high, dual_clip, kl_coef, kl,
-      entropy_coef, entropy, temperature, reduction, grad_scale, need_grad):
+      entropy_coef, need_stats, temperature, reduction, grad_scale, need_grad):
     n, t, _v = logits.shape
     return (_f32(logits), _f32(logits, n, t),
-            _f32(logits, n, t) if entropy or entropy_coef != 0.0 else _f32(logits, 0), _f32(logits, 5),
+            _f32(logits, n, t) if need_stats or entropy_coef != 0.0 else _f32(logits, 0),
+            _f32(logits, 5 if need_stats else 0),
             _norm_fake(mask, logits, n, reduction), _row_stats_fake(logits, True),
             _grad_buffer_fake(logits) if need_grad else torch.empty((0,), dtype=logits.dtype, device=logits.device))
 

@@ -70,7 +70,8 @@ def compute_policy_loss(
     _placed(logprobs, old_logprobs, advantages, mask, ref_logprobs)
     _warn_copies({"logprobs": logprobs, "old_logprobs": old_logprobs, "advantages": advantages, "mask": mask,
                   "ref_logprobs": ref_logprobs})
-    loss, stats = nat.ops.policy_loss(logprobs, old_logprobs, advantages, mask, ref_logprobs, *c, float(grad_scale))
+    loss, stats = nat.ops.policy_loss(logprobs, old_logprobs, advantages, mask, ref_logprobs, *c, float(grad_scale),
+                                      bool(return_stats))
     _done(logprobs)
     return (loss, _stats(stats, False)) if return_stats else loss
 
