@@ -303,6 +303,14 @@ int rls_segment_compose(const float* summaries, int rank, int world, int backwar
 #define RLS_MASK_I32  4
 #define RLS_MASK_I64  5
 
+/* An order of the rows for calls with a mask: order[0] = the number of steps
+ * that count, then those steps (env * seq_len + step), then the others (int32
+ * [num_envs * seq_len + 1]).  Given to the calls below together with the mask it was made
+ * from, it spreads the work evenly (rows of more than RLS_SHORT_VOCAB logits;
+ * shorter ones do not use it); NULL: they go by the mask alone.                */
+int rls_row_order(const void* mask, int mask_kind, int64_t num_envs, int64_t seq_len, int32_t* order,
+                  void* ws, size_t ws_bytes, void* stream);
+
 /* With z = logits / temperature:  logprobs = z[token] - logsumexp(z),
  * entropy = -sum p log p (NULL: not computed).  row_stats (fp32 [N, T,
  * RLS_ROW_STATS], may be NULL) keeps each row's maximum and sums for the backward
@@ -310,7 +318,7 @@ int rls_segment_compose(const float* summaries, int rank, int world, int backwar
 #define RLS_ROW_STATS   8
 #define RLS_SHORT_VOCAB 1024
 int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
-                       const void* mask, int mask_kind, float* logprobs, float* entropy, float* row_stats,
+                       const void* mask, int mask_kind, const int32_t* order, float* logprobs, float* entropy, float* row_stats,
                        int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature, int in_dtype,
                        void* stream);
 
@@ -320,7 +328,7 @@ int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stri
  * (zero); row_stats as the forward call with an entropy output wrote it where
  * grad_entropy is given.                                                      */
 int rls_token_logprobs_backward(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
-                                const void* mask, int mask_kind, const float* row_stats,
+                                const void* mask, int mask_kind, const int32_t* order, const float* row_stats,
                                 const float* grad_logprobs, const float* grad_entropy, void* grad_logits,
                                 int64_t grad_env_stride, int64_t grad_step_stride, int64_t num_envs,
                                 int64_t seq_len, int64_t vocab, double temperature, int in_dtype, void* stream);
@@ -379,7 +387,7 @@ int rls_policy_loss_backward(const float* logprobs, const float* old_logprobs, c
  * is given). */
 int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
                            const float* old_logprobs, const float* advantages, int advantages_per_env,
-                           const float* ref_logprobs, const void* mask, int mask_kind, const rls_policy_t* policy,
+                           const float* ref_logprobs, const void* mask, int mask_kind, const int32_t* order, const rls_policy_t* policy,
                            float grad_scale, float* norm, float* logprobs, float* entropy, float* row_stats,
                            float* loss, float* stats, void* grad_logits, int64_t grad_env_stride,
                            int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature, int in_dtype,
@@ -387,7 +395,7 @@ int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_
 int rls_policy_loss_logits_backward(const void* logits, int64_t env_stride, int64_t step_stride,
                                     const int64_t* tokens, const float* old_logprobs, const float* advantages,
                                     int advantages_per_env, const float* ref_logprobs, const void* mask,
-                                    int mask_kind, const rls_policy_t* policy, float grad_scale,
+                                    int mask_kind, const int32_t* order, const rls_policy_t* policy, float grad_scale,
                                     const float* grad_loss, int force, const float* norm,
                                     const float* row_stats, void* grad_logits, int64_t grad_env_stride,
                                     int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab,

@@ -130,6 +130,7 @@ struct Rows {
   int V;
   const int64_t* tokens;
   Mask mask;
+  const int* order;    // null, or what rls_row_order made of the mask
   float c;             // log2(e) / temperature, rounded
   double c64, c_off;   // the same, not rounded; c64 / c - 1
   float inv_temp;
@@ -1027,8 +1028,9 @@ struct Walk {
   const unsigned rank = CL ? cluster_rank() : 0, size = CL ? cluster_size() : 1;
   const int log_size = !CL || size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3;  // sizes are powers of two
   const int64_t teams = gridDim.x >> log_size;
-  int64_t next_row = blockIdx.x >> log_size;
-  unsigned window = 0;  // which of the next 32 rows are to be worked on; the others only get their zeros
+  int64_t next = blockIdx.x >> log_size;  // the team's next place in the order of the rows
+  const int64_t kept = in.order ? in.order[0] : 0;
+  unsigned window = 0;  // without an order: which of the next 32 rows are to be worked on; the others only get their zeros
   int left = 0;
 
   __device__ __forceinline__ Walk(const Rows<T>& i, const RowOut& o, const GradRows<T>& g, const Src& s)
@@ -1054,28 +1056,46 @@ struct Walk {
     const int ends = ends_of(cut);
     if (tid < ends) g[tid < cut.head ? tid : in.V - ends + tid] = Vec<T>::put(0.f);
   }
+  // A row that does not count.
+  __device__ __forceinline__ void skip(int64_t row) const {
+    if constexpr (MODE != kBwd) {
+      if (rank == 0 && tid == 0) {
+        out.logprob[row] = 0.f;
+        if (out.entropy) out.entropy[row] = 0.f;
+        if (out.stats) out.stats[2 * row] = out.stats[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    if (MODE != kFwd && gr.g) zeros(row);
+  }
   // The next row to work on, or -1; the same in all threads of the team.
   __device__ __forceinline__ int64_t advance() {
+    if (in.order) {
+      // The rows that count come first, so that every team gets as many of them; the others are
+      // taken in between, as many to each.
+      const int64_t at = next;
+      next += teams;
+      const int64_t other = in.rows - 1 - at;  // from the far end
+      if (other >= kept) skip(in.order[1 + other]);
+      if (at < kept) return in.order[1 + at];
+      for (int64_t more = in.rows - 1 - next; more >= kept; more -= teams) {
+        skip(in.order[1 + more]);
+        next += teams;
+      }
+      return -1;
+    }
     for (;;) {
-      if (next_row >= in.rows) return -1;
+      if (next >= in.rows) return -1;
       if (left == 0) {
-        window = __ballot_sync(0xffffffffu, wanted(next_row + (tid & 31) * teams));
+        window = __ballot_sync(0xffffffffu, wanted(next + (tid & 31) * teams));
         left = 32;
       }
       const bool yes = window & 1u;
-      const int64_t row = next_row;
+      const int64_t row = next;
       window >>= 1;
       --left;
-      next_row += teams;
+      next += teams;
       if (yes) return row;
-      if constexpr (MODE != kBwd) {
-        if (rank == 0 && tid == 0) {
-          out.logprob[row] = 0.f;
-          if (out.entropy) out.entropy[row] = 0.f;
-          if (out.stats) out.stats[2 * row] = out.stats[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-      }
-      if (MODE != kFwd && gr.g) zeros(row);
+      skip(row);
     }
   }
   __device__ __forceinline__ const T* row_at(int64_t row) const { return in.x + in.at(row); }

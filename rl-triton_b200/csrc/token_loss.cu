@@ -71,6 +71,45 @@ __global__ void __launch_bounds__(kThreads) count_kernel(Mask mask, int64_t N, i
   }
 }
 
+// ---- an order of the rows -----------------------------------------------------------
+// order[0] = the number of rows that count, order[1 ..] = those, then the others.
+// Which row comes where depends on timing; nothing that a row gives does.
+__global__ void __launch_bounds__(kThreads) order_kernel(Mask mask, int rows, int* order, unsigned* front,
+                                                         unsigned* back, unsigned* ticket) {
+  __shared__ unsigned counts[kThreads / 32], base[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int64_t row0 = (int64_t)blockIdx.x * kThreads; row0 < rows; row0 += (int64_t)gridDim.x * kThreads) {
+    const int64_t row = row0 + tid;
+    const bool there = row < rows, yes = there && mask_at(mask, row);
+    const unsigned votes = __ballot_sync(0xffffffffu, yes);
+    if (lane == 0) counts[warp] = __popc(votes);
+    __syncthreads();
+    unsigned before = 0, all = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += counts[w];
+      all += counts[w];
+    }
+    const unsigned here = (unsigned)(rows - row0 < kThreads ? rows - row0 : kThreads);
+    if (tid == 0) {
+      base[0] = atomicAdd(front, all);
+      base[1] = atomicAdd(back, here - all);
+    }
+    __syncthreads();
+    const unsigned rank = before + __popc(votes & ((1u << lane) - 1u));
+    if (there) order[1 + (yes ? (int64_t)(base[0] + rank) : rows - 1 - (int64_t)(base[1] + tid - rank))] = (int)row;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    __threadfence();
+    if (atomicAdd(ticket, 1u) == gridDim.x - 1) {
+      __threadfence();
+      order[0] = (int)atomicExch(front, 0u);
+      atomicExch(back, 0u);
+      *ticket = 0u;
+    }
+  }
+}
+
 // ---- the loss over log-probabilities ----------------------------------------------
 struct Terms {
   const float* lp;
@@ -253,6 +292,7 @@ struct LogitsCall {
   int64_t es, ss;
   const int64_t* tokens;
   Mask mask;
+  const int* order;
   void* g;
   int64_t ges, gss;
   int64_t N, T, V;
@@ -270,6 +310,7 @@ int check_logits(const LogitsCall& c) {
   if (c.T > 0 && c.N > INT64_MAX / c.T) return RLS_EINVAL;
   if (c.N == 0 || c.T == 0) return RLS_OK;
   if (!c.x || !c.tokens) return RLS_EINVAL;
+  if (c.order && (!c.mask.p || c.N * c.T > 0x7ffffffe)) return RLS_EINVAL;
   if (c.es < 0 || c.ss < 0 || c.ges < 0 || c.gss < 0) return RLS_EINVAL;
   // a gradient's rows may not overlap, in whichever order they lie
   if (c.g) {
@@ -278,7 +319,7 @@ int check_logits(const LogitsCall& c) {
     if (!steps_in && !envs_in) return RLS_EINVAL;
   }
   const size_t e = c.dtype == RLS_BF16 ? 2 : 4;
-  if (!aligned(c.x, e) || !aligned(c.g, e) || !aligned(c.tokens, 8) || !aligned(c.mask.p, mask_align(c.mask.kind)))
+  if (!aligned(c.x, e) || !aligned(c.g, e) || !aligned(c.tokens, 8) || !aligned(c.mask.p, mask_align(c.mask.kind)) || !aligned(c.order, 4))
     return RLS_EALIGN;
   return RLS_OK;
 }
@@ -295,6 +336,7 @@ Rows<T> rows_of_call(const LogitsCall& c) {
   r.V = (int)c.V;
   r.tokens = c.tokens;
   r.mask = c.mask;
+  r.order = c.order;
   r.c64 = 1.4426950408889634074 / c.temperature;
   r.c = (float)r.c64;
   r.c_off = r.c64 / (double)r.c - 1.0;
@@ -339,17 +381,34 @@ int64_t rls::tok::sum_blocks(int64_t need) {
   return need < most ? need : most;
 }
 
+extern "C" int rls_row_order(const void* mask, int mask_kind, int64_t num_envs, int64_t seq_len, int32_t* order,
+                             void* ws, size_t ws_bytes, void* stream) {
+  if (num_envs < 0 || seq_len < 0 || !mask_ok(mask, mask_kind)) return RLS_EINVAL;
+  if (num_envs == 0 || seq_len == 0) return RLS_OK;
+  if (!mask || !order || !ws || num_envs > 0x7ffffffe / seq_len) return RLS_EINVAL;
+  if (ws_bytes < sizeof(WsHeader)) return RLS_EWORKSPACE;
+  if (!aligned(order, 4) || !aligned(ws) || !aligned(mask, mask_align(mask_kind))) return RLS_EALIGN;
+  DeviceGuard guard{mask, order, ws};
+  if (guard.status()) return guard.status();
+  std::lock_guard<std::recursive_mutex> lock(launch_mutex());
+  const int64_t rows = num_envs * seq_len, need = (rows + kThreads - 1) / kThreads;
+  unsigned* pad = static_cast<WsHeader*>(ws)->pad;
+  order_kernel<<<(unsigned)sum_blocks(need), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      Mask{mask, mask_kind}, (int)rows, order, &pad[9], &pad[10], ticket_of(ws));
+  return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
+}
+
 extern "C" int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
-                                  const void* mask, int mask_kind, float* logprobs, float* entropy, float* row_stats,
+                                  const void* mask, int mask_kind, const int32_t* order, float* logprobs, float* entropy, float* row_stats,
                                   int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature, int in_dtype,
                                   void* stream) {
-  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, nullptr, 0, 0, num_envs, seq_len,
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, order, nullptr, 0, 0, num_envs, seq_len,
                vocab, temperature, in_dtype};
   if (int st = check_logits(c)) return st;
   if (num_envs == 0 || seq_len == 0) return RLS_OK;
   if (!logprobs) return RLS_EINVAL;
   if (!aligned(logprobs) || !aligned(entropy) || !aligned(row_stats)) return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, mask, logprobs, entropy, row_stats};
+  DeviceGuard guard{logits, tokens, order, mask, logprobs, entropy, row_stats};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   return launch_logits<kFwd>(c, entropy != nullptr, RowOut{logprobs, entropy, reinterpret_cast<float4*>(row_stats)},
@@ -357,18 +416,18 @@ extern "C" int rls_token_logprobs(const void* logits, int64_t env_stride, int64_
 }
 
 extern "C" int rls_token_logprobs_backward(const void* logits, int64_t env_stride, int64_t step_stride,
-                                           const int64_t* tokens, const void* mask, int mask_kind,
+                                           const int64_t* tokens, const void* mask, int mask_kind, const int32_t* order,
                                            const float* row_stats, const float* grad_logprobs,
                                            const float* grad_entropy, void* grad_logits, int64_t grad_env_stride,
                                            int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab,
                                            double temperature, int in_dtype, void* stream) {
-  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, order, grad_logits, grad_env_stride,
                grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
   if (int st = check_logits(c)) return st;
   if (num_envs == 0 || seq_len == 0) return RLS_OK;
   if ((!row_stats && vocab > kLaneVocab) || !grad_logits) return RLS_EINVAL;
   if (!aligned(row_stats) || !aligned(grad_logprobs, 4) || !aligned(grad_entropy, 4)) return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, mask, row_stats, grad_logprobs, grad_entropy, grad_logits};
+  DeviceGuard guard{logits, tokens, order, mask, row_stats, grad_logprobs, grad_entropy, grad_logits};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   const RowOut out{nullptr, nullptr, reinterpret_cast<float4*>(const_cast<float*>(row_stats))};
@@ -450,12 +509,12 @@ extern "C" int rls_policy_loss_backward(const float* logprobs, const float* old_
 extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_stride,
                                       const int64_t* tokens, const float* old_logprobs, const float* advantages,
                                       int advantages_per_env, const float* ref_logprobs, const void* mask,
-                                      int mask_kind, const rls_policy_t* policy, float grad_scale, float* norm,
+                                      int mask_kind, const int32_t* order, const rls_policy_t* policy, float grad_scale, float* norm,
                                       float* logprobs, float* entropy, float* row_stats, float* loss, float* stats,
                                       void* grad_logits, int64_t grad_env_stride, int64_t grad_step_stride,
                                       int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature,
                                       int in_dtype, void* ws, size_t ws_bytes, void* stream) {
-  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, order, grad_logits, grad_env_stride,
                grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
   if (!policy_ok(policy) || !loss) return RLS_EINVAL;
   if (int st = check_logits(c)) return st;
@@ -470,7 +529,7 @@ extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, in
   if (!aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) || !aligned(logprobs) ||
       !aligned(entropy) || !aligned(row_stats) || !aligned(ws) || !aligned(norm, 4) || !aligned(loss, 4) || !aligned(stats, 4))
     return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, old_logprobs, advantages, ref_logprobs, mask, norm, logprobs, entropy, row_stats,
+  DeviceGuard guard{logits, tokens, order, old_logprobs, advantages, ref_logprobs, mask, norm, logprobs, entropy, row_stats,
                     loss, stats, grad_logits, ws};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
@@ -490,13 +549,13 @@ extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, in
 extern "C" int rls_policy_loss_logits_backward(const void* logits, int64_t env_stride, int64_t step_stride,
                                                const int64_t* tokens, const float* old_logprobs,
                                                const float* advantages, int advantages_per_env,
-                                               const float* ref_logprobs, const void* mask, int mask_kind,
+                                               const float* ref_logprobs, const void* mask, int mask_kind, const int32_t* order,
                                                const rls_policy_t* policy, float grad_scale, const float* grad_loss,
                                                int force, const float* norm,
                                                const float* row_stats, void* grad_logits, int64_t grad_env_stride,
                                                int64_t grad_step_stride, int64_t num_envs, int64_t seq_len,
                                                int64_t vocab, double temperature, int in_dtype, void* stream) {
-  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, grad_logits, grad_env_stride,
+  LogitsCall c{logits, env_stride, step_stride, tokens, Mask{mask, mask_kind}, order, grad_logits, grad_env_stride,
                grad_step_stride, num_envs, seq_len, vocab, temperature, in_dtype};
   if (!policy_ok(policy)) return RLS_EINVAL;
   if (int st = check_logits(c)) return st;
@@ -506,7 +565,7 @@ extern "C" int rls_policy_loss_logits_backward(const void* logits, int64_t env_s
   if (!aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) || !aligned(row_stats) ||
       !aligned(norm, 4) || !aligned(grad_loss, 4))
     return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, row_stats,
+  DeviceGuard guard{logits, tokens, order, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, row_stats,
                     grad_logits};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());

@@ -102,7 +102,18 @@ struct LogitsArgs {
   int64_t n, t, v;
   LogitsArgs(const Tensor& logits, const Tensor& tok, const OptT& m)
       : x(logits_arg(logits)), tokens(tokens_arg(tok)), mask(mask_arg(m)), n(x.size(0)), t(x.size(1)), v(x.size(2)) {}
+  // Long rows with a mask go by an order of the rows, made once for both directions.
+  Tensor order() const {
+    if (!mask.t || v <= RLS_SHORT_VOCAB || n * t > 0x7ffffffe) return at::empty({0}, x.options().dtype(at::kInt));
+    Tensor o = at::empty({n * t + 1}, x.options().dtype(at::kInt));
+    Tensor ws = workspace_for(x.device(), stream_of(x), 1 << 20);
+    check(rls_row_order(mask.ptr(), mask.kind, n, t, o.data_ptr<int32_t>(), ws.data_ptr(), (size_t)ws.numel(),
+                        stream_of(x)),
+          "rls_row_order");
+    return o;
+  }
 };
+const int32_t* I(const Tensor& t) { return t.numel() ? t.data_ptr<int32_t>() : nullptr; }
 
 Tensor like(const Tensor& t, at::IntArrayRef sizes) { return at::empty(sizes, t.options().dtype(at::kFloat)); }
 
@@ -112,27 +123,28 @@ Tensor row_stats(const LogitsArgs& a, bool keep) {
 }
 
 // ---- log-probabilities -------------------------------------------------------------
-// (logprobs, entropy or an empty tensor, the rows' statistics or an empty tensor)
-std::tuple<Tensor, Tensor, Tensor> op_logprobs(const Tensor& logits, const Tensor& tokens, const OptT& mask,
+// (logprobs, entropy or empty, the rows' statistics or empty, their order or empty)
+std::tuple<Tensor, Tensor, Tensor, Tensor> op_logprobs(const Tensor& logits, const Tensor& tokens, const OptT& mask,
                                                double temperature, bool entropy, bool keep) {
   const LogitsArgs a(logits, tokens, mask);
   Tensor lp = like(a.x, {a.n, a.t});
   Tensor ent = like(a.x, entropy ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
-  Tensor stats = row_stats(a, keep);
+  Tensor stats = row_stats(a, keep), order = a.order();
   check(rls_token_logprobs(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), a.mask.ptr(),
-                           a.mask.kind, W(lp), W(ent), W(stats), a.n, a.t, a.v, temperature, dtype_of(a.x),
+                           a.mask.kind, I(order), W(lp), W(ent), W(stats), a.n, a.t, a.v, temperature, dtype_of(a.x),
                            stream_of(a.x)),
         "rls_token_logprobs");
-  return {lp, ent, stats};
+  return {lp, ent, stats, order};
 }
 
-Tensor op_logprobs_backward(const Tensor& logits, const Tensor& tokens, const OptT& mask, const Tensor& stats,
+Tensor op_logprobs_backward(const Tensor& logits, const Tensor& tokens, const OptT& mask, const Tensor& order,
+                            const Tensor& stats,
                             const OptT& g_lp, const OptT& g_ent, double temperature) {
   const LogitsArgs a(logits, tokens, mask);
   const OptT gl = f32(g_lp), ge = f32(g_ent);
   Tensor g = op_grad_buffer(a.x);
   check(rls_token_logprobs_backward(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(),
-                                    a.mask.ptr(), a.mask.kind, W(stats), F(gl), F(ge), g.data_ptr(), g.stride(0),
+                                    a.mask.ptr(), a.mask.kind, I(order), W(stats), F(gl), F(ge), g.data_ptr(), g.stride(0),
                                     g.stride(1), a.n, a.t, a.v, temperature, dtype_of(a.x), stream_of(a.x)),
         "rls_token_logprobs_backward");
   return g;
@@ -193,8 +205,8 @@ void op_policy_backward_(Tensor& grad, const Tensor& logprobs, const Tensor& old
         "rls_policy_loss_backward");
 }
 
-// (loss, logprobs, entropy or empty, statistics [5], norm, the rows' statistics, gradient or empty)
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_policy_logits(
+// (loss, logprobs, entropy or empty, statistics [5], norm, the rows' order and statistics, gradient or empty)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_policy_logits(
     const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
     const OptT& mask, const OptT& ref, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
     double entropy_coef, bool need_stats, double temperature, int64_t reduction, double grad_scale, bool need_grad) {
@@ -203,23 +215,23 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_policy_log
   const OptT rf = f32(ref);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
   Tensor loss = like(a.x, {}), stats = like(a.x, {need_stats ? 5 : 0}), norm = norm_for(a.mask, a.x, a.n, reduction);
-  Tensor lp = like(a.x, {a.n, a.t}), rows = row_stats(a, true);
+  Tensor lp = like(a.x, {a.n, a.t}), rows = row_stats(a, true), order = a.order();
   Tensor ent = like(a.x, need_stats || entropy_coef != 0.0 ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
   Tensor g = need_grad ? op_grad_buffer(a.x) : at::empty({0}, a.x.options());
   Tensor ws = policy_workspace(a.x);
   check(rls_policy_loss_logits(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), F(old_lp),
-                               F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, &p, (float)grad_scale,
+                               F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, I(order), &p, (float)grad_scale,
                                W(norm), W(lp), W(ent), W(rows), loss.data_ptr<float>(), W(stats),
                                need_grad ? g.data_ptr() : nullptr, need_grad ? g.stride(0) : 0,
                                need_grad ? g.stride(1) : 0, a.n, a.t, a.v, temperature, dtype_of(a.x),
                                ws.data_ptr(), (size_t)ws.numel(), stream_of(a.x)),
         "rls_policy_loss_logits");
-  return {loss, lp, ent, stats, norm, rows, g};
+  return {loss, lp, ent, stats, norm, order, rows, g};
 }
 
 void op_policy_logits_backward_(Tensor& grad, const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
                                 const Tensor& advantages, const OptT& mask, const OptT& ref, const Tensor& norm,
-                                const Tensor& rows, const Tensor& grad_loss, double clip_low,
+                                const Tensor& order, const Tensor& rows, const Tensor& grad_loss, double clip_low,
                                 double clip_high, double dual_clip, double kl_coef, int64_t kl, double entropy_coef,
                                 double temperature, int64_t reduction, double grad_scale, bool force) {
   const LogitsArgs a(logits, tokens, mask);
@@ -227,7 +239,7 @@ void op_policy_logits_backward_(Tensor& grad, const Tensor& logits, const Tensor
   const OptT rf = f32(ref);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
   check(rls_policy_loss_logits_backward(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(),
-                                        F(old_lp), F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, &p,
+                                        F(old_lp), F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, I(order), &p,
                                         (float)grad_scale, F(up), force, W(norm), W(rows),
                                         grad.data_ptr(), grad.stride(0), grad.stride(1), a.n, a.t, a.v,
                                         temperature, dtype_of(a.x), stream_of(a.x)),
@@ -369,8 +381,8 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
                                double temperature, bool entropy) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = op_handle<decltype(op_logprobs)>("rl_triton::_token_logprobs");
-    auto [lp, ent, stats] = op.call(logits, tokens, mask, temperature, entropy, true);
-    ctx->save_for_backward({logits, tokens, plain(mask), stats});
+    auto [lp, ent, stats, order] = op.call(logits, tokens, mask, temperature, entropy, true);
+    ctx->save_for_backward({logits, tokens, plain(mask), order, stats});
     ctx->saved_data["temperature"] = temperature;
     ctx->set_materialize_grads(false);
     if (!entropy) ctx->mark_non_differentiable({ent});
@@ -381,7 +393,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
     const auto s = ctx->get_saved_variables();
     Tensor out;
     if (g[0].defined() || g[1].defined())
-      out = op.call(s[0], s[1], opt(s[2]), s[3], opt(g[0]), opt(g[1]), ctx->saved_data["temperature"].toDouble());
+      out = op.call(s[0], s[1], opt(s[2]), s[3], s[4], opt(g[0]), opt(g[1]), ctx->saved_data["temperature"].toDouble());
     return {out, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -394,7 +406,7 @@ std::tuple<Tensor, Tensor> token_logprobs_autograd(const Tensor& logits, const T
   }
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_handle<decltype(op_logprobs)>("rl_triton::_token_logprobs");
-  auto [lp, ent, stats] = op.call(logits, tokens, mask, temperature, entropy, false);
+  auto [lp, ent, stats, order] = op.call(logits, tokens, mask, temperature, entropy, false);
   return {lp, ent};
 }
 
@@ -455,10 +467,10 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
                                double temperature, int64_t reduction, double grad_scale) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = op_handle<decltype(op_policy_logits)>("rl_triton::_policy_loss_logits");
-    auto [loss, lp, ent, stats, norm, rows, grad] =
+    auto [loss, lp, ent, stats, norm, order, rows, grad] =
         op.call(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef,
                 need_stats, temperature, reduction, grad_scale, true);
-    ctx->save_for_backward({logits, tokens, old_lp, adv, plain(mask), plain(ref), norm, rows});
+    ctx->save_for_backward({logits, tokens, old_lp, adv, plain(mask), plain(ref), norm, order, rows});
     auto k = c10::make_intrusive<Kept>();
     k->clip_low = clip_low; k->clip_high = clip_high; k->dual_clip = dual_clip; k->kl_coef = kl_coef;
     k->entropy_coef = entropy_coef; k->temperature = temperature; k->grad_scale = grad_scale;
@@ -477,7 +489,7 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
     Tensor grad = k.take();
     const bool fresh = !grad.defined();
     if (fresh) grad = call_grad_buffer(s[0]);
-    op.call(grad, s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), s[6], s[7], g[0], k.clip_low, k.clip_high, k.dual_clip,
+    op.call(grad, s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), s[6], s[7], s[8], g[0], k.clip_low, k.clip_high, k.dual_clip,
             k.kl_coef, k.kl, k.entropy_coef, k.temperature, k.reduction, k.grad_scale, fresh);
     variable_list out(16);
     out[0] = grad;
@@ -564,8 +576,8 @@ TORCH_LIBRARY_FRAGMENT(rl_triton, m) {
         "-> (Tensor, Tensor)");
   m.def("_grad_buffer(Tensor logits) -> Tensor");
   m.def("_token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature, bool entropy, bool keep) "
-        "-> (Tensor, Tensor, Tensor)");
-  m.def("_token_logprobs_backward(Tensor logits, Tensor tokens, Tensor? mask, Tensor row_stats, Tensor? g_logprobs, "
+        "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("_token_logprobs_backward(Tensor logits, Tensor tokens, Tensor? mask, Tensor order, Tensor row_stats, Tensor? g_logprobs, "
         "Tensor? g_entropy, float temperature) -> Tensor");
   m.def("_policy_loss(Tensor logprobs, Tensor old_logprobs, Tensor advantages, Tensor? mask, Tensor? ref_logprobs, "
         "float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, int reduction, float grad_scale, "
@@ -576,9 +588,9 @@ TORCH_LIBRARY_FRAGMENT(rl_triton, m) {
   m.def("_policy_loss_logits(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? mask, "
         "Tensor? ref_logprobs, float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, "
         "float entropy_coef, bool need_stats, float temperature, int reduction, float grad_scale, bool need_grad) "
-        "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("_policy_loss_logits_backward_(Tensor(a!) grad, Tensor logits, Tensor tokens, Tensor old_logprobs, "
-        "Tensor advantages, Tensor? mask, Tensor? ref_logprobs, Tensor norm, Tensor row_stats, "
+        "Tensor advantages, Tensor? mask, Tensor? ref_logprobs, Tensor norm, Tensor order, Tensor row_stats, "
         "Tensor grad_loss, float clip_low, float clip_high, float dual_clip, float kl_coef, int kl, "
         "float entropy_coef, float temperature, int reduction, float grad_scale, bool force) -> ()");
   m.def("_preference_loss(Tensor chosen, Tensor? rejected, Tensor? ref_chosen, Tensor? ref_rejected, "

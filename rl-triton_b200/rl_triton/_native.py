@@ -166,15 +166,21 @@ def _row_stats_fake(logits, keep):
     return _f32(logits, n, t, ROW_STATS) if keep and v > SHORT_VOCAB else _f32(logits, 0)
 
 
+def _order_fake(logits, mask):
+    n, t, v = logits.shape
+    some = mask is not None and mask.numel() and v > SHORT_VOCAB and n * t <= 0x7ffffffe
+    return torch.empty((n * t + 1 if some else 0,), dtype=torch.int32, device=logits.device)
+
+
 @torch.library.register_fake("rl_triton::_token_logprobs")
 def _(logits, tokens, mask, temperature, entropy, keep):
     n, t, _v = logits.shape
     return (_f32(logits, n, t), _f32(logits, n, t) if entropy else _f32(logits, 0),
-            _row_stats_fake(logits, keep))
+            _row_stats_fake(logits, keep), _order_fake(logits, mask))
 
 
 @torch.library.register_fake("rl_triton::_token_logprobs_backward")
-def _(logits, tokens, mask, row_stats, g_logprobs, g_entropy, temperature):
+def _(logits, tokens, mask, order, row_stats, g_logprobs, g_entropy, temperature):
     return _grad_buffer_fake(logits)
 
 
@@ -202,7 +208,7 @@ def _(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, clip_low, cl
     return (_f32(logits), _f32(logits, n, t),
             _f32(logits, n, t) if need_stats or entropy_coef != 0.0 else _f32(logits, 0),
             _f32(logits, 5 if need_stats else 0),
-            _norm_fake(mask, logits, n, reduction), _row_stats_fake(logits, True),
+            _norm_fake(mask, logits, n, reduction), _order_fake(logits, mask), _row_stats_fake(logits, True),
             _grad_buffer_fake(logits) if need_grad else torch.empty((0,), dtype=logits.dtype, device=logits.device))
 
 
@@ -255,14 +261,15 @@ _SIGS = {
     "rls_gae_value_loss": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I, _F, _I, _P, _SZ,
                                 _P]),
     "rls_gae_obs_skip": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _F, _F, _I, _P]),
-    "rls_token_logprobs": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _D, _I, _P]),
-    "rls_token_logprobs_backward": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _D,
-                                         _I, _P]),
+    "rls_row_order": (_I, [_P, _I, _I64, _I64, _P, _P, _SZ, _P]),
+    "rls_token_logprobs": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _D, _I, _P]),
+    "rls_token_logprobs_backward": (_I, [_P, _I64, _I64, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
+                                         _D, _I, _P]),
     "rls_policy_loss": (_I, [_P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _P, _P, _P, _I64, _I64, _P, _SZ, _P]),
     "rls_policy_loss_backward": (_I, [_P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _I, _P, _P, _I64, _I64, _P]),
-    "rls_policy_loss_logits": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _P, _P, _P, _P, _P, _P,
-                                    _I64, _I64, _I64, _I64, _I64, _D, _I, _P, _SZ, _P]),
-    "rls_policy_loss_logits_backward": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _POL, _F, _P, _I, _P, _P,
+    "rls_policy_loss_logits": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _P, _POL, _F, _P, _P, _P, _P, _P, _P,
+                                    _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _P, _SZ, _P]),
+    "rls_policy_loss_logits_backward": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _P, _POL, _F, _P, _I, _P, _P,
                                              _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _P]),
     "rls_preference_loss": (_I, [_P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _F, _F, _I, _I, _P, _P, _P, _P,
                                  _SZ, _P]),
