@@ -94,6 +94,12 @@ size_t rls_workspace_bytes(int64_t num_elements);
  * (1 = tile look-back wait, 2 = bulk-copy wait).                          */
 int rls_workspace_error(void* ws, void* stream);
 const char* rls_status_string(int status);
+/* For callers that know where their arrays are: until it is called again with
+ * -1, the calling thread's calls take every array to be memory of GPU `device`
+ * and leave out the placement queries (one driver query an array, a third of a
+ * small call's host time).  Returns the value before (-1: none).  An array that
+ * is elsewhere then faults the GPU instead of returning RLS_ENOTDEVICE.      */
+int rls_assume_device(int device);
 const char* rls_build_info(void);
 
 /* ---- the seven estimators ---------------------------------------------- */
@@ -382,12 +388,13 @@ int rls_policy_loss_backward(const float* logprobs, const float* old_logprobs, c
 /* From the logits, in one pass over them: each row's log-probability is taken
  * and its gradient written while the row is at hand.  logprobs and row_stats
  * (as rls_token_logprobs) are written; entropy is (and has to be given) where entropy_coef != 0, else
- * may be NULL.  grad_logits (NULL: no gradient) = grad_scale * d loss / d logits
+ * may be NULL.  order (may be NULL) is written as rls_row_order does, where the rows are
+ * long.  grad_logits (NULL: no gradient) = grad_scale * d loss / d logits
  * in in_dtype.  loss and stats as rls_policy_loss (with the mean entropy where it
  * is given). */
 int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
                            const float* old_logprobs, const float* advantages, int advantages_per_env,
-                           const float* ref_logprobs, const void* mask, int mask_kind, const int32_t* order, const rls_policy_t* policy,
+                           const float* ref_logprobs, const void* mask, int mask_kind, int32_t* order, const rls_policy_t* policy,
                            float grad_scale, float* norm, float* logprobs, float* entropy, float* row_stats,
                            float* loss, float* stats, void* grad_logits, int64_t grad_env_stride,
                            int64_t grad_step_stride, int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature, int in_dtype,
@@ -410,8 +417,8 @@ int rls_policy_loss_logits_backward(const void* logits, int64_t env_stride, int6
  *   RLS_PREFERENCE_SIGMOID  -(1 - smoothing) log sig(x) - smoothing log sig(-x),
  *   RLS_PREFERENCE_IPO      (x / beta - 1 / (2 beta))^2,
  *   RLS_PREFERENCE_HINGE    max(0, 1 - x),
- * loss = the mean over the pairs (0 of none).  rewards (fp32 [2, pairs]) = beta s of the
- * chosen, then of the rejected.  coef (fp32 [2, pairs], may be NULL) keeps
+ * loss = the mean over the pairs (0 of none).  chosen_rewards and rejected_rewards
+ * (fp32 [pairs]) = beta s.  coef (fp32 [2, pairs], may be NULL) keeps
  * d loss / d logprob of a step that counts, for the backward call, which writes
  * *grad_loss times it at those steps and 0 elsewhere.  Deterministic.          */
 #define RLS_PREFERENCE_SIGMOID 0
@@ -421,7 +428,8 @@ int rls_preference_loss(const float* chosen, const float* rejected, const float*
                         const float* ref_rejected, int ref_per_pair, const void* chosen_mask,
                         const void* rejected_mask, int mask_kind, int64_t pairs, int64_t chosen_len,
                         int64_t rejected_len, float beta, float smoothing, int kind, int length_normalized,
-                        float* loss, float* rewards, float* coef, void* ws, size_t ws_bytes, void* stream);
+                        float* loss, float* chosen_rewards, float* rejected_rewards, float* coef, void* ws,
+                        size_t ws_bytes, void* stream);
 int rls_preference_loss_backward(const float* coef, const float* grad_loss, const void* chosen_mask,
                                  const void* rejected_mask, int mask_kind, float* grad_chosen,
                                  float* grad_rejected, int64_t pairs, int64_t chosen_len, int64_t rejected_len,

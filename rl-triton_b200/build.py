@@ -22,8 +22,10 @@ LIB = os.path.join(LIBDIR, "librlscan.so")
 TORCH_LIB = os.path.join(LIBDIR, "librlscan_torch.so")
 SOURCES = ["rlscan.cu", "segment.cu", "ppo.cu", "token_loss.cu", "token_lanes.cu", "token_rows.cu", "preference.cu"]
 TORCH_SOURCES = ["torch_ops.cpp", "torch_token_ops.cpp"]
-HEADERS = ["common.cuh", "algs.cuh", "scan_kernel.cuh", "rows_kernel.cuh", "rows2_kernel.cuh", "tile_kernel.cuh", "tile_policies.cuh", "host_shared.h",
-           "token_kernels.cuh", "token_launch.h"]
+TOKEN_HEADERS = ["token_kernels.cuh", "token_launch.h"]
+HEADERS = ["common.cuh", "algs.cuh", "scan_kernel.cuh", "rows_kernel.cuh", "rows2_kernel.cuh", "tile_kernel.cuh",
+           "tile_policies.cuh", "host_shared.h", *TOKEN_HEADERS]
+TOKEN_SOURCES = {"token_loss.cu", "token_lanes.cu", "token_rows.cu", "preference.cu"}
 
 
 def nvcc_path() -> str:
@@ -100,9 +102,11 @@ OBJDIR = os.path.join(HERE, "_build")
 
 
 def _deps(src: str) -> list[str]:
-    # every source includes some of the headers; rebuild on any of them
-    return [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(ROOT, "include",
-                                                                                               "rlscan.h")]
+    # the token-level kernels and the scans include headers of their own
+    heads = (["common.cuh", "host_shared.h", *TOKEN_HEADERS] if src in TOKEN_SOURCES
+             else [h for h in HEADERS if h not in TOKEN_HEADERS])
+    return [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in heads] + [os.path.join(ROOT, "include",
+                                                                                              "rlscan.h")]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

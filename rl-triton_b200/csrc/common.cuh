@@ -204,24 +204,19 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 // pageable or pinned host memory), and runs the call with that device current,
 // restoring the caller's device afterwards.  A host pointer handed to a kernel
 // would fault the GPU; here it returns a status instead.
+//
+// A caller that knows where its arrays are (the operator library looks at each
+// tensor's device) may say so for its thread through rls_assume_device: the
+// queries, a third of a small call's host time, are left out then.
+int assumed_device();  // -1: none
+
 class DeviceGuard {
  public:
   // status(): 0 = ok; otherwise RLS_ENOTDEVICE (7) from rlscan.h.
   DeviceGuard(std::initializer_list<const void*> ptrs) {
-    int dev = -1;
-    for (const void* p : ptrs) {
-      if (!p) continue;
-      cudaPointerAttributes at;
-      if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
-        cudaGetLastError();  // clear the sticky-free error the query leaves
-        status_ = 7;
-        return;
-      }
-      if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) { status_ = 7; return; }
-      if (dev < 0) dev = at.device;
-      else if (at.device != dev) { status_ = 7; return; }
-    }
-    if (dev < 0) return;
+    int dev = assumed_device();
+    if (dev < 0) dev = device_of(ptrs);
+    if (status_ || dev < 0) return;
     if (cudaGetDevice(&prev_) != cudaSuccess) { cudaGetLastError(); prev_ = -1; }
     if (prev_ != dev) {
       if (cudaSetDevice(dev) != cudaSuccess) { status_ = 7; prev_ = -1; return; }
@@ -236,6 +231,23 @@ class DeviceGuard {
   DeviceGuard& operator=(const DeviceGuard&) = delete;
 
  private:
+  int device_of(std::initializer_list<const void*> ptrs) {
+    int dev = -1;
+    for (const void* p : ptrs) {
+      if (!p) continue;
+      cudaPointerAttributes at;
+      if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();  // clear the sticky-free error the query leaves
+        status_ = 7;
+        return -1;
+      }
+      if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) { status_ = 7; return -1; }
+      if (dev < 0) dev = at.device;
+      else if (at.device != dev) { status_ = 7; return -1; }
+    }
+    return dev;
+  }
+
   int status_ = 0;
   int prev_ = -1;
   bool switched_ = false;

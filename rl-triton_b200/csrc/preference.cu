@@ -30,64 +30,84 @@ struct PrefArgs {
   int kind;
   bool normalized;
   float* loss;
-  float* rewards;    // [2, B]
+  float* rewards[2]; // [B] each
   float* coef;       // [2, B] or null
   double* terms;     // [B]
   unsigned* ticket;
 };
 
-template <int NT>
-__device__ __forceinline__ double2 block_sum2(double a, double b) {
-  __shared__ double2 part[NT / 32];
+template <int NT, int K>
+__device__ __forceinline__ void block_sums(double (&v)[K]) {
+  __shared__ double part[NT / 32][K];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) part[threadIdx.x >> 5][k] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = part[0][k];
+    for (int w = 1; w < NT / 32; ++w) v[k] += part[w][k];
   }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_double2(a, b);
-  __syncthreads();
-  double2 s = part[0];
-  for (int w = 1; w < NT / 32; ++w) { s.x += part[w].x; s.y += part[w].y; }
-  return s;
 }
 
-// A response's sum and count, over the CTA.  Sums are fp64: a sum over 10^5
-// steps of differences near 0 keeps the accuracy of its terms.
+// A thread's share of a response's sum and count.  Differences are fp32, of four steps
+// at a time; their sums fp64: a sum over 10^5 steps of differences near 0 keeps the
+// accuracy of its terms.
 template <int NT>
-__device__ __forceinline__ double2 side_sum(const Side& d, bool ref_pair, int64_t b) {
-  double sum = 0, n = 0;
-  const bool ref = d.ref && !ref_pair;
-  for (int64_t t = threadIdx.x; t < d.T; t += NT) {
-    const int64_t i = b * d.T + t;
-    if (mask_at(d.mask, i)) {
-      sum += (double)d.lp[i] - (ref ? (double)d.ref[i] : 0.0);
-      n += 1.0;
+__device__ __forceinline__ void side_sum(const Side& d, bool ref_pair, int64_t b, double& sum, double& n) {
+  const float* ref = ref_pair ? nullptr : d.ref;
+  const int64_t i0 = b * d.T;
+  unsigned count = 0;
+  sum = 0;
+  if (d.T % 4 == 0 && (((uintptr_t)d.lp | (uintptr_t)ref) & 15) == 0) {
+#pragma unroll 2
+    for (int64_t t = threadIdx.x * 4; t < d.T; t += NT * 4) {
+      const unsigned m = mask_four(d.mask, i0 + t, i0 + d.T);
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(d.lp + i0 + t));
+      const float4 y = ref ? __ldcs(reinterpret_cast<const float4*>(ref + i0 + t)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float a = (m & 1u ? x.x - y.x : 0.f) + (m & 2u ? x.y - y.y : 0.f);
+      const float c = (m & 4u ? x.z - y.z : 0.f) + (m & 8u ? x.w - y.w : 0.f);
+      sum += (double)(a + c);
+      count += __popc(m);
     }
+  } else {
+#pragma unroll 4
+    for (int64_t t = threadIdx.x; t < d.T; t += NT)
+      if (mask_at(d.mask, i0 + t)) {
+        sum += (double)(d.lp[i0 + t] - (ref ? ref[i0 + t] : 0.f));
+        ++count;
+      }
   }
-  double2 s = block_sum2<NT>(sum, n);
-  if (d.ref && ref_pair) s.x -= (double)d.ref[b];
-  return s;
+  n = count;
 }
 
 template <int NT>
 __global__ void __launch_bounds__(NT) preference_kernel(PrefArgs p) {
   __shared__ bool last;
   const int64_t b = blockIdx.x;
-  double s[2], n[2];
+  double s[2], n[2], v[4];
+  side_sum<NT>(p.side[0], p.ref_pair, b, v[0], v[1]);
+  side_sum<NT>(p.side[1], p.ref_pair, b, v[2], v[3]);
+  block_sums<NT>(v);
   for (int k = 0; k < 2; ++k) {
-    const double2 q = side_sum<NT>(p.side[k], p.ref_pair, b);
-    n[k] = p.normalized ? fmax(q.y, 1.0) : 1.0;
-    s[k] = q.x / n[k];
+    if (p.side[k].ref && p.ref_pair) v[2 * k] -= (double)p.side[k].ref[b];
+    n[k] = p.normalized ? fmax(v[2 * k + 1], 1.0) : 1.0;
+    s[k] = v[2 * k] / n[k];
   }
   if (threadIdx.x == 0) {
     const double beta = p.beta, gap = s[0] - s[1], x = beta * gap, e = p.smoothing;
     double term, d;  // d: by gap
     if (p.kind == RLS_PREFERENCE_SIGMOID) {
-      const double z = exp(-fabs(x)), l = log1p(z);
-      term = (1.0 - e) * (l + fmax(-x, 0.0)) + e * (l + fmax(x, 0.0));
-      const double sig = x >= 0 ? 1.0 / (1.0 + z) : z / (1.0 + z);
-      d = beta * (sig - (1.0 - e));
+      // the parts of size 1 in fp32, as one thread forms them while the CTA waits
+      const float z = expf(-fabsf((float)x)), l = log1pf(z);
+      term = (double)l + (1.0 - e) * fmax(-x, 0.0) + e * fmax(x, 0.0);
+      const float less = z / (1.f + z);  // the smaller of sig(x) and sig(-x)
+      d = beta * (x >= 0 ? e - (double)less : (double)less - (1.0 - e));
       if (isnan(x)) term = d = x;
     } else if (p.kind == RLS_PREFERENCE_IPO) {
       const double y = gap - 0.5 / beta;
@@ -97,8 +117,8 @@ __global__ void __launch_bounds__(NT) preference_kernel(PrefArgs p) {
       term = 1.0 - x > 0.0 ? 1.0 - x : isnan(x) ? x : 0.0;
       d = x < 1.0 ? -beta : isnan(x) ? x : 0.0;
     }
-    p.rewards[b] = (float)(beta * s[0]);
-    p.rewards[p.B + b] = (float)(beta * s[1]);
+    p.rewards[0][b] = (float)(beta * s[0]);
+    p.rewards[1][b] = (float)(beta * s[1]);
     if (p.coef) {
       p.coef[b] = (float)(d / (n[0] * (double)p.B));
       p.coef[p.B + b] = (float)(-d / (n[1] * (double)p.B));
@@ -110,16 +130,17 @@ __global__ void __launch_bounds__(NT) preference_kernel(PrefArgs p) {
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double sum = 0;
-  for (int64_t i = threadIdx.x; i < p.B; i += NT) sum += __ldcg(&p.terms[i]);
-  const double2 all = block_sum2<NT>(sum, 0.0);
+  double all[1] = {0};
+  for (int64_t i = threadIdx.x; i < p.B; i += NT) all[0] += __ldcg(&p.terms[i]);
+  block_sums<NT>(all);
   if (threadIdx.x == 0) {
-    *p.loss = (float)(all.x / (double)p.B);
+    *p.loss = (float)(all[0] / (double)p.B);
     *p.ticket = 0u;
   }
 }
 
 constexpr int kSpread = 256;
+constexpr int64_t kSpreadSteps = kSpread * 16;  // of a response, a CTA's
 
 struct SpreadArgs {
   const float* coef;
@@ -127,7 +148,7 @@ struct SpreadArgs {
   Mask mask[2];
   float* grad[2];
   int64_t T[2];
-  int64_t B, chunks[2];  // chunks of kSpread * 4 steps in a response
+  int64_t B, chunks[2];  // CTAs of a response
 };
 
 // grad = coefficient of the response where its step counts.
@@ -136,12 +157,19 @@ __global__ void __launch_bounds__(kSpread) preference_spread_kernel(SpreadArgs a
   const int k = id >= a.B * a.chunks[0] ? 1 : 0;
   if (k) id -= a.B * a.chunks[0];
   const int64_t b = id / a.chunks[k], c = id - b * a.chunks[k];
-  const int64_t T = a.T[k], t0 = c * (kSpread * 4);
+  const int64_t T = a.T[k], t0 = c * kSpreadSteps, i0 = b * T;
   const float w = a.coef[k * a.B + b] * *a.g;
-  const int64_t t1 = t0 + kSpread * 4 < T ? t0 + kSpread * 4 : T;
-  for (int64_t t = t0 + threadIdx.x; t < t1; t += kSpread) {
-    const int64_t i = b * T + t;
-    a.grad[k][i] = mask_at(a.mask[k], i) ? w : 0.f;
+  const int64_t t1 = t0 + kSpreadSteps < T ? t0 + kSpreadSteps : T;
+  if (T % 4 == 0 && ((uintptr_t)a.grad[k] & 15) == 0) {
+#pragma unroll 4
+    for (int64_t t = t0 + threadIdx.x * 4; t < t1; t += kSpread * 4) {
+      const unsigned m = mask_four(a.mask[k], i0 + t, i0 + T);
+      __stcs(reinterpret_cast<float4*>(a.grad[k] + i0 + t),
+             make_float4(m & 1u ? w : 0.f, m & 2u ? w : 0.f, m & 4u ? w : 0.f, m & 8u ? w : 0.f));
+    }
+  } else {
+#pragma unroll 4
+    for (int64_t t = t0 + threadIdx.x; t < t1; t += kSpread) a.grad[k][i0 + t] = mask_at(a.mask[k], i0 + t) ? w : 0.f;
   }
 }
 
@@ -162,7 +190,7 @@ extern "C" int rls_preference_loss(const float* chosen, const float* rejected, c
                                    const float* ref_rejected, int ref_per_pair, const void* chosen_mask,
                                    const void* rejected_mask, int mask_kind, int64_t pairs, int64_t chosen_len,
                                    int64_t rejected_len, float beta, float smoothing, int kind,
-                                   int length_normalized, float* loss, float* rewards, float* coef, void* ws,
+                                   int length_normalized, float* loss, float* chosen_rewards, float* rejected_rewards, float* coef, void* ws,
                                    size_t ws_bytes, void* stream) {
   if (!sizes_ok(pairs, chosen_len, rejected_len) || !loss) return RLS_EINVAL;
   if (kind < RLS_PREFERENCE_SIGMOID || kind > RLS_PREFERENCE_HINGE) return RLS_EINVAL;
@@ -176,14 +204,15 @@ extern "C" int rls_preference_loss(const float* chosen, const float* rejected, c
     return cudaMemsetAsync(loss, 0, sizeof(float), s) == cudaSuccess ? RLS_OK : RLS_ECUDA;
   }
   if (pairs > 0x7fffffffLL) return RLS_EINVAL;
-  if ((chosen_len > 0 && !chosen) || (rejected_len > 0 && !rejected) || !rewards || !ws) return RLS_EINVAL;
-  if (!al(chosen, 16) || !al(rejected, 16) || !al(ref_chosen, ref_per_pair ? 4 : 16) ||
-      !al(ref_rejected, ref_per_pair ? 4 : 16) || !al(rewards, 4) || !al(coef, 4) || !al(loss, 4) || !al(ws, 16) ||
+  if ((chosen_len > 0 && !chosen) || (rejected_len > 0 && !rejected) || !chosen_rewards ||
+      !rejected_rewards || !ws) return RLS_EINVAL;
+  if (!al(chosen, 4) || !al(rejected, 4) || !al(ref_chosen, 4) || !al(ref_rejected, 4) || !al(chosen_rewards, 4) ||
+      !al(rejected_rewards, 4) || !al(coef, 4) || !al(loss, 4) || !al(ws, 16) ||
       !al(chosen_mask, mask_align(mask_kind)) || !al(rejected_mask, mask_align(mask_kind)))
     return RLS_EALIGN;
   if (64 + (size_t)pairs * sizeof(double) > ws_bytes) return RLS_EWORKSPACE;
   DeviceGuard guard{chosen_len ? chosen : nullptr, rejected_len ? rejected : nullptr, ref_chosen, ref_rejected,
-                    chosen_mask, rejected_mask, loss, rewards, coef, ws};
+                    chosen_mask, rejected_mask, loss, chosen_rewards, rejected_rewards, coef, ws};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   if (int st = prepare_layout(ws, ws_bytes, kLayoutScratch, s)) return st;
@@ -197,7 +226,8 @@ extern "C" int rls_preference_loss(const float* chosen, const float* rejected, c
   p.kind = kind;
   p.normalized = length_normalized != 0;
   p.loss = loss;
-  p.rewards = rewards;
+  p.rewards[0] = chosen_rewards;
+  p.rewards[1] = rejected_rewards;
   p.coef = coef;
   p.terms = reinterpret_cast<double*>(static_cast<char*>(ws) + 64);
   p.ticket = &static_cast<WsHeader*>(ws)->pad[4];
@@ -212,7 +242,7 @@ extern "C" int rls_preference_loss_backward(const float* coef, const float* grad
   if (!sizes_ok(pairs, chosen_len, rejected_len)) return RLS_EINVAL;
   if (mask_kind < RLS_MASK_NONE || mask_kind > RLS_MASK_I64) return RLS_EINVAL;
   if ((chosen_mask || rejected_mask) && mask_kind == RLS_MASK_NONE) return RLS_EINVAL;
-  const int64_t per = kSpread * 4;
+  const int64_t per = kSpreadSteps;
   // a side without a gradient takes no blocks
   const int64_t c0 = grad_chosen ? (chosen_len + per - 1) / per : 0;
   const int64_t c1 = grad_rejected ? (rejected_len + per - 1) / per : 0;
@@ -220,7 +250,7 @@ extern "C" int rls_preference_loss_backward(const float* coef, const float* grad
   if (blocks == 0) return RLS_OK;
   if (blocks > 0x7fffffffLL) return RLS_EINVAL;
   if (!coef || !grad_loss) return RLS_EINVAL;
-  if (!al(coef, 4) || !al(grad_loss, 4) || !al(grad_chosen, 16) || !al(grad_rejected, 16) ||
+  if (!al(coef, 4) || !al(grad_loss, 4) || !al(grad_chosen, 4) || !al(grad_rejected, 4) ||
       !al(chosen_mask, mask_align(mask_kind)) || !al(rejected_mask, mask_align(mask_kind)))
     return RLS_EALIGN;
   DeviceGuard guard{coef, grad_loss, chosen_mask, rejected_mask, grad_chosen, grad_rejected};

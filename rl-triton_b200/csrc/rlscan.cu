@@ -20,6 +20,9 @@
 
 using namespace rls;
 
+static thread_local int g_assumed_device = -1;
+int rls::assumed_device() { return g_assumed_device; }
+
 namespace rls {
 std::recursive_mutex& launch_mutex() {
   static std::recursive_mutex mu;
@@ -757,6 +760,12 @@ int rls_workspace_error(void* ws, void* stream) {
     cudaStreamSynchronize(s);
   }
   return (int)h;
+}
+
+int rls_assume_device(int device) {
+  const int before = g_assumed_device;
+  g_assumed_device = device < 0 ? -1 : device;
+  return before;
 }
 
 const char* rls_status_string(int status) {

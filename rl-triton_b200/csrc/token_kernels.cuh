@@ -98,6 +98,19 @@ __device__ __forceinline__ bool mask_at(const Mask& m, int64_t i) {
   }
 }
 
+// Bits 0 .. 3: steps i .. i + 3 (i a multiple of 4; none past the end M).
+__device__ __forceinline__ unsigned mask_four(const Mask& m, int64_t i, int64_t M) {
+  if (m.kind == RLS_MASK_NONE) return i + 4 <= M ? 15u : (1u << (M - i)) - 1u;
+  if (m.kind == RLS_MASK_U8 && i + 4 <= M && ((uintptr_t)m.p & 3) == 0) {
+    const unsigned w = *reinterpret_cast<const unsigned*>(reinterpret_cast<const uint8_t*>(m.p) + i);
+    return ((w & 0xffu) != 0) | ((w & 0xff00u) != 0) << 1 | ((w & 0xff0000u) != 0) << 2 | ((w & 0xff000000u) != 0) << 3;
+  }
+  unsigned b = 0;
+  for (int e = 0; e < 4; ++e)
+    if (i + e < M && mask_at(m, i + e)) b |= 1u << e;
+  return b;
+}
+
 // ---- rows ------------------------------------------------------------------
 // row / seq by a multiplication, for rows below 2^31 (else by a division):
 // q = (umulhi(n, mul) + n) >> shift, shift = ceil(log2 seq),
@@ -471,9 +484,9 @@ struct Policy {
   const float* adv;
   bool adv_row;          // adv holds one value a row of the batch
   const float* ref;      // may be null
-  float lo, hi;          // ratio bounds
-  double log_lo, log_hi, log_dual;  // their logarithms: -inf, +inf where there is none
-  float dual;
+  float lo, hi, dual;    // ratio bounds
+  // their logarithms as sums of two floats; -inf, +inf where there is none
+  float2 log_lo, log_hi, log_dual;
   float kl_coef;
   int kl_kind;
   float ent_coef;
@@ -495,45 +508,59 @@ struct PolicyTerm {
   bool clipped;
 };
 
+// A difference of log-probabilities as the sum of two floats (low: what the first leaves).
+struct Diff {
+  float x, low;
+};
+__device__ __forceinline__ Diff diff(double a, float b) {
+  const double d = a - (double)b;
+  const float x = (float)d;
+  return Diff{x, fabsf(x) < INFINITY ? (float)(d - (double)x) : 0.f};
+}
+// The same of two floats, exactly (Knuth's two-sum).
+__device__ __forceinline__ Diff diff(float a, float b) {
+  const float x = __fsub_rn(a, b), v = __fsub_rn(x, a);
+  const float low = __fsub_rn(__fsub_rn(a, __fsub_rn(x, v)), __fadd_rn(b, v));
+  return Diff{x, fabsf(x) < INFINITY ? low : 0.f};
+}
+__device__ __forceinline__ Diff minus(Diff d) { return Diff{-d.x, -d.low}; }
+__device__ __forceinline__ bool above(Diff d, float2 bound) {
+  return (d.x - bound.x) + (d.low - bound.y) > 0.f;  // d.x - bound.x is exact where it is small
+}
+__device__ __forceinline__ bool below(Diff d, float2 bound) {
+  return (d.x - bound.x) + (d.low - bound.y) < 0.f;
+}
+
 // r - 1 - log r
-__device__ __forceinline__ float drift_of(double lp, float old_lp) {
-  const float lr = (float)(lp - (double)old_lp);
-  return expm1f(lr) - lr;
+__device__ __forceinline__ float drift_of(Diff lr) {
+  return expm1f(lr.x) - lr.x;
 }
 
 // -min(r A, clip(r) A), at most -dual A where A < 0, plus the KL estimate:
 // k1 = lp - ref, k2 = (lp - ref)^2 / 2, k3 = exp(ref - lp) - (ref - lp) - 1.
-// Whether the clip holds is decided on log r in fp64 (exact for fp32 inputs):
-// the derivative jumps there, and exp's rounding would put steps near a bound
-// on either side of it.
-__device__ __forceinline__ PolicyTerm policy_term(const Policy& p, double lp, float old_lp, float adv, float ref) {
+// Whether the clip holds is decided on log r with twice fp32's digits (exact for
+// fp32 inputs): the derivative jumps there, and exp's rounding would put
+// steps near a bound on either side of it.  lr = lp - old, away = lp - ref.
+__device__ __forceinline__ PolicyTerm policy_term(const Policy& p, Diff lr, float adv, Diff away) {
   PolicyTerm o;
-  const double lr64 = lp - (double)old_lp;
-  const float lr = (float)lr64, lr_low = (float)(lr64 - (double)lr);  // the part that fp32 drops
-  float gain = expf(lr);
-  if (gain < INFINITY) gain = fmaf(gain, lr_low, gain);
+  float gain = expf(lr.x);
+  if (gain < INFINITY) gain = fmaf(gain, lr.low, gain);
   gain *= adv;
-  o.loss = -gain;
-  o.d = -gain;
-  o.clipped = false;
-  if (adv > 0.f) {
-    if (lr64 > p.log_hi) { o.loss = -p.hi * adv; o.clipped = true; }
-  } else if (adv < 0.f) {
-    if (lr64 < p.log_lo) { o.loss = -p.lo * adv; o.clipped = true; }
-    else if (lr64 > p.log_dual) { o.loss = -p.dual * adv; o.clipped = true; }
-  }
-  if (o.clipped) o.d = 0.f;
+  const bool up = above(lr, p.log_hi), down = below(lr, p.log_lo), far = above(lr, p.log_dual);
+  o.clipped = adv > 0.f ? up : adv < 0.f && (down || far);
+  const float held = adv > 0.f ? p.hi : down ? p.lo : p.dual;
+  o.loss = o.clipped ? -held * adv : -gain;
+  o.d = o.clipped ? 0.f : -gain;
   o.kl = 0.f;
   if (p.ref) {
-    const double x64 = (double)ref - lp;
-    const float x = (float)x64, x_low = (float)(x64 - (double)x);
+    const Diff x = minus(away);
     float dk;
-    if (p.kl_kind == RLS_KL_K1) { o.kl = -x; dk = 1.f; }
-    else if (p.kl_kind == RLS_KL_K2) { o.kl = 0.5f * x * x; dk = -x; }
+    if (p.kl_kind == RLS_KL_K1) { o.kl = -x.x; dk = 1.f; }
+    else if (p.kl_kind == RLS_KL_K2) { o.kl = 0.5f * x.x * x.x; dk = -x.x; }
     else {
-      float e = expm1f(x);
-      if (fabsf(x) < INFINITY) e = fmaf(e + 1.f, x_low, e);
-      o.kl = e - x;
+      float e = expm1f(x.x);
+      if (e < INFINITY) e = fmaf(e + 1.f, x.low, e);
+      o.kl = e - x.x;
       dk = -e;
     }
     if (p.kl_coef != 0.f) {
@@ -816,14 +843,15 @@ __global__ void __launch_bounds__(NT) cta_rows_kernel(Rows<T> in, RowOut out, Gr
       if constexpr (Src::kPolicy) {
         const int64_t env = in.env(row);
         const Policy& p = src.p;
-        const PolicyTerm o = policy_term(p, lp, p.old_lp[row], p.adv[p.adv_row ? env : row], p.ref ? p.ref[row] : 0.f);
+        const PolicyTerm o = policy_term(p, diff(lp, p.old_lp[row]), p.adv[p.adv_row ? env : row],
+                                         diff(lp, p.ref ? p.ref[row] : 0.f));
         const float w = policy_weight(p, env);
         a = w * o.d;
         if constexpr (ENT) b = -w * p.ent_coef;
         if (o.clipped) flags |= kFlagClipped;
         if (threadIdx.x == 0) {
           const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
-          out.stats[2 * row + 1] = make_float4(a, w * term, o.kl, drift_of(lp, p.old_lp[row]));
+          out.stats[2 * row + 1] = make_float4(a, w * term, o.kl, drift_of(diff(lp, p.old_lp[row])));
         }
       }
       if (threadIdx.x == 0) {
@@ -1252,7 +1280,7 @@ struct Walk {
     Result q{};
     q.lp = logprob_of(ex.xt, r, in.c, in.c64, in.c_off);
     if constexpr (Src::kPolicy) {
-      q.o = policy_term(src.p, q.lp, ex.old_lp, ex.adv, ex.ref);
+      q.o = policy_term(src.p, diff(q.lp, ex.old_lp), ex.adv, diff(q.lp, ex.ref));
       a = ex.w * q.o.d;
       b = ENT ? -ex.w * src.p.ent_coef : 0.f;
     }
@@ -1266,7 +1294,7 @@ struct Walk {
     if constexpr (Src::kPolicy) {
       const float term = ENT && src.p.ent_coef != 0.f ? q.o.loss - src.p.ent_coef * ent : q.o.loss;
       if (q.o.clipped) flags |= kFlagClipped;
-      out.stats[2 * row + 1] = make_float4(a, ex.w * term, q.o.kl, drift_of(q.lp, ex.old_lp));
+      out.stats[2 * row + 1] = make_float4(a, ex.w * term, q.o.kl, drift_of(diff(q.lp, ex.old_lp)));
     }
     out.logprob[row] = (float)q.lp;
     if (out.entropy) out.entropy[row] = ent;
@@ -1675,14 +1703,14 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) tile_rows_kernel(Rows
         if constexpr (ENT && MODE != kBwd) ent = entropy_of(st);
         if constexpr (Src::kPolicy) {
           const Policy& p = src.p;
-          const PolicyTerm o = policy_term(p, lp, old_lp, adv, ref);
+          const PolicyTerm o = policy_term(p, diff(lp, old_lp), adv, diff(lp, ref));
           a = w * o.d;
           if constexpr (ENT) b = -w * p.ent_coef;
           if constexpr (kTerms) {
             const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
             sum[0] += (double)w * (double)term;
             if (src.sums.stats) {
-              sum[1] += o.kl; sum[2] += drift_of(lp, old_lp); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent;
+              sum[1] += o.kl; sum[2] += drift_of(diff(lp, old_lp)); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent;
               sum[5] += 1.0;
             }
           }
@@ -1810,7 +1838,8 @@ __global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, 
       if constexpr (Src::kPolicy) {
         const int64_t env = in.env(row);
         const Policy& p = src.p;
-        const PolicyTerm o = policy_term(p, lp, p.old_lp[row], p.adv[p.adv_row ? env : row], p.ref ? p.ref[row] : 0.f);
+        const PolicyTerm o = policy_term(p, diff(lp, p.old_lp[row]), p.adv[p.adv_row ? env : row],
+                                         diff(lp, p.ref ? p.ref[row] : 0.f));
         const float w = policy_weight(p, env);
         a = w * o.d;
         if constexpr (ENT) b = -w * p.ent_coef;
@@ -1818,7 +1847,7 @@ __global__ void __launch_bounds__(256) lane_rows_kernel(Rows<T> in, RowOut out, 
           if (live && lane == 0) {
             const float term = ENT && p.ent_coef != 0.f ? o.loss - p.ent_coef * ent : o.loss;
             sum[0] += (double)w * (double)term;
-            sum[1] += o.kl; sum[2] += drift_of(lp, p.old_lp[row]); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent; sum[5] += 1.0;
+            sum[1] += o.kl; sum[2] += drift_of(diff(lp, p.old_lp[row])); sum[3] += o.clipped ? 1.0 : 0.0; sum[4] += ent; sum[5] += 1.0;
           }
         }
         a *= src.up();

@@ -18,8 +18,6 @@ constexpr int kThreads = 256;
 // The ticket and the counts lie in words of the workspace header that the
 // estimators do not use; every launch leaves them zero.
 unsigned* ticket_of(void* ws) { return &static_cast<WsHeader*>(ws)->pad[4]; }
-unsigned long long* total_of(void* ws) { return reinterpret_cast<unsigned long long*>(&static_cast<WsHeader*>(ws)->pad[6]); }
-unsigned* rows_of(void* ws) { return &static_cast<WsHeader*>(ws)->pad[8]; }
 static_assert(offsetof(WsHeader, pad) % 8 == 0, "the total is 8-byte aligned");
 
 int num_sms() {
@@ -34,78 +32,114 @@ int num_sms() {
   return sms[dev];
 }
 
-// ---- what the steps' weights come from ------------------------------------------
-// norm[1 + n] = steps of env n that count; norm[0] = 1 / (all of them), or
-// 1 / (envs that have any) for the mean by sequence.  Counts are whole numbers:
-// their atomics give the same sum in any order.
+// ---- the mask once over -------------------------------------------------------------
+// norm (may be null): norm[1 + n] = steps of env n that count; norm[0] = 1 / (all of
+// them), or 1 / (envs that have any) for the mean by sequence.  order (may be null):
+// order[0] = all of them, order[1 ..] = those rows, then the others; which row comes
+// where depends on timing, nothing that a row gives does.  Counts are whole numbers: their
+// atomics give the same sum in any order.
+struct CountWords {
+  unsigned long long* total;
+  unsigned *some, *front, *back, *ticket;
+};
+// A thread's share (of NT) of the steps that count among T from i0 on.
+template <int NT>
+__device__ __forceinline__ unsigned count_steps(const Mask& mask, int64_t i0, int64_t T, int tid) {
+  unsigned c = 0;
+  int64_t t = 0;
+  if (mask.kind == RLS_MASK_U8) {  // 16 bytes at a time from the first boundary on
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(mask.p) + i0;
+    const int64_t head = (int64_t)((16 - ((uintptr_t)p & 15)) & 15), lead = head < T ? head : T;
+    if (tid < lead) c += p[tid] != 0;
+    const int64_t vecs = (T - lead) / 16;
+#pragma unroll 4
+    for (int64_t v = tid; v < vecs; v += NT) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p + lead + v * 16);
+      c += __popc(__vsetne4(w.x, 0u)) + __popc(__vsetne4(w.y, 0u)) + __popc(__vsetne4(w.z, 0u)) +
+           __popc(__vsetne4(w.w, 0u));
+    }
+    t = lead + vecs * 16;
+  }
+  for (t += tid; t < T; t += NT) c += mask_at(mask, i0 + t) ? 1u : 0u;
+  return c;
+}
+
 __global__ void __launch_bounds__(kThreads) count_kernel(Mask mask, int64_t N, int64_t T, int reduction, float* norm,
-                                                         unsigned long long* total, unsigned* some, unsigned* ticket) {
-  __shared__ unsigned part[kThreads / 32];
+                                                         int* order, bool warps, CountWords words) {
+  __shared__ unsigned part[kThreads / 32], base[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned long long sum = 0;
   unsigned rows = 0;
+  if (warps) {  // many envs: a warp each
+    for (int64_t n = (int64_t)blockIdx.x * (kThreads / 32) + warp; n < N; n += (int64_t)gridDim.x * (kThreads / 32)) {
+      const unsigned c = __reduce_add_sync(0xffffffffu, count_steps<32>(mask, n * T, T, lane));
+      if (lane == 0 && norm) norm[1 + n] = (float)c;
+      sum += c;
+      rows += c > 0;
+    }
+    __syncthreads();
+    if (lane == 0) {
+      part[warp] = rows;
+      atomicAdd(words.total, sum);
+    }
+    __syncthreads();
+    sum = 0;
+    rows = 0;
+    for (int w = 0; w < kThreads / 32; ++w) rows += part[w];
+    N = 0;
+  }
   for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
-    unsigned c = 0;
-    for (int64_t t = threadIdx.x; t < T; t += kThreads) c += mask_at(mask, n * T + t) ? 1u : 0u;
+    const int64_t i0 = n * T;
+    unsigned c = count_steps<kThreads>(mask, i0, T, tid);
     c = __reduce_add_sync(0xffffffffu, c);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = c;
+    if (lane == 0) part[warp] = c;
     __syncthreads();
     c = 0;
     for (int w = 0; w < kThreads / 32; ++w) c += part[w];
-    if (threadIdx.x == 0) norm[1 + n] = (float)c;
     sum += c;
     rows += c > 0;
-  }
-  if (threadIdx.x == 0) {
-    atomicAdd(total, sum);
-    atomicAdd(some, rows);
-    __threadfence();
-    if (atomicAdd(ticket, 1u) == gridDim.x - 1) {
-      __threadfence();
-      const unsigned long long all = atomicExch(total, 0ull);
-      const unsigned envs = atomicExch(some, 0u);
-      const double by = reduction == RLS_REDUCE_SEQUENCE ? (double)envs : (double)all;
-      norm[0] = by > 0.0 ? (float)(1.0 / by) : 0.f;
-      *ticket = 0u;
-    }
-  }
-}
-
-// ---- an order of the rows -----------------------------------------------------------
-// order[0] = the number of rows that count, order[1 ..] = those, then the others.
-// Which row comes where depends on timing; nothing that a row gives does.
-__global__ void __launch_bounds__(kThreads) order_kernel(Mask mask, int rows, int* order, unsigned* front,
-                                                         unsigned* back, unsigned* ticket) {
-  __shared__ unsigned counts[kThreads / 32], base[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int64_t row0 = (int64_t)blockIdx.x * kThreads; row0 < rows; row0 += (int64_t)gridDim.x * kThreads) {
-    const int64_t row = row0 + tid;
-    const bool there = row < rows, yes = there && mask_at(mask, row);
-    const unsigned votes = __ballot_sync(0xffffffffu, yes);
-    if (lane == 0) counts[warp] = __popc(votes);
-    __syncthreads();
-    unsigned before = 0, all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += counts[w];
-      all += counts[w];
-    }
-    const unsigned here = (unsigned)(rows - row0 < kThreads ? rows - row0 : kThreads);
     if (tid == 0) {
-      base[0] = atomicAdd(front, all);
-      base[1] = atomicAdd(back, here - all);
+      if (norm) norm[1 + n] = (float)c;
+      if (order) {
+        base[0] = atomicAdd(words.front, c);
+        base[1] = atomicAdd(words.back, (unsigned)T - c);
+      }
     }
-    __syncthreads();
-    const unsigned rank = before + __popc(votes & ((1u << lane) - 1u));
-    if (there) order[1 + (yes ? (int64_t)(base[0] + rank) : rows - 1 - (int64_t)(base[1] + tid - rank))] = (int)row;
-    __syncthreads();
+    if (order) {
+      const int64_t last = N * T;  // order's last place
+      unsigned yes_before = 0;     // of the env, before the chunk
+      for (int64_t t0 = 0; t0 < T; t0 += kThreads) {
+        const int64_t u = t0 + tid;
+        const bool there = u < T, yes = there && mask_at(mask, i0 + u);
+        const unsigned votes = __ballot_sync(0xffffffffu, yes);
+        __syncthreads();
+        if (lane == 0) part[warp] = __popc(votes);
+        __syncthreads();
+        unsigned before = yes_before;
+        for (int w = 0; w < kThreads / 32; ++w) {
+          if (w < warp) before += part[w];
+          yes_before += part[w];
+        }
+        const unsigned rank = before + __popc(votes & ((1u << lane) - 1u));
+        if (there) order[yes ? 1 + (int64_t)(base[0] + rank) : last - (int64_t)(base[1] + (unsigned)u - rank)] = (int)(i0 + u);
+      }
+    }
   }
   if (tid == 0) {
+    atomicAdd(words.total, sum);
+    atomicAdd(words.some, rows);
     __threadfence();
-    if (atomicAdd(ticket, 1u) == gridDim.x - 1) {
+    if (atomicAdd(words.ticket, 1u) == gridDim.x - 1) {
       __threadfence();
-      order[0] = (int)atomicExch(front, 0u);
-      atomicExch(back, 0u);
-      *ticket = 0u;
+      const unsigned long long all = atomicExch(words.total, 0ull);
+      const unsigned envs = atomicExch(words.some, 0u);
+      atomicExch(words.front, 0u);
+      atomicExch(words.back, 0u);
+      const double by = reduction == RLS_REDUCE_SEQUENCE ? (double)envs : (double)all;
+      if (norm) norm[0] = by > 0.0 ? (float)(1.0 / by) : 0.f;
+      if (order) order[0] = (int)all;
+      *words.ticket = 0u;
     }
   }
 }
@@ -159,8 +193,9 @@ __device__ __forceinline__ void count_alone(const Mask& mask, int N, int T, int 
   __syncthreads();
 }
 
+constexpr int kPolicyCtas = 5;  // an SM
 template <bool SUMS, bool GRAD, bool COUNT, int NT>
-__global__ void __launch_bounds__(NT) policy_kernel(Terms t, float scale, const float* g, int force, float* grad,
+__global__ void __launch_bounds__(NT, NT == kThreads ? kPolicyCtas : 1) policy_kernel(Terms t, float scale, const float* g, int force, float* grad,
                                                     float* norm, SumOut out) {
   if constexpr (!SUMS) {
     if (g && !force && *g == scale) return;
@@ -171,29 +206,37 @@ __global__ void __launch_bounds__(NT) policy_kernel(Terms t, float scale, const 
   const int64_t step = (int64_t)gridDim.x * NT * 4;
   for (int64_t i = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4; i < t.M; i += step) {
     float lp[4], old_lp[4], adv[4], ref[4], d[4];
+    const unsigned mask = mask_four(t.mask, i, t.M);
     load4(t.lp, i, t.M, lp);
     load4(t.p.old_lp, i, t.M, old_lp);
     if (!t.p.adv_row) load4(t.p.adv, i, t.M, adv);
     if (t.p.ref) load4(t.p.ref, i, t.M, ref);
     int64_t env = t.env(i), col = i - env * t.T;
+    float w = policy_weight(t.p, env), a_row = t.p.adv_row ? t.p.adv[env] : 0.f;
+    float loss = 0.f;  // of the four
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       d[e] = 0.f;
-      if (i + e < t.M && mask_at(t.mask, i + e)) {
-        const PolicyTerm o = policy_term(t.p, (double)lp[e], old_lp[e], t.p.adv_row ? t.p.adv[env] : adv[e],
-                                         t.p.ref ? ref[e] : 0.f);
-        const float w = policy_weight(t.p, env);
+      if (mask >> e & 1u) {
+        const Diff lr = diff(lp[e], old_lp[e]);
+        const PolicyTerm o = policy_term(t.p, lr, t.p.adv_row ? a_row : adv[e], diff(lp[e], t.p.ref ? ref[e] : 0.f));
         d[e] = w * o.d * up;
         if constexpr (SUMS) {
-          sum[0] += (double)w * (double)o.loss;
+          loss = fmaf(w, o.loss, loss);
           if (out.stats) {
-            sum[1] += o.kl; sum[2] += drift_of((double)lp[e], old_lp[e]); sum[3] += o.clipped ? 1.0 : 0.0;
+            sum[1] += o.kl; sum[2] += drift_of(lr); sum[3] += o.clipped ? 1.0 : 0.0;
             sum[5] += 1.0;
           }
         }
       }
-      if (++col == t.T) { col = 0; ++env; }
+      if (++col == t.T && e < 3 && i + e + 1 < t.M) {
+        col = 0;
+        ++env;
+        w = policy_weight(t.p, env);
+        if (t.p.adv_row) a_row = t.p.adv[env];
+      }
     }
+    if constexpr (SUMS) sum[0] += (double)loss;
     if constexpr (GRAD) {
       if (i + 4 <= t.M) {
         *reinterpret_cast<float4*>(grad + i) = make_float4(d[0], d[1], d[2], d[3]);
@@ -246,9 +289,13 @@ Policy make_policy(const rls_policy_t& q, const float* old_lp, const float* adv,
   p.lo = 1.f - q.clip_low;
   p.hi = 1.f + q.clip_high;
   p.dual = q.dual_clip;
-  p.log_lo = q.clip_low < 1.f ? std::log1p(-(double)q.clip_low) : -INFINITY;
-  p.log_hi = std::log1p((double)q.clip_high);
-  p.log_dual = q.dual_clip > 0.f ? std::log((double)q.dual_clip) : INFINITY;
+  auto two = [](double x) {
+    const float a = (float)x;
+    return make_float2(a, std::isfinite(x) ? (float)(x - (double)a) : 0.f);
+  };
+  p.log_lo = two(q.clip_low < 1.f ? std::log1p(-(double)q.clip_low) : -INFINITY);
+  p.log_hi = two(std::log1p((double)q.clip_high));
+  p.log_dual = two(q.dual_clip > 0.f ? std::log((double)q.dual_clip) : INFINITY);
   p.kl_coef = q.kl_coef;
   p.kl_kind = q.kl_kind;
   p.ent_coef = q.entropy_coef;
@@ -259,15 +306,26 @@ Policy make_policy(const rls_policy_t& q, const float* old_lp, const float* adv,
   return p;
 }
 
-int launch_count(const Policy& p, const Mask& mask, float* norm, int64_t N, int64_t T, void* ws, cudaStream_t s) {
-  if (!p.norm) return RLS_OK;
-  const int64_t blocks = N < 8LL * num_sms() ? N : 8LL * num_sms();
-  count_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(mask, N, T, p.reduction, norm, total_of(ws), rows_of(ws),
-                                                     ticket_of(ws));
+CountWords count_words(void* ws) {
+  unsigned* pad = static_cast<WsHeader*>(ws)->pad;
+  return CountWords{reinterpret_cast<unsigned long long*>(&pad[6]), &pad[8], &pad[9], &pad[10], ticket_of(ws)};
+}
+
+// norm and order may be null.
+int launch_count(int reduction, const Mask& mask, float* norm, int* order, int64_t N, int64_t T, void* ws,
+                 cudaStream_t s) {
+  if (!norm && !order) return RLS_OK;
+  int64_t blocks = N < 8LL * num_sms() ? N : 8LL * num_sms();
+  const bool warps = !order && N > 16 * num_sms();
+  if (warps && (N + 7) / 8 < blocks) blocks = (N + 7) / 8;
+  count_kernel<<<(unsigned)blocks, kThreads, 0, s>>>(mask, N, T, reduction, norm, order, warps, count_words(ws));
   return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
 }
 
-int64_t policy_blocks(int64_t M) { return sum_blocks((M + kThreads * 4 - 1) / (kThreads * 4)); }
+int64_t policy_blocks(int64_t M) {
+  const int64_t need = (M + kThreads * 4 - 1) / (kThreads * 4), most = (int64_t)kPolicyCtas * num_sms();
+  return need < most ? need : most;
+}
 
 // Where a call of `blocks` CTAs leaves its sums.
 int sums_in(void* ws, size_t wsb, int64_t blocks, float* loss, float* stats, cudaStream_t s, SumOut* o) {
@@ -391,11 +449,8 @@ extern "C" int rls_row_order(const void* mask, int mask_kind, int64_t num_envs, 
   DeviceGuard guard{mask, order, ws};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
-  const int64_t rows = num_envs * seq_len, need = (rows + kThreads - 1) / kThreads;
-  unsigned* pad = static_cast<WsHeader*>(ws)->pad;
-  order_kernel<<<(unsigned)sum_blocks(need), kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      Mask{mask, mask_kind}, (int)rows, order, &pad[9], &pad[10], ticket_of(ws));
-  return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;
+  return launch_count(RLS_REDUCE_TOKEN, Mask{mask, mask_kind}, nullptr, order, num_envs, seq_len, ws,
+                      reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int rls_token_logprobs(const void* logits, int64_t env_stride, int64_t step_stride, const int64_t* tokens,
@@ -472,7 +527,8 @@ extern "C" int rls_policy_loss(const float* logprobs, const float* old_logprobs,
                                        : policy_kernel<true, false, false, kAloneThreads>);
     kern<<<1, kAloneThreads, 0, s>>>(t, grad_scale, nullptr, 0, grad_logprobs, norm, sums);
   } else {
-    if (int st = launch_count(t.p, t.mask, norm, num_envs, seq_len, ws, s)) return st;
+    if (int st = launch_count(t.p.reduction, t.mask, t.p.norm ? norm : nullptr, nullptr, num_envs, seq_len, ws, s))
+      return st;
     auto kern = grad_logprobs ? policy_kernel<true, true, false, kThreads> : policy_kernel<true, false, false, kThreads>;
     kern<<<(unsigned)blocks, kThreads, 0, s>>>(t, grad_scale, nullptr, 0, grad_logprobs, nullptr, sums);
   }
@@ -509,7 +565,7 @@ extern "C" int rls_policy_loss_backward(const float* logprobs, const float* old_
 extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, int64_t step_stride,
                                       const int64_t* tokens, const float* old_logprobs, const float* advantages,
                                       int advantages_per_env, const float* ref_logprobs, const void* mask,
-                                      int mask_kind, const int32_t* order, const rls_policy_t* policy, float grad_scale, float* norm,
+                                      int mask_kind, int32_t* order, const rls_policy_t* policy, float grad_scale, float* norm,
                                       float* logprobs, float* entropy, float* row_stats, float* loss, float* stats,
                                       void* grad_logits, int64_t grad_env_stride, int64_t grad_step_stride,
                                       int64_t num_envs, int64_t seq_len, int64_t vocab, double temperature,
@@ -538,7 +594,9 @@ extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, in
   PolicyGrad src{p, grad_scale, nullptr, false, SumOut{}, &static_cast<WsHeader*>(ws)->error};
   const int64_t blocks = sum_blocks((M + kThreads - 1) / kThreads);
   if (int st = sums_in(ws, ws_bytes, sum_blocks(M), loss, stats, s, &src.sums)) return st;
-  if (int st = launch_count(p, c.mask, norm, num_envs, seq_len, ws, s)) return st;
+  if (vocab <= kLaneVocab) order = nullptr;
+  if (int st = launch_count(p.reduction, c.mask, p.norm ? norm : nullptr, order, num_envs, seq_len, ws, s)) return st;
+  c.order = order;
   const RowOut ro{logprobs, entropy, reinterpret_cast<float4*>(row_stats)};
   if (int st = launch_logits<kBoth>(c, entropy != nullptr, ro, src, s)) return st;
   if (vocab <= kLaneVocab) return RLS_OK;  // its kernel added up the terms itself

@@ -44,6 +44,31 @@ OptT opt(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 Tensor plain(const OptT& t) { return t ? *t : Tensor(); }
 
 // ---- inputs ----------------------------------------------------------------------
+// Looks at every tensor's device, then spares the library its queries for the
+// calls in this scope.
+class Placed {
+ public:
+  template <class... Ts>
+  explicit Placed(const Tensor& first, const Ts&... rest) {
+    TORCH_CHECK(first.is_cuda(), "inputs must be on CUDA");
+    (same(first, rest), ...);
+    before_ = rls_assume_device(first.device().index());
+  }
+  ~Placed() { rls_assume_device(before_); }
+  Placed(const Placed&) = delete;
+  Placed& operator=(const Placed&) = delete;
+
+ private:
+  static void same(const Tensor& first, const Tensor& t) {
+    TORCH_CHECK(!t.defined() || t.device() == first.device(), "all tensors of one call must be on ", first.device(),
+                "; got a tensor on ", t.device());
+  }
+  static void same(const Tensor& first, const OptT& t) {
+    if (t) same(first, *t);
+  }
+  int before_;
+};
+
 struct MaskArg {
   OptT t;
   int kind = RLS_MASK_NONE;
@@ -103,9 +128,13 @@ struct LogitsArgs {
   LogitsArgs(const Tensor& logits, const Tensor& tok, const OptT& m)
       : x(logits_arg(logits)), tokens(tokens_arg(tok)), mask(mask_arg(m)), n(x.size(0)), t(x.size(1)), v(x.size(2)) {}
   // Long rows with a mask go by an order of the rows, made once for both directions.
+  Tensor order_buffer() const {
+    const bool some = mask.t && v > RLS_SHORT_VOCAB && n * t <= 0x7ffffffe;
+    return at::empty({some ? n * t + 1 : 0}, x.options().dtype(at::kInt));
+  }
   Tensor order() const {
-    if (!mask.t || v <= RLS_SHORT_VOCAB || n * t > 0x7ffffffe) return at::empty({0}, x.options().dtype(at::kInt));
-    Tensor o = at::empty({n * t + 1}, x.options().dtype(at::kInt));
+    Tensor o = order_buffer();
+    if (!o.numel()) return o;
     Tensor ws = workspace_for(x.device(), stream_of(x), 1 << 20);
     check(rls_row_order(mask.ptr(), mask.kind, n, t, o.data_ptr<int32_t>(), ws.data_ptr(), (size_t)ws.numel(),
                         stream_of(x)),
@@ -113,7 +142,7 @@ struct LogitsArgs {
     return o;
   }
 };
-const int32_t* I(const Tensor& t) { return t.numel() ? t.data_ptr<int32_t>() : nullptr; }
+int32_t* I(const Tensor& t) { return t.numel() ? t.data_ptr<int32_t>() : nullptr; }
 
 Tensor like(const Tensor& t, at::IntArrayRef sizes) { return at::empty(sizes, t.options().dtype(at::kFloat)); }
 
@@ -126,6 +155,7 @@ Tensor row_stats(const LogitsArgs& a, bool keep) {
 // (logprobs, entropy or empty, the rows' statistics or empty, their order or empty)
 std::tuple<Tensor, Tensor, Tensor, Tensor> op_logprobs(const Tensor& logits, const Tensor& tokens, const OptT& mask,
                                                double temperature, bool entropy, bool keep) {
+  const Placed placed(logits, tokens, mask);
   const LogitsArgs a(logits, tokens, mask);
   Tensor lp = like(a.x, {a.n, a.t});
   Tensor ent = like(a.x, entropy ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
@@ -140,6 +170,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_logprobs(const Tensor& logits, con
 Tensor op_logprobs_backward(const Tensor& logits, const Tensor& tokens, const OptT& mask, const Tensor& order,
                             const Tensor& stats,
                             const OptT& g_lp, const OptT& g_ent, double temperature) {
+  const Placed placed(logits, tokens, mask, order, stats, g_lp, g_ent);
   const LogitsArgs a(logits, tokens, mask);
   const OptT gl = f32(g_lp), ge = f32(g_ent);
   Tensor g = op_grad_buffer(a.x);
@@ -176,6 +207,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_policy(const Tensor& logprobs, con
                                                      double clip_low, double clip_high, double dual_clip,
                                                      double kl_coef, int64_t kl, int64_t reduction, double grad_scale,
                                                      bool need_stats, bool need_grad) {
+  const Placed placed(logprobs, old_logprobs, advantages, mask, ref);
   const Tensor lp = f32(logprobs), old_lp = f32(old_logprobs), adv = f32(advantages);
   const OptT rf = f32(ref);
   const MaskArg m = mask_arg(mask);
@@ -195,6 +227,7 @@ void op_policy_backward_(Tensor& grad, const Tensor& logprobs, const Tensor& old
                          const OptT& mask, const OptT& ref, const Tensor& norm, const Tensor& grad_loss,
                          double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
                          int64_t reduction, double grad_scale, bool force) {
+  const Placed placed(grad, logprobs, old_logprobs, advantages, mask, ref, norm, grad_loss);
   const Tensor lp = f32(logprobs), old_lp = f32(old_logprobs), adv = f32(advantages), g = f32(grad_loss);
   const OptT rf = f32(ref);
   const MaskArg m = mask_arg(mask);
@@ -210,12 +243,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_po
     const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
     const OptT& mask, const OptT& ref, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
     double entropy_coef, bool need_stats, double temperature, int64_t reduction, double grad_scale, bool need_grad) {
+  const Placed placed(logits, tokens, old_logprobs, advantages, mask, ref);
   const LogitsArgs a(logits, tokens, mask);
   const Tensor old_lp = f32(old_logprobs), adv = f32(advantages);
   const OptT rf = f32(ref);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
   Tensor loss = like(a.x, {}), stats = like(a.x, {need_stats ? 5 : 0}), norm = norm_for(a.mask, a.x, a.n, reduction);
-  Tensor lp = like(a.x, {a.n, a.t}), rows = row_stats(a, true), order = a.order();
+  Tensor lp = like(a.x, {a.n, a.t}), rows = row_stats(a, true), order = a.order_buffer();
   Tensor ent = like(a.x, need_stats || entropy_coef != 0.0 ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
   Tensor g = need_grad ? op_grad_buffer(a.x) : at::empty({0}, a.x.options());
   Tensor ws = policy_workspace(a.x);
@@ -234,6 +268,7 @@ void op_policy_logits_backward_(Tensor& grad, const Tensor& logits, const Tensor
                                 const Tensor& order, const Tensor& rows, const Tensor& grad_loss, double clip_low,
                                 double clip_high, double dual_clip, double kl_coef, int64_t kl, double entropy_coef,
                                 double temperature, int64_t reduction, double grad_scale, bool force) {
+  const Placed placed(grad, logits, tokens, old_logprobs, advantages, mask, ref, norm, order, rows, grad_loss);
   const LogitsArgs a(logits, tokens, mask);
   const Tensor old_lp = f32(old_logprobs), adv = f32(advantages), up = f32(grad_loss);
   const OptT rf = f32(ref);
@@ -283,19 +318,14 @@ struct Pairs {
       }
       return;
     }
-    // The second half starts b rows into the first tensor.  A half whose rows
-    // leave it off the kernels' 16-byte boundary is copied.
+    // The second half starts b rows into the first tensor.
     b = lp[0].size(0) / 2;
     t[0] = t[1] = lp[0].size(1);
     const int64_t at = b * t[0];
-    if (at % 4 != 0 && at > 0) {
-      lp[1] = lp[0].slice(0, b).clone();
-      if (rf[0] && !ref_pair) rf[1] = rf[0]->slice(0, b).clone();
-    }
     p[0] = F(lp[0]);
-    p[1] = lp[1].defined() ? F(lp[1]) : p[0] + at;
+    p[1] = p[0] + at;
     ref[0] = F(rf[0]);
-    ref[1] = !rf[0] ? nullptr : rf[1] ? F(rf[1]) : ref[0] + (ref_pair ? b : at);
+    ref[1] = rf[0] ? ref[0] + (ref_pair ? b : at) : nullptr;
     mask[0] = m[0].ptr();
     kind = m[0].kind;
     const int64_t esz = m[0].t ? m[0].t->element_size() : 0;
@@ -303,20 +333,22 @@ struct Pairs {
   }
 };
 
-// (loss, rewards [2, pairs], coefficients [2, pairs])
-std::tuple<Tensor, Tensor, Tensor> op_preference(const Tensor& chosen, const OptT& rejected, const OptT& ref_chosen,
+// (loss, rewards of the chosen, of the rejected, coefficients [2, pairs])
+std::tuple<Tensor, Tensor, Tensor, Tensor> op_preference(const Tensor& chosen, const OptT& rejected, const OptT& ref_chosen,
                                                  const OptT& ref_rejected, const OptT& chosen_mask,
                                                  const OptT& rejected_mask, double beta, double smoothing,
                                                  int64_t kind, bool normalized) {
+  const Placed placed(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask);
   const Pairs q(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask);
-  Tensor loss = like(q.lp[0], {}), rewards = like(q.lp[0], {2, q.b}), coef = like(q.lp[0], {2, q.b});
+  Tensor loss = like(q.lp[0], {}), good = like(q.lp[0], {q.b}), bad = like(q.lp[0], {q.b});
+  Tensor coef = like(q.lp[0], {2, q.b});
   const int64_t want = 64 * q.b < (1 << 20) ? (1 << 20) : 64 * q.b;
   Tensor ws = workspace_for(q.lp[0].device(), stream_of(q.lp[0]), want);
   check(rls_preference_loss(q.p[0], q.p[1], q.ref[0], q.ref[1], q.ref_pair, q.mask[0], q.mask[1], q.kind, q.b, q.t[0],
                             q.t[1], (float)beta, (float)smoothing, (int)kind, normalized, loss.data_ptr<float>(),
-                            W(rewards), W(coef), ws.data_ptr(), (size_t)ws.numel(), stream_of(q.lp[0])),
+                            W(good), W(bad), W(coef), ws.data_ptr(), (size_t)ws.numel(), stream_of(q.lp[0])),
         "rls_preference_loss");
-  return {loss, rewards, coef};
+  return {loss, good, bad, coef};
 }
 
 // The gradients by (chosen, rejected); where `halves`, one gradient over both
@@ -324,6 +356,7 @@ std::tuple<Tensor, Tensor, Tensor> op_preference(const Tensor& chosen, const Opt
 std::tuple<Tensor, Tensor> op_preference_backward(const Tensor& coef, const Tensor& grad_loss,
                                                   const OptT& chosen_mask, const OptT& rejected_mask,
                                                   int64_t chosen_len, int64_t rejected_len, bool halves) {
+  const Placed placed(coef, grad_loss, chosen_mask, rejected_mask);
   const Tensor g = f32(grad_loss);
   const int64_t b = coef.size(1);
   MaskArg m[2] = {mask_arg(chosen_mask), mask_arg(rejected_mask)};
@@ -519,16 +552,16 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
                                double smoothing, int64_t kind, bool normalized) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = op_handle<decltype(op_preference)>("rl_triton::_preference_loss");
-    auto [loss, rewards, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
+    auto [loss, good, bad, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
                                          normalized);
     ctx->save_for_backward({coef, plain(mask_c), plain(mask_r)});
     ctx->saved_data["len"] = chosen.size(1);
     ctx->saved_data["rejected_len"] = rejected ? rejected->size(1) : (int64_t)-1;
     ctx->saved_data["types"] = std::vector<int64_t>{
         (int64_t)chosen.scalar_type(), (int64_t)(rejected ? rejected->scalar_type() : chosen.scalar_type())};
-    ctx->mark_non_differentiable({rewards});
+    ctx->mark_non_differentiable({good, bad});
     ctx->set_materialize_grads(false);
-    return {loss, rewards};
+    return {loss, good, bad};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     static auto op = op_handle<decltype(op_preference_backward)>("rl_triton::_preference_loss_backward");
@@ -545,18 +578,18 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
   }
 };
 
-std::tuple<Tensor, Tensor> preference_loss_autograd(const Tensor& chosen, const OptT& rejected, const OptT& ref_c,
+std::tuple<Tensor, Tensor, Tensor> preference_loss_autograd(const Tensor& chosen, const OptT& rejected, const OptT& ref_c,
                                                     const OptT& ref_r, const OptT& mask_c, const OptT& mask_r,
                                                     double beta, double smoothing, int64_t kind, bool normalized) {
   if (at::GradMode::is_enabled() && (chosen.requires_grad() || (rejected && rejected->requires_grad()))) {
     auto o = PreferenceLoss::apply(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind, normalized);
-    return {o[0], o[1]};
+    return {o[0], o[1], o[2]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = op_handle<decltype(op_preference)>("rl_triton::_preference_loss");
-  auto [loss, rewards, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
+  auto [loss, good, bad, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
                                        normalized);
-  return {loss, rewards};
+  return {loss, good, bad};
 }
 
 }  // namespace
@@ -573,7 +606,7 @@ TORCH_LIBRARY_FRAGMENT(rl_triton, m) {
         "-> (Tensor, Tensor, Tensor, Tensor)");
   m.def("preference_loss(Tensor chosen, Tensor? rejected, Tensor? ref_chosen, Tensor? ref_rejected, "
         "Tensor? chosen_mask, Tensor? rejected_mask, float beta, float smoothing, int kind, bool normalized) "
-        "-> (Tensor, Tensor)");
+        "-> (Tensor, Tensor, Tensor)");
   m.def("_grad_buffer(Tensor logits) -> Tensor");
   m.def("_token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature, bool entropy, bool keep) "
         "-> (Tensor, Tensor, Tensor, Tensor)");
@@ -595,7 +628,7 @@ TORCH_LIBRARY_FRAGMENT(rl_triton, m) {
         "float entropy_coef, float temperature, int reduction, float grad_scale, bool force) -> ()");
   m.def("_preference_loss(Tensor chosen, Tensor? rejected, Tensor? ref_chosen, Tensor? ref_rejected, "
         "Tensor? chosen_mask, Tensor? rejected_mask, float beta, float smoothing, int kind, bool normalized) "
-        "-> (Tensor, Tensor, Tensor)");
+        "-> (Tensor, Tensor, Tensor, Tensor)");
   m.def("_preference_loss_backward(Tensor coef, Tensor grad_loss, Tensor? chosen_mask, Tensor? rejected_mask, "
         "int chosen_len, int rejected_len, bool halves) -> (Tensor, Tensor)");
 }

@@ -220,7 +220,7 @@ def _(grad, *args):
 @torch.library.register_fake("rl_triton::_preference_loss")
 def _(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta, smoothing, kind, normalized):
     b = chosen.shape[0] if rejected is not None else chosen.shape[0] // 2
-    return _f32(chosen), _f32(chosen, 2, b), _f32(chosen, 2, b)
+    return _f32(chosen), _f32(chosen, b), _f32(chosen, b), _f32(chosen, 2, b)
 
 
 @torch.library.register_fake("rl_triton::_preference_loss_backward")
@@ -244,6 +244,7 @@ _SIGS = {
     "rls_workspace_bytes": (_SZ, [_I64]),
     "rls_workspace_error": (_I, [_P, _P]),
     "rls_status_string": (ctypes.c_char_p, [_I]),
+    "rls_assume_device": (_I, [_I]),
     "rls_build_info": (ctypes.c_char_p, []),
     "rls_gae": (_I, [_P, _P, _P, _P, _P, _I, _P, _I64, _I64, _F, _F, _I, _SEG, _P, _SZ, _P]),
     "rls_vtrace": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I64, _I64, _F, _F, _F, _I, _P, _SZ, _P]),
@@ -271,7 +272,7 @@ _SIGS = {
                                     _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _P, _SZ, _P]),
     "rls_policy_loss_logits_backward": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _P, _P, _I, _P, _POL, _F, _P, _I, _P, _P,
                                              _P, _I64, _I64, _I64, _I64, _I64, _D, _I, _P]),
-    "rls_preference_loss": (_I, [_P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _F, _F, _I, _I, _P, _P, _P, _P,
+    "rls_preference_loss": (_I, [_P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _F, _F, _I, _I, _P, _P, _P, _P, _P,
                                  _SZ, _P]),
     "rls_preference_loss_backward": (_I, [_P, _P, _P, _P, _I, _P, _P, _I64, _I64, _I64, _P]),
     "rls_gae_noalloc": (_I, [_P, _P, _P, _P, _P, _I, _P, _I64, _I64, _F, _F, _I, _SEG, _P]),

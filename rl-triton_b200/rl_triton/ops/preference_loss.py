@@ -81,7 +81,7 @@ def compute_preference_loss(
     _placed(first, *(t for s in sides for t in s[1:]))
     _warn_copies({f"{what} of {s[0]}": t for s in sides for what, t in zip(("values", "reference", "mask"), s[1:])})
     lp, ref, m = ([s[k] for s in sides] + [None] * (2 - len(sides)) for k in (1, 2, 3))
-    value, rewards = nat.ops.preference_loss(lp[0], lp[1], ref[0], ref[1], m[0], m[1], float(beta),
-                                             float(label_smoothing), _KINDS[loss], bool(length_normalized))
+    value, good, bad = nat.ops.preference_loss(lp[0], lp[1], ref[0], ref[1], m[0], m[1], float(beta),
+                                               float(label_smoothing), _KINDS[loss], bool(length_normalized))
     _done(first)
-    return value, rewards[0], rewards[1]
+    return value, good, bad
