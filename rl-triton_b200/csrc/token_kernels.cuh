@@ -175,6 +175,8 @@ struct GradRows {
 struct RowStats {
   float m, s0, t;
   bool far, alone;
+  // long rows, near form: the share of S0 and the mean of d of all but the token
+  float others = -1.f, t_others = 0.f;
 };
 
 // A long row's record (RLS_ROW_STATS floats, two 16-byte words): m, S0, t and
@@ -185,7 +187,7 @@ __device__ __forceinline__ float4 stats_word(const RowStats& r, int flags) {
   return make_float4(r.m, r.s0, r.t, __int_as_float(flags | (r.far ? kFlagFar : 0)));
 }
 __device__ __forceinline__ RowStats stats_of(const float4& q) {
-  return RowStats{q.x, q.y, q.z, (__float_as_int(q.w) & kFlagFar) != 0, false};
+  return RowStats{q.x, q.y, q.z, (__float_as_int(q.w) & kFlagFar) != 0, false, -1.f, 0.f};
 }
 
 // d of one element under the row's statistics.
@@ -214,8 +216,21 @@ __device__ __forceinline__ double log2_of(float s0) {
 // the mean of d times the relative error; and ex2.approx lies 5.0e-8 low on
 // average for d below 0 (measured; 3.4e-8 high above), except at the far form's
 // maximum, where d is 0.
+//
+// Where the sum of the others is known apart from the token's term, q =
+// (others / token's) gives logprob = -log(1 + q) with the relative accuracy of
+// q, however close to 0 it is (a sum that the token's term dominates would not).
 __device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c, double c64, double c_off) {
   const Shift sh = shift_of(r, c);
+  if (!r.far && r.others >= 0.f) {
+    const double d = (double)x_tok * (double)c - (double)sh.off;
+    const double l = log2_of(r.others) - d + c_off * ((double)r.t_others - d) + 7.2e-8;  // log2 q
+    if (l > 0.0) return -(l * 0.693147180559945309417 + (double)log1pf(exp2f(-(float)l)));
+    const float lf = (float)l, low = lf > -INFINITY ? (float)(l - (double)lf) : 0.f;
+    float q = exp2f(lf);
+    q = fmaf(q, low * kLn2, q);
+    return q == 0.f ? 0.0 : -(double)log1pf(q);
+  }
   if (ex2(sh(x_tok)) == r.s0) return 0.0;  // the others are below fp32's reach
   const double res = r.far ? 0.0 : (double)r.m * (double)c - (double)sh.off;  // d at the maximum
   const double low = r.far ? 7.2e-8 * (double)(1.f - __frcp_rn(r.s0)) : 7.2e-8;
@@ -272,6 +287,14 @@ struct Vec<float> {
     asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.z) : "r"(u.z), "r"(low));
     asm("max.NaN.f32 %0, %1, %2;" : "=r"(o.w) : "r"(u.w), "r"(low));
     return o;
+  }
+  // The vector with -inf for element e.
+  __device__ __forceinline__ static uint4 without(uint4 u, int e) {
+    if (e == 0) u.x = 0xff800000u;
+    if (e == 1) u.y = 0xff800000u;
+    if (e == 2) u.z = 0xff800000u;
+    if (e == 3) u.w = 0xff800000u;
+    return u;
   }
   __device__ __forceinline__ static float top(const uint4& u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
@@ -331,6 +354,14 @@ struct Vec<__nv_bfloat16> {
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.z) : "r"(u.z), "r"(low));
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o.w) : "r"(u.w), "r"(low));
     return o;
+  }
+  __device__ __forceinline__ static uint4 without(uint4 u, int e) {
+    const unsigned keep = e & 1 ? 0x0000ffffu : 0xffff0000u, low = e & 1 ? 0xff800000u : 0x0000ff80u;
+    if (e >> 1 == 0) u.x = (u.x & keep) | low;
+    if (e >> 1 == 1) u.y = (u.y & keep) | low;
+    if (e >> 1 == 2) u.z = (u.z & keep) | low;
+    if (e >> 1 == 3) u.w = (u.w & keep) | low;
+    return u;
   }
   __device__ __forceinline__ static float top(const uint4& u) {
     const unsigned m = max2(max2(u.x, u.y), max2(u.z, u.w));
@@ -416,9 +447,10 @@ struct Run {
     s0 += e[0];
     if constexpr (!ENT) s1 = fmaf(e[0], fmaxf(fmaf(mx, c, -off), kDeep), s1);
   }
-  // M whole vectors at once.
-  template <class T, int M>
-  __device__ __forceinline__ void add_vectors(uint4 (&u)[M], float c) {
+  // M whole vectors at once; `at` places NT apart is where the token lies from the
+  // first of them (anything else: not among them), `e` its element, left out.
+  template <class T, int M, int NT>
+  __device__ __forceinline__ void add_vectors(uint4 (&u)[M], float c, int at, int e) {
     constexpr int P = Vec<T>::N / 2;
     if constexpr (ENT) {
 #pragma unroll
@@ -428,8 +460,14 @@ struct Run {
 #pragma unroll
     for (int k = 1; k < M; ++k) mx = fmaxf(mx, Vec<T>::top(u[k]));
     float dm = fmaf(mx, c, -off);
-    if (dm > kSlack - kLift) {
-      raise(mx, c);
+    if (dm > kSlack - kLift || (unsigned)at <= (unsigned)((M - 1) * NT)) {  // one branch for the two
+#pragma unroll
+      for (int k = 0; k < M; ++k)
+        if (at == k * NT) u[k] = ENT ? Vec<T>::bound(Vec<T>::without(u[k], e)) : Vec<T>::without(u[k], e);
+      mx = Vec<T>::top(u[0]);
+#pragma unroll
+      for (int k = 1; k < M; ++k) mx = fmaxf(mx, Vec<T>::top(u[k]));
+      if (fmaf(mx, c, -off) > kSlack - kLift) raise(mx, c);
       dm = fmaf(mx, c, -off);
     }
     const F2 cc = f2(c, c), no = f2(-off, -off);
@@ -930,7 +968,7 @@ constexpr int kMostCtas = 8;  // of a cluster (the portable limit)
 //
 // Across CTAs there are two ways.  A cluster barrier with release and acquire
 // waits for all of the thread's earlier stores, gradients on their way to memory among
-// them (measured at 131072 bf16 logits: 462 us with it, KASYNC us without, for 4081 rows of
+// them (measured at 131072 bf16 logits: 462 us with it, 432 us without, for 4081 rows of
 // loss and gradient); so where there are such stores the values travel as
 // asynchronous stores that count down an mbarrier of the CTA they go to.
 template <int NT, bool CL, bool ASYNC>
@@ -1194,8 +1232,20 @@ struct Walk {
   // Elements outside the row's vectors: the first CTA's threads take one each.
   __device__ __forceinline__ int ends_of(const Cut& cut) const { return rank == 0 ? (int)(cut.head + cut.tail) : 0; }
 
-  // The statistics of the row from every thread's share (the vectors; the ends
-  // are added here); the same in all threads of the team.
+  // How far the token's vector lies from the thread's first, and the element there; the
+  // thread has it where that is a multiple of NT.  Far below 0: not in the stretch.
+  __device__ __forceinline__ int token_vector(int64_t row, const Extra& ex, int& e) const {
+    const Cut cut = cut_row(row_at(row), in.V);
+    int v0;
+    const int n = stretch(cut, v0);
+    const int rel = (int)ex.tok - cut.head - v0 * N;
+    e = rel & (N - 1);
+    return ex.tok >= 0 && ex.tok < in.V && rel >= 0 && rel < n * N ? rel / N - tid : -(1 << 30);
+  }
+
+  // The statistics of the row from every thread's share of the vectors, the token
+  // left out (the ends are added here, and the token last); the same in all
+  // threads of the team.
   template <bool ASYNC>
   __device__ __forceinline__ RowStats join(Run<ENT>& run, int64_t row, const Extra& ex, Table<NT, CL, ASYNC>& table,
                                            Turns& turn) const {
@@ -1204,7 +1254,7 @@ struct Walk {
     const T* x = row_at(row);
     const Cut cut = cut_row(x, in.V);
     const int ends = ends_of(cut);
-    if (tid < ends) {
+    if (tid < ends && ex.tok != (tid < cut.head ? tid : in.V - ends + tid)) {
       const float f[1] = {ex.end};
       run.add(f, c);
     }
@@ -1233,10 +1283,17 @@ struct Walk {
         gather<32>(run.m, run.s0, run.s1, c);
       }
     }
-    if (run.s0 >= kLeast && run.s0 <= kMost) {
-      const float off = offset_of(run.m, c), dm = fmaf(run.m, c, -off), em = ex2(dm);
-      const bool alone = ENT && run.s0 == em && run.s1 == em * dm;
-      return RowStats{run.m, run.s0, alone ? dm : run.s1 / run.s0, false, alone};
+    {
+      const float others = run.s0, by_others = run.s1;
+      run.off = offset_of(run.m, c);
+      if (ex.xt > run.m) run.raise(ex.xt, c);
+      const float d = fmaf(ex.xt, c, -run.off), e = ex2(d);
+      const float s0 = run.s0 + e, s1 = fmaf(e, fmaxf(d, kDeep), run.s1);
+      if (s0 >= kLeast && s0 <= kMost) {
+        const bool alone = ENT && others == 0.f && by_others == 0.f;
+        return RowStats{run.m, s0, alone ? d : s1 / s0, false, alone, run.s0,
+                        run.s0 > 0.f ? __fdividef(run.s1, run.s0) : 0.f};
+      }
     }
     // The far form, from global memory (what the row was read into may hold the
     // next one).  All threads of the team come here or none.
@@ -1266,7 +1323,7 @@ struct Walk {
     tab = exchange(table, turn, make_float4(s0, s1, 0.f, 0.f), rank, size);
     s0 = s1 = 0.f;
     for (int w = 0; w < (int)size * (NT / 32); ++w) { s0 += tab[w].x; s1 += tab[w].y; }
-    return RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f};
+    return RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f, -1.f, 0.f};
   }
 
   // What a row gives besides its gradient; one warp of a CTA calls these.  The
@@ -1425,7 +1482,9 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
       nx = walk.extra(row);
     }
     Run<ENT> run(in.c);
-    typename W::Writer wr;
+    int token_e = 0;
+    const int token_v = MODE == kFwd ? walk.token_vector(now.row, ex, token_e) : 0;
+    typename W::Writer wr{};
     float a = 0.f, b = 0.f;
     if constexpr (MODE == kBwd) {
       a = ex.a;
@@ -1447,7 +1506,7 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
           uint4 t[M];
 #pragma unroll
           for (int k = 0; k < M; ++k) t[k] = u[j + k];
-          run.template add_vectors<T, M>(t, in.c);
+          run.template add_vectors<T, M, NT>(t, in.c, token_v - (base + j * NT), token_e);
         } else if (near) {
 #pragma unroll
           for (int k = 0; k < M; ++k) {
@@ -1510,6 +1569,8 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
   }
   for (;;) {
     Run<ENT> run(in.c);
+    int token_e = 0;
+    const int token_v = walk.token_vector(now.row, ex, token_e);
 #pragma unroll
     for (int j = 0; j < K; j += M) {
       copy_wait_upto<K - M>(K - M - j);
@@ -1519,7 +1580,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
         u[k] = make_uint4(low, low, low, low);
         if ((j + k) * NT < now.mid) u[k] = mine[(j + k) * NT];
       }
-      run.template add_vectors<T, M>(u, in.c);
+      run.template add_vectors<T, M, NT>(u, in.c, token_v - j * NT, token_e);
     }
     const RowStats r = walk.join(run, now.row, ex, table, turn);
     typename W::Result q;
