@@ -16,6 +16,8 @@
 // gets a buffer of its own.
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/record_function.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -105,20 +107,17 @@ Tensor tokens_arg(const Tensor& t) {
 
 // The buffer of a logits gradient.  It takes the logits' own strides where they
 // leave no more than a quarter of the buffer unused (a slice of the steps, a
-// vocabulary cut from a padded one), and starts at the same place within 16
-// bytes: every row then has the alignment of its logits, which the kernels need
-// for 16-byte stores.
+// vocabulary cut from a padded one): if the logits start on a 16-byte boundary too, every
+// row then has the alignment of its logits, which the kernels need for 16-byte stores.
 Tensor op_grad_buffer(const Tensor& logits) {
   const int64_t n = logits.size(0), t = logits.size(1), v = logits.size(2);
-  const int64_t e = logits.element_size();
   const int64_t es = logits.stride(0), ss = logits.stride(1);
   if (logits.numel() == 0 || (v > 1 && logits.stride(2) != 1)) return at::empty(logits.sizes(), logits.options());
   const bool apart = (t == 1 || ss >= v) && (n == 1 || es >= (t - 1) * ss + v);
   const int64_t span = (n - 1) * es + (t - 1) * ss + v;
-  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16) / e;
-  if (!apart || span > n * t * v + n * t * v / 4 || (off == 0 && logits.is_contiguous()))
+  if (!apart || span > n * t * v + n * t * v / 4 || logits.is_contiguous())
     return at::empty(logits.sizes(), logits.options());
-  return at::empty({span + off}, logits.options()).as_strided(logits.sizes(), logits.strides(), off);
+  return at::empty_strided(logits.sizes(), logits.strides(), logits.options());
 }
 
 struct LogitsArgs {
@@ -382,9 +381,37 @@ std::tuple<Tensor, Tensor> op_preference_backward(const Tensor& coef, const Tens
 }
 
 // ---- autograd ------------------------------------------------------------------------
+// Calls an operator of this file through the dispatcher where something has to see
+// the call (fake or functional tensors, a dispatch mode, a profiler), straight otherwise.
 template <class Sig>
-auto op_handle(const char* name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+struct Inner;
+template <class R, class... A>
+struct Inner<R(A...)> {
+  c10::TypedOperatorHandle<R(A...)> handle;
+  R (*kernel)(A...);
+  template <class... B>
+  R call(const Tensor& first, B&&... rest) const {
+    const bool seen =
+        first.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize})) ||
+        !first.is_cuda() || c10::impl::TorchDispatchModeTLS::any_modes_set() || at::hasCallbacks() ||
+        // a backward call that is itself to be differentiated: the dispatcher's fallback refuses
+        (at::GradMode::is_enabled() && !c10::impl::tls_is_dispatch_key_excluded(c10::DispatchKey::AutogradCUDA));
+    return seen ? through(first, std::forward<B>(rest)...) : straight(first, std::forward<B>(rest)...);
+  }
+
+ private:
+  template <class... B>
+  R through(const Tensor& first, B&&... rest) const {
+    return handle.call(const_cast<Tensor&>(first), std::forward<B>(rest)...);
+  }
+  template <class... B>
+  R straight(const Tensor& first, B&&... rest) const {
+    return kernel(const_cast<Tensor&>(first), std::forward<B>(rest)...);
+  }
+};
+template <class R, class... A>
+Inner<R(A...)> inner(const char* name, R (*kernel)(A...)) {
+  return {c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<R(A...)>(), kernel};
 }
 
 // What a policy loss keeps for its backward call besides tensors: the
@@ -405,7 +432,7 @@ Kept& kept_of(AutogradContext* ctx) {
 }
 
 Tensor call_grad_buffer(const Tensor& logits) {
-  static auto op = op_handle<Tensor(const Tensor&)>("rl_triton::_grad_buffer");
+  static auto op = inner("rl_triton::_grad_buffer", &op_grad_buffer);
   return op.call(logits);
 }
 
@@ -413,7 +440,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const OptT& mask,
                                double temperature, bool entropy) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = op_handle<decltype(op_logprobs)>("rl_triton::_token_logprobs");
+    static auto op = inner("rl_triton::_token_logprobs", &op_logprobs);
     auto [lp, ent, stats, order] = op.call(logits, tokens, mask, temperature, entropy, true);
     ctx->save_for_backward({logits, tokens, plain(mask), order, stats});
     ctx->saved_data["temperature"] = temperature;
@@ -422,7 +449,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
     return {lp, ent};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    static auto op = op_handle<decltype(op_logprobs_backward)>("rl_triton::_token_logprobs_backward");
+    static auto op = inner("rl_triton::_token_logprobs_backward", &op_logprobs_backward);
     const auto s = ctx->get_saved_variables();
     Tensor out;
     if (g[0].defined() || g[1].defined())
@@ -438,7 +465,7 @@ std::tuple<Tensor, Tensor> token_logprobs_autograd(const Tensor& logits, const T
     return {o[0], o[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  static auto op = op_handle<decltype(op_logprobs)>("rl_triton::_token_logprobs");
+  static auto op = inner("rl_triton::_token_logprobs", &op_logprobs);
   auto [lp, ent, stats, order] = op.call(logits, tokens, mask, temperature, entropy, false);
   return {lp, ent};
 }
@@ -448,7 +475,7 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
                                const OptT& mask, const OptT& ref, double clip_low, double clip_high, double dual_clip,
                                double kl_coef, int64_t kl, int64_t reduction, double grad_scale, bool need_stats) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = op_handle<decltype(op_policy)>("rl_triton::_policy_loss");
+    static auto op = inner("rl_triton::_policy_loss", &op_policy);
     auto [loss, stats, norm, grad] = op.call(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl,
                                              reduction, grad_scale, need_stats, true);
     ctx->save_for_backward({lp, old_lp, adv, plain(mask), plain(ref), norm});
@@ -462,7 +489,7 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
     return {loss, stats};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    static auto op = op_handle<decltype(op_policy_backward_)>("rl_triton::_policy_loss_backward_");
+    static auto op = inner("rl_triton::_policy_loss_backward_", &op_policy_backward_);
     if (!g[0].defined()) return variable_list(13);
     const auto s = ctx->get_saved_variables();
     Kept& k = kept_of(ctx);
@@ -487,7 +514,7 @@ std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& lp, const Tensor& 
     return {o[0], o[1]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  static auto op = op_handle<decltype(op_policy)>("rl_triton::_policy_loss");
+  static auto op = inner("rl_triton::_policy_loss", &op_policy);
   auto [loss, stats, norm, grad] = op.call(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl,
                                            reduction, grad_scale, need_stats, false);
   return {loss, stats};
@@ -499,7 +526,7 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
                                double dual_clip, double kl_coef, int64_t kl, double entropy_coef, bool need_stats,
                                double temperature, int64_t reduction, double grad_scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = op_handle<decltype(op_policy_logits)>("rl_triton::_policy_loss_logits");
+    static auto op = inner("rl_triton::_policy_loss_logits", &op_policy_logits);
     auto [loss, lp, ent, stats, norm, order, rows, grad] =
         op.call(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef,
                 need_stats, temperature, reduction, grad_scale, true);
@@ -515,7 +542,7 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
     return {loss, lp, ent, stats};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    static auto op = op_handle<decltype(op_policy_logits_backward_)>("rl_triton::_policy_loss_logits_backward_");
+    static auto op = inner("rl_triton::_policy_loss_logits_backward_", &op_policy_logits_backward_);
     if (!g[0].defined()) return variable_list(16);
     const auto s = ctx->get_saved_variables();
     Kept& k = kept_of(ctx);
@@ -540,7 +567,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss_logits_autograd(
     return {o[0], o[1], o[2], o[3]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  static auto op = op_handle<decltype(op_policy_logits)>("rl_triton::_policy_loss_logits");
+  static auto op = inner("rl_triton::_policy_loss_logits", &op_policy_logits);
   auto r = op.call(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef,
                    need_stats, temperature, reduction, grad_scale, false);
   return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r)};
@@ -551,7 +578,7 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
                                const OptT& ref_r, const OptT& mask_c, const OptT& mask_r, double beta,
                                double smoothing, int64_t kind, bool normalized) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = op_handle<decltype(op_preference)>("rl_triton::_preference_loss");
+    static auto op = inner("rl_triton::_preference_loss", &op_preference);
     auto [loss, good, bad, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
                                          normalized);
     ctx->save_for_backward({coef, plain(mask_c), plain(mask_r)});
@@ -564,7 +591,7 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
     return {loss, good, bad};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    static auto op = op_handle<decltype(op_preference_backward)>("rl_triton::_preference_loss_backward");
+    static auto op = inner("rl_triton::_preference_loss_backward", &op_preference_backward);
     if (!g[0].defined()) return variable_list(10);
     const auto s = ctx->get_saved_variables();
     const int64_t other = ctx->saved_data["rejected_len"].toInt();
@@ -586,7 +613,7 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss_autograd(const Tensor& chosen
     return {o[0], o[1], o[2]};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  static auto op = op_handle<decltype(op_preference)>("rl_triton::_preference_loss");
+  static auto op = inner("rl_triton::_preference_loss", &op_preference);
   auto [loss, good, bad, coef] = op.call(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind,
                                        normalized);
   return {loss, good, bad};

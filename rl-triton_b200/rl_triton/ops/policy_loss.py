@@ -6,8 +6,12 @@ from __future__ import annotations
 import torch
 
 from rl_triton import _native as nat
-from rl_triton.ops._scan import _done, _float_ok, _placed, _warn_copies
-from rl_triton.ops.token_logprobs import _logits_args, _mask_arg
+from rl_triton.ops import _scan
+from rl_triton.ops._scan import _CORRECTNESS_WARNINGS, _float_ok, _placed, _warn_copies
+from rl_triton.ops.token_logprobs import _finished, _logits_args, _mask_arg
+
+_op = nat.ops.policy_loss.default
+_op_logits = nat.ops.policy_loss_logits.default
 
 _REDUCTIONS = {"token": nat.REDUCE_TOKEN, "sequence": nat.REDUCE_SEQUENCE, "sum": nat.REDUCE_SUM}
 _KL = {"k1": nat.KL_K1, "k2": nat.KL_K2, "k3": nat.KL_K3}
@@ -68,11 +72,12 @@ def compute_policy_loss(
     c = _policy_args(logprobs.shape, old_logprobs, advantages, mask, ref_logprobs, clip_low, clip_high, dual_clip,
                      kl_coef, kl, reduction)
     _placed(logprobs, old_logprobs, advantages, mask, ref_logprobs)
-    _warn_copies({"logprobs": logprobs, "old_logprobs": old_logprobs, "advantages": advantages, "mask": mask,
-                  "ref_logprobs": ref_logprobs})
-    loss, stats = nat.ops.policy_loss(logprobs, old_logprobs, advantages, mask, ref_logprobs, *c, float(grad_scale),
-                                      bool(return_stats))
-    _done(logprobs)
+    if _scan._PERF_WARNINGS:
+        _warn_copies({"logprobs": logprobs, "old_logprobs": old_logprobs, "advantages": advantages, "mask": mask,
+                      "ref_logprobs": ref_logprobs})
+    loss, stats = _op(logprobs, old_logprobs, advantages, mask, ref_logprobs, *c, grad_scale, return_stats)
+    if _CORRECTNESS_WARNINGS():
+        _finished(logprobs)
     return (loss, _stats(stats, False)) if return_stats else loss
 
 
@@ -111,16 +116,18 @@ def compute_policy_loss_from_logits(
         gradient, or (loss, logprobs, stats) when return_stats is True; stats
         then also holds "entropy".
     """
-    _logits_args(logits, tokens, mask, temperature)
+    checks = _CORRECTNESS_WARNINGS()
+    _logits_args(logits, tokens, mask, temperature, checks)
     c = _policy_args(logits.shape[:2], old_logprobs, advantages, None, ref_logprobs, clip_low, clip_high, dual_clip,
                      kl_coef, kl, reduction)
     _placed(logits, tokens, old_logprobs, advantages, mask, ref_logprobs)
-    _warn_copies({"old_logprobs": old_logprobs, "advantages": advantages, "mask": mask,
-                  "ref_logprobs": ref_logprobs})
-    loss, lp, _, stats = nat.ops.policy_loss_logits(
-        logits, tokens, old_logprobs, advantages, mask, ref_logprobs, *c[:5], float(entropy_coef),
-        bool(return_stats), float(temperature), c[5], float(grad_scale))
-    _done(logits)
+    if _scan._PERF_WARNINGS:
+        _warn_copies({"old_logprobs": old_logprobs, "advantages": advantages, "mask": mask,
+                      "ref_logprobs": ref_logprobs})
+    loss, lp, _, stats = _op_logits(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, *c[:5], entropy_coef,
+                                    return_stats, temperature, c[5], grad_scale)
+    if checks:
+        _finished(logits)
     return (loss, lp, _stats(stats, True)) if return_stats else (loss, lp)
 
 
@@ -128,7 +135,7 @@ def _policy_args(shape, old_logprobs, advantages, mask, ref_logprobs, clip_low, 
                  reduction):
     """Checks; (clip_low, clip_high, dual_clip, kl_coef, kl, reduction) as the
     operators take them."""
-    for name, t in [("old_logprobs", old_logprobs), ("ref_logprobs", ref_logprobs)]:
+    for name, t in (("old_logprobs", old_logprobs), ("ref_logprobs", ref_logprobs)):
         if t is not None:
             assert _float_ok(t), f"{name}: expected float32 or bfloat16, got {t.dtype}"
             assert t.shape == shape, f"{name} shape {t.shape} != {shape}"
@@ -142,7 +149,7 @@ def _policy_args(shape, old_logprobs, advantages, mask, ref_logprobs, clip_low, 
     high = clip_low if clip_high is None else clip_high
     assert clip_low >= 0.0 and high >= 0.0, f"clip bounds must not be negative, got {clip_low}, {high}"
     assert dual_clip is None or dual_clip > 1.0, f"dual_clip must be greater than 1, got {dual_clip}"
-    return (float(clip_low), float(high), float(dual_clip or 0.0), float(kl_coef), _KL[kl], _REDUCTIONS[reduction])
+    return clip_low, high, dual_clip or 0.0, kl_coef, _KL[kl], _REDUCTIONS[reduction]
 
 
 def _stats(stats, entropy):

@@ -5,8 +5,11 @@ from __future__ import annotations
 import torch
 
 from rl_triton import _native as nat
-from rl_triton.ops._scan import _done, _float_ok, _placed, _warn_copies
-from rl_triton.ops.token_logprobs import _mask_arg
+from rl_triton.ops import _scan
+from rl_triton.ops._scan import _CORRECTNESS_WARNINGS, _float_ok, _placed, _warn_copies
+from rl_triton.ops.token_logprobs import _finished, _mask_arg
+
+_op = nat.ops.preference_loss.default
 
 _KINDS = {"sigmoid": nat.PREFERENCE_SIGMOID, "ipo": nat.PREFERENCE_IPO, "hinge": nat.PREFERENCE_HINGE}
 
@@ -79,9 +82,11 @@ def compute_preference_loss(
     if len(sides) == 2 and sides[0][2] is not None:
         assert sides[0][2].dim() == sides[1][2].dim(), "ref_logprobs: per step or per response, alike for both"
     _placed(first, *(t for s in sides for t in s[1:]))
-    _warn_copies({f"{what} of {s[0]}": t for s in sides for what, t in zip(("values", "reference", "mask"), s[1:])})
-    lp, ref, m = ([s[k] for s in sides] + [None] * (2 - len(sides)) for k in (1, 2, 3))
-    value, good, bad = nat.ops.preference_loss(lp[0], lp[1], ref[0], ref[1], m[0], m[1], float(beta),
-                                               float(label_smoothing), _KINDS[loss], bool(length_normalized))
-    _done(first)
+    if _scan._PERF_WARNINGS:
+        _warn_copies({f"{what} of {s[0]}": t for s in sides for what, t in zip(("values", "reference", "mask"), s[1:])})
+    lp, ref, m = sides[0][1:]
+    lp2, ref2, m2 = sides[1][1:] if len(sides) == 2 else (None, None, None)
+    value, good, bad = _op(lp, lp2, ref, ref2, m, m2, beta, label_smoothing, _KINDS[loss], length_normalized)
+    if _CORRECTNESS_WARNINGS():
+        _finished(first)
     return value, good, bad

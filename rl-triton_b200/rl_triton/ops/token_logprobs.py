@@ -7,7 +7,9 @@ from __future__ import annotations
 import torch
 
 from rl_triton import _native as nat
-from rl_triton.ops._scan import _CORRECTNESS_WARNINGS, _done, _float_ok, _perf_warn, _placed
+from rl_triton.ops._scan import _CORRECTNESS_WARNINGS, _float_ok, _perf_warn, _placed
+
+_op = nat.ops.token_logprobs.default
 
 
 def compute_token_logprobs(
@@ -44,29 +46,42 @@ def compute_token_logprobs(
         logprobs [num_envs, seq_len] float32, or (logprobs, entropy) when
         return_entropy is True.
     """
-    _logits_args(logits, tokens, mask, temperature)
+    checks = _CORRECTNESS_WARNINGS()
+    _logits_args(logits, tokens, mask, temperature, checks)
     _placed(logits, tokens, mask)
-    lp, ent = nat.ops.token_logprobs(logits, tokens, mask, float(temperature), bool(return_entropy))
-    _done(logits)
+    lp, ent = _op(logits, tokens, mask, temperature, return_entropy)
+    if checks:
+        _finished(logits)
     return (lp, ent) if return_entropy else lp
 
 
-def _logits_args(logits, tokens, mask, temperature):
+def _logits_args(logits, tokens, mask, temperature, checks):
     assert logits.is_cuda, "logits must be on CUDA"
-    assert logits.dim() == 3, f"logits must have shape [num_envs, seq_len, vocab], got {logits.shape}"
+    shape = logits.shape
+    assert len(shape) == 3, f"logits must have shape [num_envs, seq_len, vocab], got {shape}"
     assert _float_ok(logits), f"logits: expected float32 or bfloat16, got {logits.dtype}"
-    assert logits.shape[2] > 0, "logits: the vocabulary is empty"
-    assert tokens.shape == logits.shape[:2], f"tokens shape {tokens.shape} != {logits.shape[:2]} of the logits"
-    assert not tokens.is_floating_point() and not tokens.is_complex() and tokens.dtype != torch.bool, \
-        f"tokens: expected integers, got {tokens.dtype}"
+    assert shape[2] > 0, "logits: the vocabulary is empty"
+    steps = shape[:2]
+    assert tokens.shape == steps, f"tokens shape {tokens.shape} != {steps} of the logits"
+    assert tokens.dtype in _INTEGERS, f"tokens: expected integers, got {tokens.dtype}"
     assert 0.0 < temperature < float("inf"), f"temperature must be positive and finite, got {temperature}"
-    _mask_arg(mask, logits.shape[:2])
-    if logits.shape[2] > 1 and logits.stride(2) != 1:
+    _mask_arg(mask, steps)
+    if shape[2] > 1 and logits.stride(2) != 1:
         _perf_warn("logits: the vocabulary is not contiguous; a copy will be made.")
-    if _CORRECTNESS_WARNINGS() and not torch.cuda.is_current_stream_capturing():
-        bad = (tokens < 0) | (tokens >= logits.shape[2])
+    if checks and not torch.cuda.is_current_stream_capturing():
+        bad = (tokens < 0) | (tokens >= shape[2])
         assert not (bad if mask is None else bad & (mask != 0)).any(), \
             "tokens: a step that counts has a token outside the vocabulary"
+
+
+_INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
+
+
+def _finished(ref):
+    """RL_TRITON_CORRECTNESS_WARNINGS=1: wait for the call and raise if one of
+    its bounded device waits ran out."""
+    if not torch.cuda.is_current_stream_capturing():
+        nat.raise_if_device_error(ref.device)
 
 
 def _mask_arg(mask, shape, name="mask"):

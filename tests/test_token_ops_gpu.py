@@ -629,3 +629,146 @@ def test_graph_capture_of_a_training_step(monkeypatch):
     torch.cuda.synchronize()
     for p, q in zip(want, out):
         torch.testing.assert_close(p, q.detach())
+
+
+@pytest.mark.parametrize("v", [1500, 40000, 131072])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_likely_tokens_keep_their_relative_accuracy(v, dtype):
+    """A token with nearly all of the probability: the log-probability's error
+    is that of the sum of the others, S(V), relative to the log-probability
+    itself (rows of more than 1024 logits)."""
+    _cuda()
+    import rl_triton
+    x = torch.randn(1, 24, v, generator=torch.Generator().manual_seed(v)).to(dtype)
+    tok = torch.arange(24)[None] * 37 % v
+    top = (math.log(v) + torch.arange(24) * 0.75)[None, :, None].to(dtype)
+    x.scatter_(2, tok[..., None], top)
+    lp = rl_triton.compute_token_logprobs(x.cuda(), tok.cuda())
+    want, _ = ref64.logprobs(x.double(), tok)
+    assert float(want.max()) > -1e-5
+    torch.testing.assert_close(lp.cpu().double(), want, rtol=2 * S(v), atol=0.0)
+
+
+def test_refusals():
+    _cuda()
+    import rl_triton as rl
+    x, lp = torch.zeros(2, 3, 5).cuda(), torch.zeros(2, 3).cuda()
+    tok = torch.zeros(2, 3, dtype=torch.long).cuda()
+
+    def refuses(match, fn, *args, **kw):
+        with pytest.raises(AssertionError, match=match):
+            fn(*args, **kw)
+
+    refuses("num_envs, seq_len, vocab", rl.compute_token_logprobs, x[0], tok[0])
+    refuses("float32 or bfloat16", rl.compute_token_logprobs, x.half(), tok)
+    refuses("tokens shape", rl.compute_token_logprobs, x, tok[:, :2])
+    refuses("expected integers", rl.compute_token_logprobs, x, lp)
+    refuses("mask shape", rl.compute_token_logprobs, x, tok, lp[:1])
+    refuses("vocabulary is empty", rl.compute_token_logprobs, x[..., :0], tok)
+    for bad in (0.0, -1.0, float("inf"), float("nan")):
+        refuses("temperature", rl.compute_token_logprobs, x, tok, None, bad)
+    refuses("must be on cuda", rl.compute_token_logprobs, x, tok.cpu())
+    refuses("old_logprobs shape", rl.compute_policy_loss, lp, lp[:1], lp)
+    refuses("advantages shape", rl.compute_policy_loss, lp, lp, lp[:, :2])
+    refuses("needs ref_logprobs", rl.compute_policy_loss, lp, lp, lp, kl_coef=0.1)
+    refuses("kl must be", rl.compute_policy_loss, lp, lp, lp, kl="k4")
+    refuses("reduction must be", rl.compute_policy_loss, lp, lp, lp, reduction="mean")
+    refuses("dual_clip", rl.compute_policy_loss, lp, lp, lp, dual_clip=1.0)
+    refuses("negative", rl.compute_policy_loss, lp, lp, lp, clip_low=-0.1)
+    refuses("must be on cuda", rl.compute_policy_loss, lp, lp.cpu(), lp)
+    refuses("mask shape", rl.compute_policy_loss_from_logits, x, tok, lp, lp, lp[:1])
+    refuses("2 \\* pairs", rl.compute_preference_loss, lp[:1])
+    refuses("loss must be", rl.compute_preference_loss, lp, loss="dpo")
+    refuses("label_smoothing", rl.compute_preference_loss, lp, label_smoothing=0.5)
+    refuses("belongs to the sigmoid", rl.compute_preference_loss, lp, loss="ipo", label_smoothing=0.1)
+    refuses("beta", rl.compute_preference_loss, lp, beta=0.0)
+    refuses("neither", rl.compute_preference_loss, lp, lp[:, :2])
+    refuses("both or none", rl.compute_preference_loss, (lp, lp), (lp, None))
+    refuses("alike for both", rl.compute_preference_loss, (lp, lp), (lp, lp[:, 0]))
+    refuses("pairs, len", rl.compute_preference_loss, (lp, lp[:1]))
+    with pytest.raises(RuntimeError, match="must be on"):  # the operator itself, without the function's checks
+        torch.ops.rl_triton._token_logprobs(x, tok.cpu(), None, 1.0, False, False)
+
+
+def test_operator_schemas_and_fake_kernels(monkeypatch):
+    """torch.library.opcheck: schema and fake kernel consistency."""
+    _cuda()
+    monkeypatch.setenv("RL_TRITON_CORRECTNESS_WARNINGS", "0")
+    ops = torch.ops.rl_triton
+    for v in (9, 1100):
+        x, tok, mask, _ = make(3, 4, v, seed=v)
+        x, tok, mask = x.cuda(), tok.cuda(), mask.cuda()
+        lp, old, refl, adv, _ = (a.cuda() for a in _policy_inputs(3, 4, 1, False))
+        out = ops._token_logprobs(x, tok, mask, 1.0, True, True)
+        checks = [
+            (ops._grad_buffer, (x[:, 1:],)),
+            (ops._token_logprobs, (x, tok, mask, 1.0, True, True)),
+            (ops._token_logprobs_backward, (x, tok, mask, out[3], out[2], lp, lp, 1.0)),
+            (ops._policy_loss, (lp, old, adv, mask, refl, 0.2, 0.2, 0.0, 0.1, 3, 1, 1.0, True, True)),
+            (ops._policy_loss_logits, (x, tok, old, adv, mask, refl, 0.2, 0.2, 0.0, 0.1, 3, 0.01, True, 1.0, 0, 1.0,
+                                       True)),
+            (ops._preference_loss, (lp[:2], None, refl[:2], None, mask[:2], None, 0.1, 0.0, 0, False)),
+            (ops._preference_loss_backward, (torch.ones(2, 3).cuda(), torch.ones(()).cuda(), None, None, 4, 5, False)),
+        ]
+        for op, args in checks:
+            torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("n,t", [(1, 1), (3, 7), (40, 33), (1, 70001), (3000, 3)])
+def test_row_order(n, t):
+    """A permutation of the steps, those that count first."""
+    _cuda()
+    from rl_triton import _native as nat
+    mask = (torch.rand(n, t, generator=torch.Generator().manual_seed(n)) < 0.5).cuda()
+    order = torch.empty(n * t + 1, dtype=torch.int32, device="cuda")
+    ws, wsb = nat.workspace(mask.device, nat.stream_handle(mask.device), 1 << 20)
+    st = nat.lib.rls_row_order(mask.data_ptr(), nat.MASK_U8, n, t, order.data_ptr(), ws, wsb,
+                               nat.stream_handle(mask.device))
+    assert st == nat.RLS_OK
+    o = order.cpu().long()
+    k = int(mask.sum())
+    flat = mask.flatten().cpu()
+    assert int(o[0]) == k
+    assert torch.equal(torch.sort(o[1:]).values, torch.arange(n * t))
+    assert flat[o[1:1 + k]].all() and not flat[o[1 + k:]].any()
+
+
+@pytest.mark.parametrize("reduction", ["token", "sequence", "sum"])
+def test_long_rows_behind_a_ragged_mask(reduction):
+    """Many rows, most of them masked, so that every team has skipped rows."""
+    _cuda()
+    import rl_triton
+    n, t, v = 40, 50, 1200
+    x, tok, _, g = make(n, t, v, torch.bfloat16, seed=17)
+    mask = (torch.arange(t)[None] >= torch.randint(0, 10, (n, 1), generator=g)) & \
+        (torch.arange(t)[None] < torch.randint(5, t, (n, 1), generator=g))
+    mask[::4] = False
+    x[~mask] = float("nan")
+    xd = torch.where(mask[..., None], x, torch.zeros_like(x)).double().requires_grad_(True)
+    lp64, h64 = ref64.logprobs(xd, tok, mask)
+    old = (lp64 + 0.1 * torch.randn(n, t, generator=g)).detach().float()
+    adv = torch.randn(n, generator=g)
+    want, _ = ref64.policy(lp64, old.double(), adv.double(), mask, entropy=h64, entropy_coef=0.01, reduction=reduction)
+    (wg,) = torch.autograd.grad(want, xd)
+    xc = x.cuda().requires_grad_(True)
+    loss, lp = rl_triton.compute_policy_loss_from_logits(xc, tok.cuda(), old.cuda(), adv.cuda(), mask.cuda(),
+                                                         entropy_coef=0.01, reduction=reduction)
+    (got,) = torch.autograd.grad(loss, xc)
+    many = int(mask.sum()) if reduction == "sum" else 1
+    close(lp, lp64, **tol_lp(v))
+    close(loss, want, rtol=2 * U, atol=many * 12 * (S(v) + 8 * U + 0.01 * tol_ent(v)["atol"]))
+    close(got, wg, **tol_grad(v, 4 * float(wg.abs().max()), True))
+    assert (got[~mask.cuda()] == 0).all()
+
+
+def test_example_runs():
+    _cuda()
+    import importlib.util
+    import os
+    at = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "token_policy_update.py")
+    spec = importlib.util.spec_from_file_location("token_policy_update", at)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    h = m.main(steps=12, envs=32, length=16, vocab=1200, out=lambda s: None)
+    assert all(math.isfinite(v) for d in h for v in d.values())
+    assert h[-1]["reward"] > h[0]["reward"] + 0.2  # the policy learns the task
