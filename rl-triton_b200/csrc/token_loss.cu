@@ -36,7 +36,8 @@ int num_sms() {
 // norm (may be null): norm[1 + n] = steps of env n that count; norm[0] = 1 / (all of
 // them), or 1 / (envs that have any) for the mean by sequence.  order (may be null):
 // order[0] = all of them, order[1 ..] = those rows, then the others; which row comes
-// where depends on timing, nothing that a row gives does.  Counts are whole numbers: their
+// where depends on timing, nothing that a row gives does.  A CTA an env, or a warp where there are
+// many (4096 x 2048 bytes: 9 us; an order of 16 x 512: 5 us, all latency).  Counts are whole numbers: their
 // atomics give the same sum in any order.
 struct CountWords {
   unsigned long long* total;
@@ -164,7 +165,8 @@ __device__ __forceinline__ void load4(const float* p, int64_t i, int64_t M, floa
 }
 
 // One pass over the steps: the sums of the loss and the statistics (SUMS) and
-// the gradient (GRAD).  A batch of at most kAlone steps is one CTA's, which then counts
+// the gradient (GRAD).  17 bytes read and 4 written a step; bound by instruction issue (two
+// exponentials, two two-float differences): 4096 x 2048 steps in 57 us, 3.1 TB/s.  A batch of at most kAlone steps is one CTA's, which then counts
 // the steps itself first (COUNT; norm is written as count_kernel does): one launch instead of two, where
 // the launches are most of the time.
 constexpr int kAlone = 8192, kAloneThreads = 1024;
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(NT, NT == kThreads ? kPolicyCtas : 1) policy_k
   if constexpr (SUMS) finish_sums<NT>(sum, out);
 }
 
-// The policy loss over long rows: their records' terms.
+// The policy loss over long rows: their records' terms (8192 rows: 5 us, latency).
 __global__ void __launch_bounds__(kThreads) row_sums_kernel(const float4* stats, const float* entropy, int64_t rows,
                                                        SumOut o) {
   double sum[kSums] = {0, 0, 0, 0, 0, 0};
