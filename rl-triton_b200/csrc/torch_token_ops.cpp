@@ -24,6 +24,7 @@
 #include <torch/custom_class.h>
 #include <torch/library.h>
 
+#include <map>
 #include <mutex>
 #include <tuple>
 #include <utility>
@@ -120,6 +121,21 @@ Tensor op_grad_buffer(const Tensor& logits) {
   return at::empty_strided(logits.sizes(), logits.strides(), logits.options());
 }
 
+// In the place of an output that a call does not have: an empty tensor, made once a
+// device, type and output (an allocation less for each; no two outputs share one).
+enum Missing { kEntropy, kStatistics, kNorm, kRows, kGradient, kOrder };
+Tensor none(const Tensor& t, Missing what, at::ScalarType type = at::kFloat) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, int, at::ScalarType>, Tensor> made;
+  std::lock_guard<std::mutex> lock(mu);
+  Tensor& n = made[{(int)t.device().index(), (int)what, type}];
+  if (!n.defined()) {
+    c10::InferenceMode normal(false);  // it may be saved for a backward call later
+    n = at::empty({0}, at::TensorOptions().device(t.device()).dtype(type));
+  }
+  return n;
+}
+
 struct LogitsArgs {
   Tensor x, tokens;
   MaskArg mask;
@@ -129,7 +145,7 @@ struct LogitsArgs {
   // Long rows with a mask go by an order of the rows, made once for both directions.
   Tensor order_buffer() const {
     const bool some = mask.t && v > RLS_SHORT_VOCAB && n * t <= 0x7ffffffe;
-    return at::empty({some ? n * t + 1 : 0}, x.options().dtype(at::kInt));
+    return some ? at::empty({n * t + 1}, x.options().dtype(at::kInt)) : none(x, kOrder, at::kInt);
   }
   Tensor order() const {
     Tensor o = order_buffer();
@@ -147,7 +163,7 @@ Tensor like(const Tensor& t, at::IntArrayRef sizes) { return at::empty(sizes, t.
 
 // What a long row keeps for the backward call.
 Tensor row_stats(const LogitsArgs& a, bool keep) {
-  return like(a.x, keep && a.v > RLS_SHORT_VOCAB ? at::IntArrayRef({a.n, a.t, RLS_ROW_STATS}) : at::IntArrayRef({0}));
+  return keep && a.v > RLS_SHORT_VOCAB ? like(a.x, {a.n, a.t, RLS_ROW_STATS}) : none(a.x, kRows);
 }
 
 // ---- log-probabilities -------------------------------------------------------------
@@ -157,7 +173,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_logprobs(const Tensor& logits, con
   const Placed placed(logits, tokens, mask);
   const LogitsArgs a(logits, tokens, mask);
   Tensor lp = like(a.x, {a.n, a.t});
-  Tensor ent = like(a.x, entropy ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
+  Tensor ent = entropy ? like(a.x, {a.n, a.t}) : none(a.x, kEntropy);
   Tensor stats = row_stats(a, keep), order = a.order();
   check(rls_token_logprobs(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), a.mask.ptr(),
                            a.mask.kind, I(order), W(lp), W(ent), W(stats), a.n, a.t, a.v, temperature, dtype_of(a.x),
@@ -195,7 +211,7 @@ rls_policy_t policy_of(double clip_low, double clip_high, double dual_clip, doub
 }
 
 Tensor norm_for(const MaskArg& m, const Tensor& ref, int64_t n, int64_t reduction) {
-  return like(ref, {m.t && reduction != RLS_REDUCE_SUM ? n + 1 : 0});
+  return m.t && reduction != RLS_REDUCE_SUM ? like(ref, {n + 1}) : none(ref, kNorm);
 }
 
 Tensor policy_workspace(const Tensor& t) { return workspace_for(t.device(), stream_of(t), 1 << 20); }
@@ -212,8 +228,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_policy(const Tensor& logprobs, con
   const MaskArg m = mask_arg(mask);
   const int64_t n = lp.size(0), t = lp.size(1);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, 0.0, reduction);
-  Tensor loss = like(lp, {}), stats = like(lp, {need_stats ? 5 : 0}), norm = norm_for(m, lp, n, reduction);
-  Tensor grad = like(lp, need_grad ? at::IntArrayRef({n, t}) : at::IntArrayRef({0}));
+  Tensor loss = like(lp, {}), stats = need_stats ? like(lp, {5}) : none(lp, kStatistics), norm = norm_for(m, lp, n, reduction);
+  Tensor grad = need_grad ? like(lp, {n, t}) : none(lp, kGradient);
   Tensor ws = policy_workspace(lp);
   check(rls_policy_loss(F(lp), F(old_lp), F(adv), adv.dim() == 1, F(rf), m.ptr(), m.kind, &p, (float)grad_scale,
                         W(norm), loss.data_ptr<float>(), W(stats), W(grad), n, t, ws.data_ptr(),
@@ -247,10 +263,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_po
   const Tensor old_lp = f32(old_logprobs), adv = f32(advantages);
   const OptT rf = f32(ref);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
-  Tensor loss = like(a.x, {}), stats = like(a.x, {need_stats ? 5 : 0}), norm = norm_for(a.mask, a.x, a.n, reduction);
+  Tensor loss = like(a.x, {}), stats = need_stats ? like(a.x, {5}) : none(a.x, kStatistics), norm = norm_for(a.mask, a.x, a.n, reduction);
   Tensor lp = like(a.x, {a.n, a.t}), rows = row_stats(a, true), order = a.order_buffer();
-  Tensor ent = like(a.x, need_stats || entropy_coef != 0.0 ? at::IntArrayRef({a.n, a.t}) : at::IntArrayRef({0}));
-  Tensor g = need_grad ? op_grad_buffer(a.x) : at::empty({0}, a.x.options());
+  Tensor ent = need_stats || entropy_coef != 0.0 ? like(a.x, {a.n, a.t}) : none(a.x, kEntropy);
+  Tensor g = need_grad ? op_grad_buffer(a.x) : none(a.x, kGradient, a.x.scalar_type());
   Tensor ws = policy_workspace(a.x);
   check(rls_policy_loss_logits(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(), F(old_lp),
                                F(adv), adv.dim() == 1, F(rf), a.mask.ptr(), a.mask.kind, I(order), &p, (float)grad_scale,
@@ -366,7 +382,7 @@ std::tuple<Tensor, Tensor> op_preference_backward(const Tensor& coef, const Tens
   if (halves) {
     // coefficients [2, b] are those of 2b rows one below the other
     gc = like(coef, {2 * b, chosen_len});
-    gr = like(coef, {0});
+    gr = none(coef, kGradient);
     check(rls_preference_loss_backward(W(coef), F(g), m[0].ptr(), nullptr, kind, W(gc), nullptr, 2 * b, chosen_len, 0,
                                        stream_of(coef)),
           "rls_preference_loss_backward");
