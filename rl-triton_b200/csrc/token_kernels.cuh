@@ -1648,10 +1648,11 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
 // log-probability, loss term and coefficients -- the fp64 and the transcendental steps
 // that would cost a whole warp's time with a warp a row -- and the gradient is
 // written over the stretch again, by vectors that need not respect the rows.
-// Bound by instruction issue (two thirds of the slots): 1.07 GB in rows of 18 fp32 take 266 us forward
-// (0.62 of the copy bandwidth) and 641 us with the gradient (0.52), where a warp's lanes
-// in groups of 8 took 887 and 2211; rows of 1024 fp32 181 us (0.92) and 428 us (0.78).  More
-// CTAs an SM are faster at any unrolling (5 of 256 threads: 48 registers).
+// Bound by instruction issue (two thirds of the slots): 1.07 GB in rows of 18 fp32 take 281 us forward
+// (0.59 of the copy bandwidth) and 652 us with the gradient (0.51), where a warp's lanes
+// in groups of 8 took 887 and 2211; rows of 64 bf16 279 us (0.60), of 512 bf16 252 us
+// (0.66), of 200 fp32 201 us (0.83).  More CTAs an SM are faster at any unrolling (5
+// of 256 threads: 48 registers).
 // ACC: how a lane reads a row: 0 one element, 1 two (V even), 2 a 16-byte vector (rows are whole vectors).
 constexpr int kTileThreads = 256;
 constexpr int kTileCtas = 5;  // an SM: 48 registers a thread
@@ -1659,7 +1660,7 @@ constexpr int kTileCtas = 5;  // an SM: 48 registers a thread
 struct TileShape {
   int rows, log_lanes; // R, log2 G
   int turn;            // a row's lanes start `turn` rounds further than the last row's do (bank conflicts), ...
-  int rounds;          // ... of so many whole ones
+  int rounds;          // ... of so many that all lanes take part in
   Divide by_vocab;     // an element's row
 };
 
@@ -1678,7 +1679,7 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) tile_rows_kernel(Rows
   const float c = in.c;
   double sum[kTerms ? kSums : 1] = {};
   const int r = tid >> shape.log_lanes, lane = tid & (G - 1);
-  const int first = lane + (shape.turn ? r % shape.rounds * G : 0);
+  const int first = lane + (shape.turn && shape.rounds ? r % shape.rounds * G : 0);
   const int64_t tiles = (in.rows + R - 1) / R;
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int64_t row0 = t * R;
@@ -1727,10 +1728,21 @@ __global__ void __launch_bounds__(kTileThreads, kTileCtas) tile_rows_kernel(Rows
           f[0] = f2(Vec<T>::get(line + k), -INFINITY);
         }
       };
-      // the lane's accesses from `first` on, then those before it
+      // the lane's accesses; with a turn from `first` on, around the end of the whole
+      // rounds, then the rest (always going round costs 8 % where no turn is needed)
       auto each = [&](auto&& f) {
-        for (int k = first; k < n; k += G) f(k);
-        for (int k = lane; k < first && k < n; k += G) f(k);
+        if (!shape.turn) {
+          for (int k = lane; k < n; k += G) f(k);
+        } else {
+          const int whole = there ? shape.rounds : 0, wrap = shape.rounds * G;
+          int k = first;
+          for (int i = 0; i < whole; ++i) {
+            f(k);
+            k += G;
+            if (k >= wrap) k -= wrap;
+          }
+          if (lane + wrap < n) f(lane + wrap);
+        }
       };
       float m = -INFINITY;
       each([&](int k) {
