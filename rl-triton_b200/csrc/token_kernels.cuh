@@ -312,10 +312,6 @@ struct Vec<float> {
     const float2 v = *reinterpret_cast<const float2*>(p);
     return f2(v.x, v.y);
   }
-  // The vector's elements, one store each.
-  __device__ __forceinline__ static void scatter(float* p, const uint4& u) {
-    p[0] = __uint_as_float(u.x); p[1] = __uint_as_float(u.y); p[2] = __uint_as_float(u.z); p[3] = __uint_as_float(u.w);
-  }
   __device__ __forceinline__ static float get(const float* p) { return *p; }
   __device__ __forceinline__ static float put(float v) { return v; }
 };
@@ -380,15 +376,6 @@ struct Vec<__nv_bfloat16> {
   __device__ __forceinline__ static F2 two(const __nv_bfloat16* p) {
     const unsigned w = *reinterpret_cast<const unsigned*>(p);
     return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  }
-  __device__ __forceinline__ static void scatter(__nv_bfloat16* p, const uint4& u) {
-    unsigned short* h = reinterpret_cast<unsigned short*>(p);
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[2 * k] = (unsigned short)(w[k] & 0xffffu);
-      h[2 * k + 1] = (unsigned short)(w[k] >> 16);
-    }
   }
   __device__ __forceinline__ static float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   __device__ __forceinline__ static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
