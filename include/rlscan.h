@@ -349,7 +349,9 @@ int rls_token_logprobs_backward(const void* logits, int64_t env_stride, int64_t 
  *   RLS_REDUCE_SEQUENCE  loss = mean over the envs that have any of the mean
  *                        of the env's terms,
  *   RLS_REDUCE_SUM       loss = sum(term).
- * No step counts: loss 0, gradients 0.                                        */
+ * No step counts: loss 0, gradients 0.  The derivative jumps at the bounds; a step's
+ * side is that of its exact ratio against 1 - clip_low, 1 + clip_high and dual_clip
+ * in 64 bits, so at steps within a rounding of one an evaluation in fp32 may differ. */
 #define RLS_KL_K1 1
 #define RLS_KL_K2 2
 #define RLS_KL_K3 3
@@ -357,9 +359,9 @@ int rls_token_logprobs_backward(const void* logits, int64_t env_stride, int64_t 
 #define RLS_REDUCE_SEQUENCE 1
 #define RLS_REDUCE_SUM      2
 typedef struct rls_policy {
-    float clip_low, clip_high, dual_clip;
-    float kl_coef, entropy_coef;
-    int   kl_kind, reduction;
+    double clip_low, clip_high, dual_clip;
+    float  kl_coef, entropy_coef;
+    int    kl_kind, reduction;
 } rls_policy_t;
 
 /* From log-probabilities.  advantages: [num_envs, seq_len], or [num_envs] with

@@ -564,8 +564,9 @@ __device__ __forceinline__ float drift_of(Diff lr) {
 // -min(r A, clip(r) A), at most -dual A where A < 0, plus the KL estimate:
 // k1 = lp - ref, k2 = (lp - ref)^2 / 2, k3 = exp(ref - lp) - (ref - lp) - 1.
 // Whether the clip holds is decided on log r with twice fp32's digits (exact for
-// fp32 inputs): the derivative jumps there, and exp's rounding would put
-// steps near a bound on either side of it.  lr = lp - old, away = lp - ref.
+// fp32 inputs), against the logarithms of the caller's bounds: the derivative jumps there,
+// and exp's rounding would put steps near a bound on either side of it (in fp32
+// exp(-0.22314358) may round to 0.8f; it is 0.79999998).  lr = lp - old, away = lp - ref.
 __device__ __forceinline__ PolicyTerm policy_term(const Policy& p, Diff lr, float adv, Diff away) {
   PolicyTerm o;
   float gain = expf(lr.x);

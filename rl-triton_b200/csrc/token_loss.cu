@@ -288,16 +288,19 @@ Policy make_policy(const rls_policy_t& q, const float* old_lp, const float* adv,
   p.adv = adv;
   p.adv_row = per_env != 0;
   p.ref = ref;
-  p.lo = 1.f - q.clip_low;
-  p.hi = 1.f + q.clip_high;
-  p.dual = q.dual_clip;
+  // The bounds are the caller's numbers: what the ratio is compared with (their
+  // logarithms) and what the clip holds it at (rounded once) come from the same ones.
+  const double lo = 1.0 - q.clip_low, hi = 1.0 + q.clip_high;
+  p.lo = (float)lo;
+  p.hi = (float)hi;
+  p.dual = (float)q.dual_clip;
   auto two = [](double x) {
     const float a = (float)x;
     return make_float2(a, std::isfinite(x) ? (float)(x - (double)a) : 0.f);
   };
-  p.log_lo = two(q.clip_low < 1.f ? std::log1p(-(double)q.clip_low) : -INFINITY);
-  p.log_hi = two(std::log1p((double)q.clip_high));
-  p.log_dual = two(q.dual_clip > 0.f ? std::log((double)q.dual_clip) : INFINITY);
+  p.log_lo = two(lo > 0.0 ? std::log(lo) : -INFINITY);
+  p.log_hi = two(std::log(hi));
+  p.log_dual = two(q.dual_clip > 0.0 ? std::log(q.dual_clip) : INFINITY);
   p.kl_coef = q.kl_coef;
   p.kl_kind = q.kl_kind;
   p.ent_coef = q.entropy_coef;

@@ -200,9 +200,9 @@ Tensor op_logprobs_backward(const Tensor& logits, const Tensor& tokens, const Op
 rls_policy_t policy_of(double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
                        double entropy_coef, int64_t reduction) {
   rls_policy_t p{};
-  p.clip_low = (float)clip_low;
-  p.clip_high = (float)clip_high;
-  p.dual_clip = (float)dual_clip;
+  p.clip_low = clip_low;
+  p.clip_high = clip_high;
+  p.dual_clip = dual_clip;
   p.kl_coef = (float)kl_coef;
   p.entropy_coef = (float)entropy_coef;
   p.kl_kind = (int)kl;

@@ -54,7 +54,7 @@ class Segment(ctypes.Structure):
 class Policy(ctypes.Structure):
     """Mirror of rls_policy_t."""
 
-    _fields_ = [("clip_low", ctypes.c_float), ("clip_high", ctypes.c_float), ("dual_clip", ctypes.c_float),
+    _fields_ = [("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double), ("dual_clip", ctypes.c_double),
                 ("kl_coef", ctypes.c_float), ("entropy_coef", ctypes.c_float), ("kl_kind", ctypes.c_int),
                 ("reduction", ctypes.c_int)]
 
