@@ -223,6 +223,7 @@ __device__ __forceinline__ double log2_of(float s0) {
 __device__ __forceinline__ double logprob_of(float x_tok, const RowStats& r, float c, double c64, double c_off) {
   const Shift sh = shift_of(r, c);
   if (!r.far && r.others >= 0.f) {
+    if (x_tok == -INFINITY) return -INFINITY;  // c_off times an infinite d would be NaN
     const double d = (double)x_tok * (double)c - (double)sh.off;
     const double l = log2_of(r.others) - d + c_off * ((double)r.t_others - d) + 7.2e-8;  // log2 q
     if (l > 0.0) return -(l * 0.693147180559945309417 + (double)log1pf(exp2f(-(float)l)));

@@ -1,14 +1,17 @@
 """The token-level policy operators at the edges of their definitions: steps at
-a clip bound."""
+a clip bound, tokens whose own logit is -inf.  Tolerances of log-probabilities,
+entropies and gradients as in test_token_ops_gpu.py."""
 import math
 
 import pytest
 import torch
 
 import _token_ref as ref64
+from test_token_ops_gpu import S, close, make, tol_ent, tol_grad, tol_lp
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
+INF = float("inf")
 
 
 def _cuda():
@@ -54,3 +57,43 @@ def test_steps_at_a_clip_bound(low, high, dual):
     assert abs(float(st["clip_fraction"]) - stats["clip_fraction"]) <= U
     size = float(((lp.double() - old.double()).exp() * adv.double()).abs().sum())
     assert abs(float(loss.detach()) - float(want.detach())) <= 8 * U * size
+
+
+@pytest.mark.parametrize("temp", [0.7, 0.8, 1.0, 1.1, 1.5])
+@pytest.mark.parametrize("v", [18, 600, 1025, 5003, 131072, 300001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tokens_whose_logit_is_minus_infinity(v, dtype, temp):
+    """A masked action that was taken: log-probability -inf, the entropy and all
+    gradients as ever, and a policy loss with ratio 0."""
+    _cuda()
+    import rl_triton
+    x, tok, _, g = make(2, 3, v, dtype, seed=v, pad=5)
+    tok[0, 1], tok[1, 0], tok[1, 2] = v - 1, v - 5, v - 3
+    up, up_h = torch.randn(2, 3, generator=g), torch.randn(2, 3, generator=g)
+    bf16 = dtype == torch.bfloat16
+    xd = x.double().requires_grad_(True)
+    lp64, h64 = ref64.logprobs(xd, tok, None, temp)
+    (wg,) = torch.autograd.grad([lp64, h64], xd, [up.double(), up_h.double()])
+    xc = x.cuda().requires_grad_(True)
+    lp, h = rl_triton.compute_token_logprobs(xc, tok.cuda(), temperature=temp, return_entropy=True)
+    (got,) = torch.autograd.grad([lp, h], xc, [up.cuda(), up_h.cuda()])
+    assert int((lp == -INF).sum()) == 3
+    close(lp, lp64, **tol_lp(v))
+    close(h, h64, **tol_ent(v))
+    close(got, wg, **tol_grad(v, 4.0 / temp, bf16))
+    with torch.no_grad():
+        close(rl_triton.compute_token_logprobs(xc, tok.cuda(), temperature=temp), lp64, **tol_lp(v))
+    old = (torch.where(lp64 > -INF, lp64, torch.tensor(-4.0, dtype=torch.float64)) - 0.05).detach().float()
+    adv = torch.tensor([[1.0, -0.5, 0.7], [1.5, -1.0, -0.3]])
+    for ent in (0.0, 0.02):
+        xd = x.double().requires_grad_(True)
+        lp64, h64 = ref64.logprobs(xd, tok, None, temp)
+        want, _ = ref64.policy(lp64, old.double(), adv.double(), entropy=h64, entropy_coef=ent)
+        (wg,) = torch.autograd.grad(want, xd)
+        assert torch.isfinite(want) and torch.isfinite(wg).all()
+        loss, lp = rl_triton.compute_policy_loss_from_logits(xc, tok.cuda(), old.cuda(), adv.cuda(), entropy_coef=ent,
+                                                             temperature=temp)
+        (got,) = torch.autograd.grad(loss, xc)
+        close(lp, lp64, **tol_lp(v))
+        close(loss, want, rtol=2 * U, atol=12 * (S(v) + 8 * U + ent * tol_ent(v)["atol"]))
+        close(got, wg, **tol_grad(v, 4 * float(wg.abs().max()), bf16))
