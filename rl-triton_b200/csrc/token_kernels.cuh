@@ -572,6 +572,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const Policy& p, Diff lr, floa
   PolicyTerm o;
   float gain = expf(lr.x);
   if (gain < INFINITY) gain = fmaf(gain, lr.low, gain);
+  else if (adv == 0.f && lr.x < INFINITY) gain = 0.f;  // a ratio past fp32's range, times 0
   gain *= adv;
   const bool up = above(lr, p.log_hi), down = below(lr, p.log_lo), far = above(lr, p.log_dual);
   o.clipped = adv > 0.f ? up : adv < 0.f && (down || far);

@@ -1,5 +1,6 @@
 """The token-level policy operators at the edges of their definitions: steps at
-a clip bound, tokens whose own logit is -inf.  Tolerances of log-probabilities,
+a clip bound, tokens whose own logit is -inf, ratios past the range of fp32.
+Tolerances of log-probabilities,
 entropies and gradients as in test_token_ops_gpu.py."""
 import math
 
@@ -97,3 +98,31 @@ def test_tokens_whose_logit_is_minus_infinity(v, dtype, temp):
         close(lp, lp64, **tol_lp(v))
         close(loss, want, rtol=2 * U, atol=12 * (S(v) + 8 * U + ent * tol_ent(v)["atol"]))
         close(got, wg, **tol_grad(v, 4 * float(wg.abs().max()), bf16))
+
+
+@pytest.mark.parametrize("v", [0, 18, 2000])
+def test_a_ratio_past_fp32_times_an_advantage_of_zero(v):
+    """exp(lp - old) is finite in 64 bits and infinite in fp32: the term of a step
+    with advantage 0 (all rewards of its group alike) is 0 all the same; v = 0: from
+    log-probabilities."""
+    _cuda()
+    import rl_triton
+    x, tok, _, _ = make(2, 3, max(v, 2), seed=3)
+    lp64 = ref64.logprobs(x.double(), tok)[0]
+    old = (lp64 - 0.1).float()
+    old[0, 1] = old[1, 2] = -150.0
+    adv = torch.tensor([[0.5, 0.0, 0.3], [0.2, -0.4, -0.0]])
+    leaf = (x if v else lp64.float()).cuda().requires_grad_(True)
+    exact = leaf.detach().cpu().double().requires_grad_(True)
+    args = [t.cuda() for t in ((tok, old, adv) if v else (old, adv))]
+    fn = rl_triton.compute_policy_loss_from_logits if v else rl_triton.compute_policy_loss
+    for dual in (None, 2.0):
+        out = fn(leaf, *args, dual_clip=dual)
+        loss = out[0] if v else out
+        lpd = ref64.logprobs(exact, tok)[0] if v else exact
+        want, _ = ref64.policy(lpd, old.double(), adv.double(), dual_clip=dual)
+        (wg,) = torch.autograd.grad(want, exact)
+        (got,) = torch.autograd.grad(loss, leaf)
+        assert torch.isfinite(want) and torch.isfinite(wg).all()
+        close(loss, want, rtol=2 * U, atol=12 * (S(max(v, 2)) + 8 * U))
+        close(got, wg, **tol_grad(max(v, 2), 4 * float(wg.abs().max()), False))
