@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(NT) preference_kernel(PrefArgs p) {
     if (p.kind == RLS_PREFERENCE_SIGMOID) {
       // the parts of size 1 in fp32, as one thread forms them while the CTA waits
       const float z = expf(-fabsf((float)x)), l = log1pf(z);
-      term = (double)l + (1.0 - e) * fmax(-x, 0.0) + e * fmax(x, 0.0);
+      term = (double)l + (1.0 - e) * fmax(-x, 0.0);
+      if (e > 0.0) term += e * fmax(x, 0.0);  // x may be +inf: a rejected token of log-probability -inf
       const float less = z / (1.f + z);  // the smaller of sig(x) and sig(-x)
       d = beta * (x >= 0 ? e - (double)less : (double)less - (1.0 - e));
       if (isnan(x)) term = d = x;

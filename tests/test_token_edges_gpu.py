@@ -1,6 +1,6 @@
 """The token-level policy operators at the edges of their definitions: steps at
-a clip bound, tokens whose own logit is -inf, ratios past the range of fp32.
-Tolerances of log-probabilities,
+a clip bound, tokens whose own logit is -inf, ratios past the range of fp32,
+responses with a token of log-probability -inf.  Tolerances of log-probabilities,
 entropies and gradients as in test_token_ops_gpu.py."""
 import math
 
@@ -126,3 +126,33 @@ def test_a_ratio_past_fp32_times_an_advantage_of_zero(v):
         assert torch.isfinite(want) and torch.isfinite(wg).all()
         close(loss, want, rtol=2 * U, atol=12 * (S(max(v, 2)) + 8 * U))
         close(got, wg, **tol_grad(max(v, 2), 4 * float(wg.abs().max()), False))
+
+
+@pytest.mark.parametrize("loss,smoothing", [("sigmoid", 0.0), ("sigmoid", 0.1), ("hinge", 0.0)])
+@pytest.mark.parametrize("normalized", [False, True])
+def test_preference_with_a_rejected_token_of_probability_zero(loss, smoothing, normalized):
+    """The pair's x is +inf: -log sig(x) and the hinge are 0, and so is its
+    gradient; with smoothing -e log sig(-x) is +inf."""
+    _cuda()
+    import rl_triton
+    g = torch.Generator().manual_seed(7)
+    lp, refl = -3 * torch.rand(6, 9, generator=g), -3 * torch.rand(6, 9, generator=g)
+    lp[4, 3] = -INF  # the second pair's rejected response
+    leaf = lp.cuda().requires_grad_(True)
+    kw = dict(beta=0.3, loss=loss, label_smoothing=smoothing, length_normalized=normalized)
+    got, good, bad = rl_triton.compute_preference_loss(leaf, refl.cuda(), **kw)
+    (grad,) = torch.autograd.grad(got, leaf)
+    assert bad[1] == -INF and torch.isfinite(bad[[0, 2]]).all() and torch.isfinite(good).all()
+    if smoothing:
+        assert got == INF
+        return
+    keep = [0, 2]  # the other pairs, their mean over all three
+    ld = lp.double().requires_grad_(True)
+    a, b = ld[:3][keep], ld[3:][keep]
+    want, _, _ = ref64.preference(a, b, (refl[:3][keep].double(), refl[3:][keep].double()), (None, None), 0.3, loss,
+                                  smoothing, normalized)
+    want = want * 2 / 3
+    (wg,) = torch.autograd.grad(want, ld)
+    close(got, want, rtol=128 * U, atol=1e-7)
+    close(grad, wg, rtol=128 * U, atol=1e-9)
+    assert (grad[[1, 4]] == 0).all()
