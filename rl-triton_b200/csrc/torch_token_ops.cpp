@@ -21,6 +21,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/custom_class.h>
 #include <torch/library.h>
 
@@ -447,6 +449,20 @@ Kept& kept_of(AutogradContext* ctx) {
   return *static_cast<Kept*>(ctx->saved_data.begin()->second.toCapsule().get());
 }
 
+// The losses' gradients have no derivative of their own.  Where the backward call is
+// itself recorded (create_graph) they get a node that raises once it is reached, on
+// the way to `sources`, so that a term that is made of them cannot get lost.
+void no_second_derivative(const char* name, torch::autograd::edge_list sources, const variable_list& grads) {
+  if (!at::GradMode::is_enabled()) return;
+  auto node = std::make_shared<torch::autograd::NotImplemented>(name, std::move(sources));
+  for (const Tensor& g : grads)
+    if (g.defined()) torch::autograd::set_history(g, node);
+}
+// The sources of a loss that does not save them.
+struct Sources : public torch::CustomClassHolder {
+  torch::autograd::edge_list edges;
+};
+
 Tensor call_grad_buffer(const Tensor& logits) {
   static auto op = inner("rl_triton::_grad_buffer", &op_grad_buffer);
   return op.call(logits);
@@ -516,6 +532,8 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
             k.kl, k.reduction, k.grad_scale, fresh);
     variable_list out(13);
     out[0] = s[0].scalar_type() == at::kFloat ? grad : grad.to(s[0].scalar_type());
+    no_second_derivative("the gradient of rl_triton::policy_loss", torch::autograd::collect_next_edges(s[0], g[0]),
+                         {out[0]});
     return out;
   }
 };
@@ -569,6 +587,8 @@ struct PolicyLossLogits : public torch::autograd::Function<PolicyLossLogits> {
             k.kl_coef, k.kl, k.entropy_coef, k.temperature, k.reduction, k.grad_scale, fresh);
     variable_list out(16);
     out[0] = grad;
+    no_second_derivative("the gradient of rl_triton::policy_loss_logits",
+                         torch::autograd::collect_next_edges(s[0], g[0]), {out[0]});
     return out;
   }
 };
@@ -602,6 +622,10 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
     ctx->saved_data["rejected_len"] = rejected ? rejected->size(1) : (int64_t)-1;
     ctx->saved_data["types"] = std::vector<int64_t>{
         (int64_t)chosen.scalar_type(), (int64_t)(rejected ? rejected->scalar_type() : chosen.scalar_type())};
+    auto sources = c10::make_intrusive<Sources>();
+    sources->edges = rejected ? torch::autograd::collect_next_edges(chosen, *rejected)
+                              : torch::autograd::collect_next_edges(chosen);
+    ctx->saved_data["sources"] = c10::IValue::make_capsule(std::move(sources));
     ctx->mark_non_differentiable({good, bad});
     ctx->set_materialize_grads(false);
     return {loss, good, bad};
@@ -617,6 +641,11 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
     variable_list out(10);
     out[0] = gc.to((at::ScalarType)types[0]);
     if (other >= 0) out[1] = gr.to((at::ScalarType)types[1]);
+    if (at::GradMode::is_enabled()) {
+      auto edges = static_cast<Sources*>(ctx->saved_data["sources"].toCapsule().get())->edges;
+      for (auto& e : torch::autograd::collect_next_edges(g[0])) edges.push_back(std::move(e));
+      no_second_derivative("the gradient of rl_triton::preference_loss", std::move(edges), out);
+    }
     return out;
   }
 };
@@ -693,7 +722,8 @@ TORCH_LIBRARY_IMPL(rl_triton, Autograd, m) {
   m.impl("policy_loss", &policy_loss_autograd);
   m.impl("policy_loss_logits", &policy_loss_logits_autograd);
   m.impl("preference_loss", &preference_loss_autograd);
-  // The kernels proper have no second derivative: differentiating them raises.
+  // The kernels proper have no second derivative: differentiating them raises (the
+  // losses' gradients by no_second_derivative()).
   for (const char* name : {"_token_logprobs", "_token_logprobs_backward", "_policy_loss", "_policy_loss_logits",
                            "_preference_loss", "_preference_loss_backward"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());

@@ -156,3 +156,24 @@ def test_preference_with_a_rejected_token_of_probability_zero(loss, smoothing, n
     close(got, want, rtol=128 * U, atol=1e-7)
     close(grad, wg, rtol=128 * U, atol=1e-9)
     assert (grad[[1, 4]] == 0).all()
+
+
+def test_gradients_with_create_graph():
+    """The same values, and an error once one of them is differentiated."""
+    _cuda()
+    import rl_triton as rl
+    x, tok, _, g = make(4, 6, 2000, seed=2)
+    old, adv = -torch.rand(4, 6, generator=g).cuda(), torch.randn(4, generator=g).cuda()
+    tok = tok.cuda()
+    logits, lp = x.cuda(), -torch.rand(4, 6, generator=g).cuda()
+    for leaf, f in [(lp, lambda z: rl.compute_policy_loss(z, old, adv)),
+                    (logits, lambda z: rl.compute_policy_loss_from_logits(z, tok, old, adv)[0]),
+                    (lp, lambda z: rl.compute_preference_loss(z)[0]),
+                    (lp, lambda z: rl.compute_preference_loss((z[:2], z[2:]))[0])]:
+        z = leaf.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(f(z), z)
+        value = f(z)
+        (got,) = torch.autograd.grad(value, z, create_graph=True)
+        assert torch.equal(got, want) and got.requires_grad and not want.requires_grad
+        with pytest.raises(RuntimeError, match="not implemented"):
+            (value + got.square().sum()).backward()
