@@ -468,6 +468,14 @@ Tensor call_grad_buffer(const Tensor& logits) {
   return op.call(logits);
 }
 
+// Forward-mode tangents would be dropped in silence below autograd.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptT& t) { return t && has_tangent(*t); }
+template <class... Ts>
+void no_tangents(const char* name, const Ts&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), name, ": forward-mode derivatives are not implemented");
+}
+
 struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const OptT& mask,
                                double temperature, bool entropy) {
@@ -492,6 +500,7 @@ struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
 
 std::tuple<Tensor, Tensor> token_logprobs_autograd(const Tensor& logits, const Tensor& tokens, const OptT& mask,
                                                    double temperature, bool entropy) {
+  no_tangents("rl_triton::token_logprobs", logits, mask);
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     auto o = TokenLogprobs::apply(logits, tokens, mask, temperature, entropy);
     return {o[0], o[1]};
@@ -542,6 +551,7 @@ std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& lp, const Tensor& 
                                                 const OptT& mask, const OptT& ref, double clip_low, double clip_high,
                                                 double dual_clip, double kl_coef, int64_t kl, int64_t reduction,
                                                 double grad_scale, bool need_stats) {
+  no_tangents("rl_triton::policy_loss", lp, old_lp, adv, mask, ref);
   if (at::GradMode::is_enabled() && lp.requires_grad()) {
     auto o = PolicyLoss::apply(lp, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef, kl, reduction,
                                grad_scale, need_stats);
@@ -597,6 +607,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss_logits_autograd(
     const Tensor& logits, const Tensor& tokens, const Tensor& old_lp, const Tensor& adv, const OptT& mask,
     const OptT& ref, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
     double entropy_coef, bool need_stats, double temperature, int64_t reduction, double grad_scale) {
+  no_tangents("rl_triton::policy_loss_logits", logits, old_lp, adv, mask, ref);
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     auto o = PolicyLossLogits::apply(logits, tokens, old_lp, adv, mask, ref, clip_low, clip_high, dual_clip, kl_coef,
                                      kl, entropy_coef, need_stats, temperature, reduction, grad_scale);
@@ -653,6 +664,7 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
 std::tuple<Tensor, Tensor, Tensor> preference_loss_autograd(const Tensor& chosen, const OptT& rejected, const OptT& ref_c,
                                                     const OptT& ref_r, const OptT& mask_c, const OptT& mask_r,
                                                     double beta, double smoothing, int64_t kind, bool normalized) {
+  no_tangents("rl_triton::preference_loss", chosen, rejected, ref_c, ref_r, mask_c, mask_r);
   if (at::GradMode::is_enabled() && (chosen.requires_grad() || (rejected && rejected->requires_grad()))) {
     auto o = PreferenceLoss::apply(chosen, rejected, ref_c, ref_r, mask_c, mask_r, beta, smoothing, kind, normalized);
     return {o[0], o[1], o[2]};

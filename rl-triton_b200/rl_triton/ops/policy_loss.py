@@ -50,7 +50,9 @@ def compute_policy_loss(
     same pass for an incoming gradient of `grad_scale` (the loss itself is not
     scaled).  The backward pass computes it anew only if the incoming gradient
     is another one: give the factor that loss.backward() will see (1 / the number
-    of accumulated minibatches, a loss scale) to spare that.
+    of accumulated minibatches, a loss scale) to spare that.  The other inputs are
+    constants of the loss: no gradient flows to old_logprobs, advantages or
+    ref_logprobs, whether they require one or not.
 
     Args:
         logprobs, old_logprobs, ref_logprobs: [num_envs, seq_len], float32 or
@@ -107,7 +109,8 @@ def compute_policy_loss_from_logits(
 
         term = (as in compute_policy_loss) - entropy_coef entropy
 
-    Arguments as there; `grad_scale` matters more here, since another incoming
+    Differentiable with respect to the logits alone.  Arguments as there;
+    `grad_scale` matters more here, since another incoming
     gradient costs a second pass over the logits.  The logits must not change
     before the backward pass.
 

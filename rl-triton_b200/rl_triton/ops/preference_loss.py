@@ -37,7 +37,8 @@ def compute_preference_loss(
         "hinge"    max(0, 1 - x)
 
     The loss is the mean over the pairs.  Differentiable with respect to the
-    log-probabilities (compute_token_logprobs gives them from the logits).
+    log-probabilities (compute_token_logprobs gives them from the logits); the
+    reference's are constants, no gradient flows to them.
 
     Args:
         logprobs: [2 * pairs, seq_len], the preferred responses in the first
