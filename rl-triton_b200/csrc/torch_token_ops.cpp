@@ -74,6 +74,37 @@ class Placed {
   int before_;
 };
 
+// The kernels go by the sizes and types that a call names, so every tensor of a call is
+// held against them: the operators can be called without the functions in front of them.
+void shaped(const Tensor& t, at::IntArrayRef sizes, const char* name) {
+  TORCH_CHECK(t.sizes() == sizes, name, ": expected shape ", sizes, ", got ", t.sizes());
+}
+void real(const Tensor& t, at::IntArrayRef sizes, const char* name) {
+  shaped(t, sizes, name);
+  TORCH_CHECK(t.is_floating_point(), name, ": expected floating point, got ", t.scalar_type());
+}
+void real(const OptT& t, at::IntArrayRef sizes, const char* name) {
+  if (t && t->defined()) real(*t, sizes, name);
+}
+void masks(const OptT& t, at::IntArrayRef sizes, const char* name) {
+  if (!t || !t->defined()) return;
+  shaped(*t, sizes, name);
+  TORCH_CHECK(!t->is_complex(), name, ": expected bool, integers or floats, got ", t->scalar_type());
+}
+void scalar(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.numel() == 1 && t.is_floating_point(), name, ": expected one floating-point number");
+}
+// Advantages, one a step or one a row.
+void advantages_ok(const Tensor& t, int64_t n, int64_t steps) {
+  const int64_t sizes[2] = {n, steps};
+  real(t, at::IntArrayRef(sizes, t.dim() == 1 ? 1 : 2), "advantages");
+}
+// What an operator of this file wrote for its backward call.
+void kept(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const char* name) {
+  shaped(t, sizes, name);
+  TORCH_CHECK(t.scalar_type() == type && t.is_contiguous(), name, ": expected contiguous ", type);
+}
+
 struct MaskArg {
   OptT t;
   int kind = RLS_MASK_NONE;
@@ -113,6 +144,7 @@ Tensor tokens_arg(const Tensor& t) {
 // vocabulary cut from a padded one): if the logits start on a 16-byte boundary too, every
 // row then has the alignment of its logits, which the kernels need for 16-byte stores.
 Tensor op_grad_buffer(const Tensor& logits) {
+  TORCH_CHECK(logits.dim() == 3, "logits: expected shape [num_envs, seq_len, vocab], got ", logits.sizes());
   const int64_t n = logits.size(0), t = logits.size(1), v = logits.size(2);
   const int64_t es = logits.stride(0), ss = logits.stride(1);
   if (logits.numel() == 0 || (v > 1 && logits.stride(2) != 1)) return at::empty(logits.sizes(), logits.options());
@@ -143,7 +175,29 @@ struct LogitsArgs {
   MaskArg mask;
   int64_t n, t, v;
   LogitsArgs(const Tensor& logits, const Tensor& tok, const OptT& m)
-      : x(logits_arg(logits)), tokens(tokens_arg(tok)), mask(mask_arg(m)), n(x.size(0)), t(x.size(1)), v(x.size(2)) {}
+      : x(logits_arg(checked(logits, tok, m))), tokens(tokens_arg(tok)), mask(mask_arg(m)), n(x.size(0)), t(x.size(1)),
+        v(x.size(2)) {}
+  static const Tensor& checked(const Tensor& logits, const Tensor& tok, const OptT& m) {
+    TORCH_CHECK(logits.dim() == 3, "logits: expected shape [num_envs, seq_len, vocab], got ", logits.sizes());
+    TORCH_CHECK(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16,
+                "logits: expected float32 or bfloat16, got ", logits.scalar_type());
+    const at::IntArrayRef steps = logits.sizes().slice(0, 2);
+    shaped(tok, steps, "tokens");
+    TORCH_CHECK(c10::isIntegralType(tok.scalar_type(), /*includeBool=*/false), "tokens: expected integers, got ",
+                tok.scalar_type());
+    masks(m, steps, "mask");
+    return logits;
+  }
+  // What the forward call kept of the rows, and a buffer for their gradient.
+  void check_kept(const Tensor& order, const Tensor& stats) const {
+    if (order.numel()) kept(order, {n * t + 1}, at::kInt, "order");
+    if (v > RLS_SHORT_VOCAB || stats.numel()) kept(stats, {n, t, RLS_ROW_STATS}, at::kFloat, "row_stats");
+  }
+  void check_grad(const Tensor& g) const {
+    shaped(g, x.sizes(), "grad");
+    TORCH_CHECK(g.scalar_type() == x.scalar_type(), "grad: expected ", x.scalar_type(), ", got ", g.scalar_type());
+    TORCH_CHECK(v <= 1 || g.numel() == 0 || g.stride(2) == 1, "grad: the vocabulary must be contiguous");
+  }
   // Long rows with a mask go by an order of the rows, made once for both directions.
   Tensor order_buffer() const {
     const bool some = mask.t && v > RLS_SHORT_VOCAB && n * t <= 0x7ffffffe;
@@ -189,6 +243,9 @@ Tensor op_logprobs_backward(const Tensor& logits, const Tensor& tokens, const Op
                             const OptT& g_lp, const OptT& g_ent, double temperature) {
   const Placed placed(logits, tokens, mask, order, stats, g_lp, g_ent);
   const LogitsArgs a(logits, tokens, mask);
+  a.check_kept(order, stats);
+  real(g_lp, {a.n, a.t}, "g_logprobs");
+  real(g_ent, {a.n, a.t}, "g_entropy");
   const OptT gl = f32(g_lp), ge = f32(g_ent);
   Tensor g = op_grad_buffer(a.x);
   check(rls_token_logprobs_backward(a.x.data_ptr(), a.x.stride(0), a.x.stride(1), a.tokens.data_ptr<int64_t>(),
@@ -216,6 +273,21 @@ Tensor norm_for(const MaskArg& m, const Tensor& ref, int64_t n, int64_t reductio
   return m.t && reduction != RLS_REDUCE_SUM ? like(ref, {n + 1}) : none(ref, kNorm);
 }
 
+// A policy loss's inputs besides the log-probabilities or logits of [n, t] steps.
+void policy_inputs_ok(const Tensor& old_lp, const Tensor& adv, const OptT& ref, int64_t n, int64_t t) {
+  real(old_lp, {n, t}, "old_logprobs");
+  advantages_ok(adv, n, t);
+  real(ref, {n, t}, "ref_logprobs");
+}
+void norm_ok(const Tensor& norm, const MaskArg& m, int64_t n, int64_t reduction) {
+  if (m.t && reduction != RLS_REDUCE_SUM) kept(norm, {n + 1}, at::kFloat, "norm");
+}
+void logprobs_ok(const Tensor& lp, const OptT& mask) {
+  TORCH_CHECK(lp.dim() == 2, "logprobs: expected shape [num_envs, seq_len], got ", lp.sizes());
+  real(lp, lp.sizes(), "logprobs");
+  masks(mask, lp.sizes(), "mask");
+}
+
 Tensor policy_workspace(const Tensor& t) { return workspace_for(t.device(), stream_of(t), 1 << 20); }
 
 // (loss, statistics [5], norm, gradient or an empty tensor)
@@ -225,6 +297,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> op_policy(const Tensor& logprobs, con
                                                      double kl_coef, int64_t kl, int64_t reduction, double grad_scale,
                                                      bool need_stats, bool need_grad) {
   const Placed placed(logprobs, old_logprobs, advantages, mask, ref);
+  logprobs_ok(logprobs, mask);
+  policy_inputs_ok(old_logprobs, advantages, ref, logprobs.size(0), logprobs.size(1));
   const Tensor lp = f32(logprobs), old_lp = f32(old_logprobs), adv = f32(advantages);
   const OptT rf = f32(ref);
   const MaskArg m = mask_arg(mask);
@@ -245,9 +319,14 @@ void op_policy_backward_(Tensor& grad, const Tensor& logprobs, const Tensor& old
                          double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t kl,
                          int64_t reduction, double grad_scale, bool force) {
   const Placed placed(grad, logprobs, old_logprobs, advantages, mask, ref, norm, grad_loss);
+  logprobs_ok(logprobs, mask);
+  policy_inputs_ok(old_logprobs, advantages, ref, logprobs.size(0), logprobs.size(1));
+  kept(grad, logprobs.sizes(), at::kFloat, "grad");
+  scalar(grad_loss, "grad_loss");
   const Tensor lp = f32(logprobs), old_lp = f32(old_logprobs), adv = f32(advantages), g = f32(grad_loss);
   const OptT rf = f32(ref);
   const MaskArg m = mask_arg(mask);
+  norm_ok(norm, m, lp.size(0), reduction);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, 0.0, reduction);
   check(rls_policy_loss_backward(F(lp), F(old_lp), F(adv), adv.dim() == 1, F(rf), m.ptr(), m.kind, &p,
                                  (float)grad_scale, F(g), force, W(norm), W(grad), lp.size(0), lp.size(1),
@@ -262,6 +341,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> op_po
     double entropy_coef, bool need_stats, double temperature, int64_t reduction, double grad_scale, bool need_grad) {
   const Placed placed(logits, tokens, old_logprobs, advantages, mask, ref);
   const LogitsArgs a(logits, tokens, mask);
+  policy_inputs_ok(old_logprobs, advantages, ref, a.n, a.t);
   const Tensor old_lp = f32(old_logprobs), adv = f32(advantages);
   const OptT rf = f32(ref);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
@@ -287,6 +367,11 @@ void op_policy_logits_backward_(Tensor& grad, const Tensor& logits, const Tensor
                                 double temperature, int64_t reduction, double grad_scale, bool force) {
   const Placed placed(grad, logits, tokens, old_logprobs, advantages, mask, ref, norm, order, rows, grad_loss);
   const LogitsArgs a(logits, tokens, mask);
+  policy_inputs_ok(old_logprobs, advantages, ref, a.n, a.t);
+  norm_ok(norm, a.mask, a.n, reduction);
+  a.check_kept(order, rows);
+  a.check_grad(grad);
+  scalar(grad_loss, "grad_loss");
   const Tensor old_lp = f32(old_logprobs), adv = f32(advantages), up = f32(grad_loss);
   const OptT rf = f32(ref);
   const rls_policy_t p = policy_of(clip_low, clip_high, dual_clip, kl_coef, kl, entropy_coef, reduction);
@@ -312,6 +397,7 @@ struct Pairs {
   bool ref_pair = false;
   Pairs(const Tensor& chosen, const OptT& rejected, const OptT& ref_c, const OptT& ref_r, const OptT& mask_c,
         const OptT& mask_r) {
+    check_sizes(chosen, rejected, ref_c, ref_r, mask_c, mask_r);
     lp[0] = f32(chosen);
     rf[0] = f32(ref_c);
     m[0] = mask_arg(mask_c);
@@ -348,6 +434,24 @@ struct Pairs {
     const int64_t esz = m[0].t ? m[0].t->element_size() : 0;
     mask[1] = m[0].t ? static_cast<const char*>(mask[0]) + at * esz : nullptr;
   }
+  static void check_sizes(const Tensor& chosen, const OptT& rejected, const OptT& ref_c, const OptT& ref_r,
+                          const OptT& mask_c, const OptT& mask_r) {
+    TORCH_CHECK(chosen.dim() == 2, "chosen: expected shape [pairs, len], got ", chosen.sizes());
+    TORCH_CHECK(rejected || (!ref_r && !mask_r), "rejected: its reference and mask go with it");
+    TORCH_CHECK(rejected || chosen.size(0) % 2 == 0, "chosen: expected shape [2 * pairs, len], got ", chosen.sizes());
+    TORCH_CHECK(!rejected || (rejected->dim() == 2 && rejected->size(0) == chosen.size(0)),
+                "rejected: expected as many responses as chosen");
+    TORCH_CHECK(!rejected || ((bool)ref_c == (bool)ref_r && (!ref_c || ref_c->dim() == ref_r->dim())),
+                "ref_rejected: expected alike with ref_chosen");
+    one(chosen, ref_c, mask_c, "chosen", "ref_chosen", "chosen_mask");
+    if (rejected) one(*rejected, ref_r, mask_r, "rejected", "ref_rejected", "rejected_mask");
+  }
+  static void one(const Tensor& lp, const OptT& ref, const OptT& mask, const char* name, const char* ref_name,
+                  const char* mask_name) {
+    real(lp, lp.sizes(), name);
+    if (ref) real(ref, ref->dim() == 1 ? lp.sizes().slice(0, 1) : lp.sizes(), ref_name);
+    masks(mask, lp.sizes(), mask_name);
+  }
 };
 
 // (loss, rewards of the chosen, of the rejected, coefficients [2, pairs])
@@ -374,8 +478,13 @@ std::tuple<Tensor, Tensor> op_preference_backward(const Tensor& coef, const Tens
                                                   const OptT& chosen_mask, const OptT& rejected_mask,
                                                   int64_t chosen_len, int64_t rejected_len, bool halves) {
   const Placed placed(coef, grad_loss, chosen_mask, rejected_mask);
-  const Tensor g = f32(grad_loss);
+  TORCH_CHECK(coef.dim() == 2 && chosen_len >= 0 && rejected_len >= 0, "coef: expected shape [2, pairs], and lengths");
   const int64_t b = coef.size(1);
+  kept(coef, {2, b}, at::kFloat, "coef");
+  scalar(grad_loss, "grad_loss");
+  masks(chosen_mask, {halves ? 2 * b : b, chosen_len}, "chosen_mask");
+  masks(rejected_mask, {b, rejected_len}, "rejected_mask");
+  const Tensor g = f32(grad_loss);
   MaskArg m[2] = {mask_arg(chosen_mask), mask_arg(rejected_mask)};
   if (m[0].t && m[1].t && m[0].kind != m[1].kind)
     for (auto& x : m) x = mask_arg(x.t->ne(0));

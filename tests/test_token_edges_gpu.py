@@ -177,3 +177,98 @@ def test_gradients_with_create_graph():
         assert torch.equal(got, want) and got.requires_grad and not want.requires_grad
         with pytest.raises(RuntimeError, match="not implemented"):
             (value + got.square().sum()).backward()
+
+
+def test_operators_check_their_tensors():
+    """Called without the functions in front: sizes and types that the kernels
+    would read or write past are refused before anything is launched."""
+    _cuda()
+    ops = torch.ops.rl_triton
+    C = dict(device="cuda")
+    x, tok, lp = torch.zeros(4, 3, 5, **C), torch.zeros(4, 3, dtype=torch.long, **C), torch.zeros(4, 3, **C)
+    long = torch.zeros(4, 3, 2000, **C)
+    small, row, one = lp[:2], lp[:, 0], torch.ones((), **C)
+    none = torch.empty(0, **C)
+    order, norm = torch.empty(0, dtype=torch.int32, **C), torch.zeros(5, **C)
+
+    def refuses(match, op, *args):
+        with pytest.raises(RuntimeError, match=match):
+            op(*args)
+
+    # logits
+    for f in (lambda *a: ops.token_logprobs(*a, 1.0, False), lambda *a: ops._token_logprobs(*a, 1.0, True, True),
+              lambda z, t, m: ops.policy_loss_logits(z, t, lp, lp, m, None, 0.2, 0.2, 0.0, 0.0, 3, 0.0, False, 1.0, 0,
+                                                     1.0),
+              lambda z, t, m: ops._token_logprobs_backward(z, t, m, order, none, lp, None, 1.0)):
+        for grad in (False, True):
+            z = x.clone().requires_grad_(grad)
+            refuses("float32 or bfloat16", f, x.half().requires_grad_(grad), tok, None)
+            refuses("float32 or bfloat16", f, x.double().requires_grad_(grad), tok, None)
+            refuses("tokens: expected shape", f, z, tok[:2], None)
+            refuses("tokens: expected integers", f, z, lp, None)
+            refuses("mask: expected shape", f, z, tok, small)
+            refuses("mask: expected bool", f, z, tok, lp.to(torch.complex64))
+            refuses("num_envs, seq_len, vocab", f, x[0].clone().requires_grad_(grad), tok[0], None)
+    refuses("num_envs, seq_len, vocab", ops._grad_buffer, lp)
+    back = ops._token_logprobs_backward
+    refuses("row_stats", back, long, tok, None, order, none, lp, None, 1.0)
+    refuses("row_stats", back, long, tok, None, order, torch.zeros(4, 3, 7, **C), lp, None, 1.0)
+    refuses("row_stats", back, long, tok, None, order, torch.zeros(4, 3, 8, dtype=torch.float64, **C), lp, None, 1.0)
+    refuses("order: expected shape", back, x, tok, lp, torch.zeros(12, dtype=torch.int32, **C), none, lp, None, 1.0)
+    refuses("g_logprobs", back, x, tok, None, order, none, small, None, 1.0)
+    refuses("g_entropy", back, x, tok, None, order, none, lp, row, 1.0)
+
+    # policy losses
+    tail = (0.2, 0.2, 0.0, 0.0, 3, 0)
+    for f in (lambda o, a, m, r: ops.policy_loss(lp, o, a, m, r, *tail, 1.0, False),
+              lambda o, a, m, r: ops.policy_loss(lp.clone().requires_grad_(True), o, a, m, r, *tail, 1.0, False),
+              lambda o, a, m, r: ops.policy_loss_logits(x, tok, o, a, m, r, *tail[:5], 0.0, False, 1.0, 0, 1.0),
+              lambda o, a, m, r: ops._policy_loss_backward_(lp.clone(), lp, o, a, m, r, norm, one, *tail, 1.0, True),
+              lambda o, a, m, r: ops._policy_loss_logits_backward_(x.clone(), x, tok, o, a, m, r, norm, order, none, one,
+                                                                   *tail[:5], 0.0, 1.0, 0, 1.0, True)):
+        refuses("old_logprobs: expected shape", f, small, lp, None, None)
+        refuses("old_logprobs: expected floating", f, tok, lp, None, None)
+        refuses("advantages: expected shape", f, lp, small, None, None)
+        refuses("advantages: expected shape", f, lp, row[:2], None, None)
+        refuses("advantages: expected shape", f, lp, one, None, None)
+        refuses("ref_logprobs: expected shape", f, lp, row, None, row)
+        refuses("mask: expected shape", f, lp, row, row, None)
+    refuses("logprobs: expected shape", ops.policy_loss, row, row, row, None, None, *tail, 1.0, False)
+    loss_back = ops._policy_loss_backward_
+    refuses("grad: expected", loss_back, small, lp, lp, lp, None, None, norm, one, *tail, 1.0, True)
+    refuses("grad: expected", loss_back, lp.bfloat16(), lp, lp, lp, None, None, norm, one, *tail, 1.0, True)
+    refuses("grad_loss", loss_back, lp, lp, lp, lp, None, None, norm, lp, *tail, 1.0, True)
+    refuses("norm: expected shape", loss_back, lp, lp, lp, lp, lp, None, norm[:4], one, *tail, 1.0, True)
+    back = lambda g, nrm, up=one: ops._policy_loss_logits_backward_(  # noqa: E731
+        g, x, tok, lp, lp, lp, None, nrm, order, none, up, *tail[:5], 0.0, 1.0, 0, 1.0, True)
+    refuses("grad: expected shape", back, x[:2], norm)
+    refuses("grad: expected", back, x.bfloat16(), norm)
+    refuses("contiguous", back, torch.zeros(4, 5, 3, **C).transpose(1, 2), norm)
+    refuses("norm: expected shape", back, x.clone(), none)
+    refuses("grad_loss", back, x.clone(), norm, lp)
+
+    # preference loss
+    for grad in (False, True):
+        z = lp.clone().requires_grad_(grad)
+        f = lambda *a: ops.preference_loss(*a, 0.1, 0.0, 0, False)  # noqa: E731
+        refuses("2 \\* pairs", f, z[:3], None, None, None, None, None)
+        refuses("chosen: expected shape", f, z[0], None, None, None, None, None)
+        refuses("go with it", f, z, None, None, lp, None, None)
+        refuses("as many responses", f, z, z[:2], None, None, None, None)
+        refuses("alike", f, z, z, lp, None, None, None)
+        refuses("alike", f, z, z, lp, row, None, None)
+        refuses("ref_chosen: expected shape", f, z, None, small, None, None, None)
+        refuses("ref_chosen: expected shape", f, z, None, row[:2], None, None, None)
+        refuses("chosen_mask: expected shape", f, z, None, None, None, small, None)
+        refuses("ref_rejected: expected shape", f, z, z, row, row[:3], None, None)
+        refuses("rejected_mask: expected shape", f, z, z, None, None, None, row)
+    f = ops._preference_loss_backward
+    coef = torch.ones(2, 2, **C)
+    refuses("coef: expected shape", f, torch.ones(3, 2, **C), one, None, None, 3, 3, False)
+    refuses("coef: expected", f, coef.double(), one, None, None, 3, 3, False)
+    refuses("coef: expected", f, coef, one, None, None, -1, 3, False)
+    refuses("grad_loss", f, coef, coef, None, None, 3, 3, False)
+    refuses("chosen_mask: expected shape", f, coef, one, lp, None, 3, 3, False)
+    refuses("chosen_mask: expected shape", f, coef, one, small, None, 3, 0, True)
+    refuses("rejected_mask: expected shape", f, coef, one, None, lp, 3, 3, False)
+    torch.cuda.synchronize()
