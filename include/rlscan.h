@@ -100,6 +100,11 @@ const char* rls_status_string(int status);
  * small call's host time).  Returns the value before (-1: none).  An array that
  * is elsewhere then faults the GPU instead of returning RLS_ENOTDEVICE.      */
 int rls_assume_device(int device);
+/* Tries of a device wait in the calling thread's calls of rls_policy_loss_logits
+ * (long rows: the CTAs of a row wait for one another's sums); -1: the default.  A wait
+ * that runs out latches bit 8 of rls_workspace_error, and the results that lack those
+ * sums are NaN (0 tries: every one).  Returns the value before.               */
+int rls_wait_tries(int tries);
 const char* rls_build_info(void);
 
 /* ---- the seven estimators ---------------------------------------------- */

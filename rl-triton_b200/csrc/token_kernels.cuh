@@ -671,6 +671,7 @@ struct PolicyGrad {
   bool force;
   SumOut sums;
   unsigned* error;  // the workspace's error word
+  unsigned tries;   // of a wait on the team
   // the gradient at hand was made for that very scale
   __device__ __forceinline__ bool skip() const { return g && !force && *g == scale; }
   __device__ __forceinline__ float up() const { return g ? *g : scale; }
@@ -1006,13 +1007,16 @@ __device__ __forceinline__ void store_async(float4* p, unsigned long long* bar, 
                "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(its) : "memory");
 }
 
-constexpr unsigned kTeamWait = 1u << 16;  // tries of a wait on the team, each suspended for a while
-
 // What a thread keeps of its exchanges.
 struct Turns {
   unsigned n = 0;
   unsigned* error;      // where a wait that ran out is noted
-  bool broken = false;  // one did: no wait any more (the results are not valid)
+  unsigned tries;       // of a wait, each suspended for a while
+  // A wait of this warp ran out (from the row's next barrier on: of the CTA).  Nothing is sent,
+  // expected or awaited any more -- a barrier whose phase did not end takes no other
+  // arrival -- and the rows' results are NaN.  The others of the team miss this one's
+  // values and run out in their turn.
+  bool broken = false;
 };
 
 template <int NT, bool CL, bool ASYNC>
@@ -1023,23 +1027,18 @@ __device__ __forceinline__ const float4* exchange(Table<NT, CL, ASYNC>& t, Turns
   ++turn.n;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if constexpr (CL && ASYNC) {
+    if (turn.broken) return tab;
     // Each warp of the team sends size x 16 bytes; this CTA's barrier gets 16 from each.
     // A barrier is used again two exchanges on: whoever sends then has had this CTA's
     // values of the exchange between, which its warps send after this wait.
     unsigned long long* bar = &t.bar[which];
     if (threadIdx.x == 0) bar_expect(bar, size * (NT / 32) * 16);
     if (lane < size) store_async(tab + rank * (NT / 32) + warp, bar, lane, mine);
-    if (!turn.broken) {
-      unsigned tries = 0;
-      while (!bar_try(bar, parity))
-        if (++tries == kTeamWait) {
-          turn.broken = true;
-          if (turn.error) atomicOr(turn.error, 8u);
-          break;
-        }
-      bar_acquire(bar, parity);
-    }
-    turn.broken = __any_sync(0xffffffffu, turn.broken);
+    bool done = false;
+    for (unsigned k = 0; k < turn.tries && !done; ++k) done = bar_try(bar, parity);
+    if (done) bar_acquire(bar, parity);
+    turn.broken = __any_sync(0xffffffffu, !done);
+    if (turn.broken && lane == 0) atomicOr(turn.error, 8u);
   } else if constexpr (CL) {
     if (lane < size) store_remote(tab + rank * (NT / 32) + warp, lane, mine);
     cluster_barrier();
@@ -1075,6 +1074,9 @@ __device__ __forceinline__ void gather(float& m, float& s0, float& s1, float c) 
 
 __device__ __forceinline__ float incoming_entropy(const PolicyGrad& s, float w, float) { return -w * s.p.ent_coef; }
 __device__ __forceinline__ float incoming_entropy(const GivenGrad&, float, float b) { return b; }
+
+// A row's statistics where the team's were not to be had.
+__device__ __forceinline__ RowStats no_stats() { return RowStats{NAN, NAN, NAN, true, false, -1.f, 0.f}; }
 
 // The rows of a team, in order, and what its CTA and threads have of each.
 template <class T, bool ENT, int MODE, class Src, int NT, bool CL>
@@ -1255,6 +1257,7 @@ struct Walk {
     gather<32>(run.m, run.s0, run.s1, c);
     {
       const float4* tab = exchange(table, turn, make_float4(run.m, run.s0, run.s1, 0.f), rank, size);
+      if (turn.broken) return no_stats();
       // every group of lanes reads all of the table
       constexpr int kWarps = NT / 32;
       if constexpr (!CL) {
@@ -1299,6 +1302,7 @@ struct Walk {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float4* tab = exchange(table, turn, make_float4(m, 0.f, 0.f, 0.f), rank, size);
+    if (turn.broken) return no_stats();
     for (int w = 0; w < (int)size * (NT / 32); ++w) m = fmaxf(m, tab[w].x);
     float s0 = 0.f, s1 = 0.f;
     auto add = [&](float y) {
@@ -1315,6 +1319,7 @@ struct Walk {
       s1 += __shfl_xor_sync(0xffffffffu, s1, o);
     }
     tab = exchange(table, turn, make_float4(s0, s1, 0.f, 0.f), rank, size);
+    if (turn.broken) return no_stats();
     s0 = s1 = 0.f;
     for (int w = 0; w < (int)size * (NT / 32); ++w) { s0 += tab[w].x; s1 += tab[w].y; }
     return RowStats{m, s0, s1 / s0, true, s0 == 1.f && s1 == 0.f, -1.f, 0.f};
@@ -1446,7 +1451,7 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
   constexpr int M = 2;  // vectors taken at a time
   static_assert(MODE != kBoth && U % M == 0, "streams");
   __shared__ Table<NT, CL, false> table;
-  Turns turn{0, nullptr, false};
+  Turns turn{0, nullptr, 0, false};
   using W = Walk<T, ENT, MODE, Src, NT, CL>;
   W walk(in, out, gr, src);
   const unsigned low = Vec<T>::kLowest;
@@ -1551,7 +1556,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
   extern __shared__ uint4 slots[];  // [K][NT]
   __shared__ Table<NT, CL, true> table;
   __shared__ float4 incoming;       // (a, b, S0, t) of the row, from the warp that formed them
-  Turns turn{0, src.error, false};
+  Turns turn{0, src.error, src.tries, false};
   using W = Walk<T, ENT, kBoth, Src, NT, CL>;
   W walk(in, out, gr, src);
   uint4* mine = slots + threadIdx.x;
@@ -1590,7 +1595,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
       }
       run.template add_vectors<T, M, NT>(u, in.c, token_v - j * NT, token_e);
     }
-    const RowStats r = walk.join(run, now.row, ex, table, turn);
+    RowStats r = walk.join(run, now.row, ex, table, turn);
     typename W::Result q;
     float own = 0.f;
     if (threadIdx.x < 32) {
@@ -1607,9 +1612,17 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
       next = walk.place(row);
       nx = walk.extra(row);
     }
-    __syncthreads();
+    if constexpr (CL) {
+      turn.broken = __syncthreads_or(turn.broken);
+      if (turn.broken) {
+        r = no_stats();
+        q.lp = q.o.loss = own = NAN;
+      }
+    } else {
+      __syncthreads();
+    }
     if (threadIdx.x < 32) walk.outputs(now.row, r, ex, q, own);
-    const typename W::Writer wr = walk.writer(now.row, r, incoming.x, incoming.y);
+    const typename W::Writer wr = walk.writer(now.row, r, turn.broken ? NAN : incoming.x, incoming.y);
     if (wr.g && !wr.sh.far) {
 #pragma unroll
       for (int j = 0; j < K; ++j) {
@@ -1627,8 +1640,13 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
     now = next;
     ex = nx;
   }
-  // No CTA leaves while another might still store to it (after a wait that ran out).
-  if constexpr (CL) cluster_barrier();
+  // No CTA leaves while another might still store to it.  Where every wait succeeded all that was
+  // sent here has come; after one that ran out the rest, all sent by now, is on its way.
+  if constexpr (CL) {
+    cluster_barrier();
+    if (turn.broken)
+      for (int k = 0; k < 64; ++k) __nanosleep(1000);
+  }
 }
 
 // ---- short rows in tiles ---------------------------------------------------------

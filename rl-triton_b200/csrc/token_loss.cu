@@ -15,6 +15,10 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Tries of a wait of a row's CTAs on one another, each suspended for a while by the hardware.
+constexpr unsigned kTeamWait = 1u << 16;
+thread_local int g_wait_tries = -1;  // rls_wait_tries
+
 // The ticket and the counts lie in words of the workspace header that the
 // estimators do not use; every launch leaves them zero.
 unsigned* ticket_of(void* ws) { return &static_cast<WsHeader*>(ws)->pad[4]; }
@@ -444,6 +448,12 @@ int64_t rls::tok::sum_blocks(int64_t need) {
   return need < most ? need : most;
 }
 
+extern "C" int rls_wait_tries(int tries) {
+  const int before = g_wait_tries;
+  g_wait_tries = tries < 0 ? -1 : tries;
+  return before;
+}
+
 extern "C" int rls_row_order(const void* mask, int mask_kind, int64_t num_envs, int64_t seq_len, int32_t* order,
                              void* ws, size_t ws_bytes, void* stream) {
   if (num_envs < 0 || seq_len < 0 || !mask_ok(mask, mask_kind)) return RLS_EINVAL;
@@ -596,7 +606,8 @@ extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, in
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   const Policy p = make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm,
                                mask != nullptr, num_envs, seq_len);
-  PolicyGrad src{p, grad_scale, nullptr, false, SumOut{}, &static_cast<WsHeader*>(ws)->error};
+  PolicyGrad src{p, grad_scale, nullptr, false, SumOut{}, &static_cast<WsHeader*>(ws)->error,
+                 g_wait_tries < 0 ? kTeamWait : (unsigned)g_wait_tries};
   const int64_t blocks = sum_blocks((M + kThreads - 1) / kThreads);
   if (int st = sums_in(ws, ws_bytes, sum_blocks(M), loss, stats, s, &src.sums)) return st;
   if (vocab <= kLaneVocab) order = nullptr;
@@ -635,6 +646,6 @@ extern "C" int rls_policy_loss_logits_backward(const void* logits, int64_t env_s
   const Policy p = make_policy(*policy, old_logprobs, advantages, advantages_per_env, ref_logprobs, norm,
                                mask != nullptr, num_envs, seq_len);
   const RowOut ro{nullptr, nullptr, reinterpret_cast<float4*>(const_cast<float*>(row_stats))};
-  return launch_logits<kBwd>(c, policy->entropy_coef != 0.f, ro, PolicyGrad{p, grad_scale, grad_loss, force != 0, SumOut{}, nullptr},
+  return launch_logits<kBwd>(c, policy->entropy_coef != 0.f, ro, PolicyGrad{p, grad_scale, grad_loss, force != 0, SumOut{}, nullptr, 0},
                              reinterpret_cast<cudaStream_t>(stream));
 }

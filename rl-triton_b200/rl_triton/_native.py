@@ -245,6 +245,7 @@ _SIGS = {
     "rls_workspace_error": (_I, [_P, _P]),
     "rls_status_string": (ctypes.c_char_p, [_I]),
     "rls_assume_device": (_I, [_I]),
+    "rls_wait_tries": (_I, [_I]),
     "rls_build_info": (ctypes.c_char_p, []),
     "rls_gae": (_I, [_P, _P, _P, _P, _P, _I, _P, _I64, _I64, _F, _F, _I, _SEG, _P, _SZ, _P]),
     "rls_vtrace": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I64, _I64, _F, _F, _F, _I, _P, _SZ, _P]),

@@ -91,3 +91,14 @@ def test_the_losses_other_inputs_are_constants():
     assert got[0] is not None and got[1:] == (None, None, None)
     loss = nat.ops.preference_loss(lp, None, refl, None, None, None, 0.1, 0.0, 0, False)[0]
     assert torch.autograd.grad(loss, (lp, refl), allow_unused=True)[1] is None
+
+
+def test_wait_tries_are_the_threads_own():
+    import threading
+    assert nat.lib.rls_wait_tries(5) == -1
+    seen = []
+    th = threading.Thread(target=lambda: seen.append(nat.lib.rls_wait_tries(-1)))
+    th.start()
+    th.join()
+    assert seen == [-1]
+    assert nat.lib.rls_wait_tries(-7) == 5 and nat.lib.rls_wait_tries(-1) == -1

@@ -272,3 +272,40 @@ def test_operators_check_their_tensors():
     refuses("chosen_mask: expected shape", f, coef, one, small, None, 3, 0, True)
     refuses("rejected_mask: expected shape", f, coef, one, None, lp, 3, 3, False)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("v,dtype,n,t", [(5000, torch.float32, 2, 4), (131072, torch.bfloat16, 2, 4),
+                                         (131072, torch.float32, 3, 40), (60000, torch.bfloat16, 30, 20)])
+def test_a_wait_that_runs_out(v, dtype, n, t, monkeypatch):
+    """Without a try the CTAs of a row do not get one another's sums: the kernel
+    ends, the rows that count are NaN (nothing wrong passes for a result), the
+    workspace says so, and the next call is as ever."""
+    _cuda()
+    import rl_triton
+    from rl_triton import _native as nat
+    monkeypatch.setenv("RL_TRITON_CORRECTNESS_WARNINGS", "0")
+    x, tok, mask, g = make(n, t, v, dtype, seed=1)
+    old, adv = -3 * torch.rand(n, t, generator=g), torch.randn(n, t, generator=g)
+    x, tok, mask, old, adv = (a.cuda() for a in (x, tok, mask, old, adv))
+    x.requires_grad_(True)
+
+    def call():
+        loss, lp = rl_triton.compute_policy_loss_from_logits(x, tok, old, adv, mask)
+        return loss.detach(), lp, torch.autograd.grad(loss, x)[0]
+
+    want = call()
+    assert nat.workspace_error() == 0 and torch.isfinite(want[0])
+    assert nat.lib.rls_wait_tries(0) == -1
+    try:
+        loss, lp, grad = call()
+        torch.cuda.synchronize()
+        assert nat.workspace_error() == 8 and nat.workspace_error() == 0
+        assert torch.isnan(loss) and torch.isnan(lp[mask]).all() and torch.isnan(grad[mask]).all()
+        assert (lp[~mask] == 0).all() and (grad[~mask] == 0).all()
+        monkeypatch.setenv("RL_TRITON_CORRECTNESS_WARNINGS", "1")
+        with pytest.raises(RuntimeError, match="wait ran out"):
+            call()
+    finally:
+        assert nat.lib.rls_wait_tries(-1) == 0
+    for a, b in zip(call(), want):
+        assert torch.equal(a, b)
