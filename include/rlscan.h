@@ -95,10 +95,11 @@ size_t rls_workspace_bytes(int64_t num_elements);
 int rls_workspace_error(void* ws, void* stream);
 const char* rls_status_string(int status);
 /* For callers that know where their arrays are: until it is called again with
- * -1, the calling thread's calls take every array to be memory of GPU `device`
- * and leave out the placement queries (one driver query an array, a third of a
- * small call's host time).  Returns the value before (-1: none).  An array that
- * is elsewhere then faults the GPU instead of returning RLS_ENOTDEVICE.      */
+ * -1, the calling thread's calls of the token-level operators (below) take every
+ * array to be memory of GPU `device` and leave out the placement queries (one
+ * driver query an array, a third of a small call's host time).  Returns the value
+ * before (-1: none).  An array of such a call that is elsewhere then faults the GPU instead
+ * of returning RLS_ENOTDEVICE; all other entry points look as ever.          */
 int rls_assume_device(int device);
 /* Tries of a device wait in the calling thread's calls of rls_policy_loss_logits
  * (long rows: the CTAs of a row wait for one another's sums); -1: the default.  A wait

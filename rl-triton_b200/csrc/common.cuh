@@ -205,17 +205,13 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 // restoring the caller's device afterwards.  A host pointer handed to a kernel
 // would fault the GPU; here it returns a status instead.
 //
-// A caller that knows where its arrays are (the operator library looks at each
-// tensor's device) may say so for its thread through rls_assume_device: the
-// queries, a third of a small call's host time, are left out then.
-int assumed_device();  // -1: none
-
+// A caller that knows where its arrays are may name the GPU: the queries, a third of a
+// small call's host time, are left out then.
 class DeviceGuard {
  public:
   // status(): 0 = ok; otherwise RLS_ENOTDEVICE (7) from rlscan.h.
-  DeviceGuard(std::initializer_list<const void*> ptrs) {
-    int dev = assumed_device();
-    if (dev < 0) dev = device_of(ptrs);
+  DeviceGuard(std::initializer_list<const void*> ptrs, int known = -1) {
+    const int dev = known < 0 ? device_of(ptrs) : known;
     if (status_ || dev < 0) return;
     if (cudaGetDevice(&prev_) != cudaSuccess) { cudaGetLastError(); prev_ = -1; }
     if (prev_ != dev) {

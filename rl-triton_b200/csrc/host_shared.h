@@ -8,6 +8,7 @@
 #include <mutex>
 #include <utility>
 
+#include "common.cuh"
 #include "rlscan.h"
 
 namespace rls {
@@ -20,6 +21,14 @@ std::recursive_mutex& launch_mutex();
 // workspace last used by another clears the records (rlscan.cu).
 enum : int { kLayoutNone = 0, kLayoutFlags = 1, kLayoutPacked = 2, kLayoutScratch = 3 };
 int prepare_layout(void* ws, size_t wsb, int layout, cudaStream_t s);
+
+// The GPU that the calling thread's arrays are on by rls_assume_device (-1: not
+// said).  Only the token-level entry points go by it: their operators look at each tensor's device.
+int assumed_device();
+class TokenGuard : public DeviceGuard {
+ public:
+  TokenGuard(std::initializer_list<const void*> ptrs) : DeviceGuard(ptrs, assumed_device()) {}
+};
 
 // Programmatic dependent launch bookkeeping (rlscan.cu): the output ranges of
 // the last early-triggering launch per stream, and whether a new launch's

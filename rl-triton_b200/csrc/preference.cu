@@ -202,7 +202,7 @@ extern "C" int rls_preference_loss(const float* chosen, const float* rejected, c
   if (!std::isfinite(beta) || (kind == RLS_PREFERENCE_IPO && beta == 0.f)) return RLS_EINVAL;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (pairs == 0) {
-    DeviceGuard guard{loss};
+    TokenGuard guard{loss};
     if (guard.status()) return guard.status();
     return cudaMemsetAsync(loss, 0, sizeof(float), s) == cudaSuccess ? RLS_OK : RLS_ECUDA;
   }
@@ -214,7 +214,7 @@ extern "C" int rls_preference_loss(const float* chosen, const float* rejected, c
       !al(chosen_mask, mask_align(mask_kind)) || !al(rejected_mask, mask_align(mask_kind)))
     return RLS_EALIGN;
   if (64 + (size_t)pairs * sizeof(double) > ws_bytes) return RLS_EWORKSPACE;
-  DeviceGuard guard{chosen_len ? chosen : nullptr, rejected_len ? rejected : nullptr, ref_chosen, ref_rejected,
+  TokenGuard guard{chosen_len ? chosen : nullptr, rejected_len ? rejected : nullptr, ref_chosen, ref_rejected,
                     chosen_mask, rejected_mask, loss, chosen_rewards, rejected_rewards, coef, ws};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
@@ -256,7 +256,7 @@ extern "C" int rls_preference_loss_backward(const float* coef, const float* grad
   if (!al(coef, 4) || !al(grad_loss, 4) || !al(grad_chosen, 4) || !al(grad_rejected, 4) ||
       !al(chosen_mask, mask_align(mask_kind)) || !al(rejected_mask, mask_align(mask_kind)))
     return RLS_EALIGN;
-  DeviceGuard guard{coef, grad_loss, chosen_mask, rejected_mask, grad_chosen, grad_rejected};
+  TokenGuard guard{coef, grad_loss, chosen_mask, rejected_mask, grad_chosen, grad_rejected};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   SpreadArgs a{};

@@ -346,7 +346,7 @@ int sums_in(void* ws, size_t wsb, int64_t blocks, float* loss, float* stats, cud
 
 // No steps at all: loss and statistics 0.
 int clear_loss(float* loss, float* stats, cudaStream_t s) {
-  DeviceGuard guard{loss, stats};
+  TokenGuard guard{loss, stats};
   if (guard.status()) return guard.status();
   if (cudaMemsetAsync(loss, 0, sizeof(float), s) != cudaSuccess) return RLS_ECUDA;
   if (stats && cudaMemsetAsync(stats, 0, (kSums - 1) * sizeof(float), s) != cudaSuccess) return RLS_ECUDA;
@@ -461,7 +461,7 @@ extern "C" int rls_row_order(const void* mask, int mask_kind, int64_t num_envs, 
   if (!mask || !order || !ws || num_envs > 0x7ffffffe / seq_len) return RLS_EINVAL;
   if (ws_bytes < sizeof(WsHeader)) return RLS_EWORKSPACE;
   if (!aligned(order, 4) || !aligned(ws) || !aligned(mask, mask_align(mask_kind))) return RLS_EALIGN;
-  DeviceGuard guard{mask, order, ws};
+  TokenGuard guard{mask, order, ws};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   return launch_count(RLS_REDUCE_TOKEN, Mask{mask, mask_kind}, nullptr, order, num_envs, seq_len, ws,
@@ -478,7 +478,7 @@ extern "C" int rls_token_logprobs(const void* logits, int64_t env_stride, int64_
   if (num_envs == 0 || seq_len == 0) return RLS_OK;
   if (!logprobs) return RLS_EINVAL;
   if (!aligned(logprobs) || !aligned(entropy) || !aligned(row_stats)) return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, order, mask, logprobs, entropy, row_stats};
+  TokenGuard guard{logits, tokens, order, mask, logprobs, entropy, row_stats};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   return launch_logits<kFwd>(c, entropy != nullptr, RowOut{logprobs, entropy, reinterpret_cast<float4*>(row_stats)},
@@ -497,7 +497,7 @@ extern "C" int rls_token_logprobs_backward(const void* logits, int64_t env_strid
   if (num_envs == 0 || seq_len == 0) return RLS_OK;
   if ((!row_stats && vocab > kLaneVocab) || !grad_logits) return RLS_EINVAL;
   if (!aligned(row_stats) || !aligned(grad_logprobs, 4) || !aligned(grad_entropy, 4)) return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, order, mask, row_stats, grad_logprobs, grad_entropy, grad_logits};
+  TokenGuard guard{logits, tokens, order, mask, row_stats, grad_logprobs, grad_entropy, grad_logits};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   const RowOut out{nullptr, nullptr, reinterpret_cast<float4*>(const_cast<float*>(row_stats))};
@@ -523,7 +523,7 @@ extern "C" int rls_policy_loss(const float* logprobs, const float* old_logprobs,
       !aligned(grad_logprobs) || !aligned(ws) || !aligned(norm, 4) || !aligned(loss, 4) || !aligned(stats, 4) ||
       !aligned(mask, mask_align(mask_kind)))
     return RLS_EALIGN;
-  DeviceGuard guard{logprobs, old_logprobs, advantages, ref_logprobs, mask, norm, loss, stats, grad_logprobs, ws};
+  TokenGuard guard{logprobs, old_logprobs, advantages, ref_logprobs, mask, norm, loss, stats, grad_logprobs, ws};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   Terms t{logprobs,
@@ -564,7 +564,7 @@ extern "C" int rls_policy_loss_backward(const float* logprobs, const float* old_
   if (!aligned(logprobs) || !aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) ||
       !aligned(grad_logprobs) || !aligned(norm, 4) || !aligned(grad_loss, 4) || !aligned(mask, mask_align(mask_kind)))
     return RLS_EALIGN;
-  DeviceGuard guard{logprobs, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, grad_logprobs};
+  TokenGuard guard{logprobs, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, grad_logprobs};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
   Terms t{logprobs,
@@ -600,7 +600,7 @@ extern "C" int rls_policy_loss_logits(const void* logits, int64_t env_stride, in
   if (!aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) || !aligned(logprobs) ||
       !aligned(entropy) || !aligned(row_stats) || !aligned(ws) || !aligned(norm, 4) || !aligned(loss, 4) || !aligned(stats, 4))
     return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, order, old_logprobs, advantages, ref_logprobs, mask, norm, logprobs, entropy, row_stats,
+  TokenGuard guard{logits, tokens, order, old_logprobs, advantages, ref_logprobs, mask, norm, logprobs, entropy, row_stats,
                     loss, stats, grad_logits, ws};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());
@@ -639,7 +639,7 @@ extern "C" int rls_policy_loss_logits_backward(const void* logits, int64_t env_s
   if (!aligned(old_logprobs) || !aligned(advantages) || !aligned(ref_logprobs) || !aligned(row_stats) ||
       !aligned(norm, 4) || !aligned(grad_loss, 4))
     return RLS_EALIGN;
-  DeviceGuard guard{logits, tokens, order, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, row_stats,
+  TokenGuard guard{logits, tokens, order, old_logprobs, advantages, ref_logprobs, mask, norm, grad_loss, row_stats,
                     grad_logits};
   if (guard.status()) return guard.status();
   std::lock_guard<std::recursive_mutex> lock(launch_mutex());

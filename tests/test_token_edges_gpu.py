@@ -309,3 +309,25 @@ def test_a_wait_that_runs_out(v, dtype, n, t, monkeypatch):
         assert nat.lib.rls_wait_tries(-1) == 0
     for a, b in zip(call(), want):
         assert torch.equal(a, b)
+
+
+def test_an_assumed_device_is_the_token_operators_alone():
+    """The other entry points still look where their arrays are (pinned host
+    memory here, which a kernel could reach)."""
+    _cuda()
+    from rl_triton import _native as nat
+    r, out = torch.ones(2, 8).pin_memory(), torch.zeros(2, 8).pin_memory()
+    ws, wsb = nat.workspace(torch.device("cuda", 0), nat.stream_handle(torch.device("cuda", 0)), 1 << 20)
+
+    def call():
+        return nat.lib.rls_discounted_returns(r.data_ptr(), r.data_ptr(), None, None, 0, out.data_ptr(), 2, 8, 0.99, 0, None,
+                                              ws, wsb, nat.stream_handle(torch.device("cuda", 0)))
+
+    assert call() == nat.RLS_ENOTDEVICE
+    assert nat.lib.rls_assume_device(0) == -1
+    try:
+        assert call() == nat.RLS_ENOTDEVICE
+    finally:
+        assert nat.lib.rls_assume_device(-1) == 0
+    torch.cuda.synchronize()
+    assert (out == 0).all()
