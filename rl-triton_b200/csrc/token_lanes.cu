@@ -49,7 +49,7 @@ int tiles(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr, const Src
   sh.by_vocab = Divide::of(in.V, 0);
   const size_t smem = ((size_t)sh.rows * line + 15) / 16 * 16;  // at most 40 KB
   auto kern = tile_rows_kernel<T, ENT, MODE, Src, ACC>;
-  const int64_t all = (in.rows + sh.rows - 1) / sh.rows, fit = sum_blocks(1 << 30) / 8 * kTileCtas;
+  const int64_t all = (in.rows + sh.rows - 1) / sh.rows, fit = (int64_t)num_sms() * kTileCtas;
   const int64_t blocks = all < fit ? all : fit;
   kern<<<(unsigned)blocks, kTileThreads, smem, s>>>(in, out, gr, src, sh);
   return cudaPeekAtLastError() == cudaSuccess ? RLS_OK : RLS_ECUDA;

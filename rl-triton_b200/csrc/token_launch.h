@@ -7,7 +7,9 @@
 namespace rls {
 namespace tok {
 
-constexpr int64_t kLaneVocab = RLS_SHORT_VOCAB;  // rows up to this many logits stay in a warp's registers
+constexpr int64_t kLaneVocab = RLS_SHORT_VOCAB;  // short rows (token_lanes.cu) have at most so many logits
+
+int num_sms();  // of the current device
 
 // CTAs of the kernels that sum: at most this many, whatever the batch.
 int64_t sum_blocks(int64_t need);

@@ -24,18 +24,6 @@ thread_local int g_wait_tries = -1;  // rls_wait_tries
 unsigned* ticket_of(void* ws) { return &static_cast<WsHeader*>(ws)->pad[4]; }
 static_assert(offsetof(WsHeader, pad) % 8 == 0, "the total is 8-byte aligned");
 
-int num_sms() {
-  static int sms[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (!sms[dev]) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    sms[dev] = n;
-  }
-  return sms[dev];
-}
-
 // ---- the mask once over -------------------------------------------------------------
 // norm (may be null): norm[1 + n] = steps of env n that count; norm[0] = 1 / (all of
 // them), or 1 / (envs that have any) for the mean by sequence.  order (may be null):
@@ -169,8 +157,9 @@ __device__ __forceinline__ void load4(const float* p, int64_t i, int64_t M, floa
 }
 
 // One pass over the steps: the sums of the loss and the statistics (SUMS) and
-// the gradient (GRAD).  17 bytes read and 4 written a step; bound by instruction issue (two
-// exponentials, two two-float differences): 4096 x 2048 steps in 57 us, 3.1 TB/s.  A batch of at most kAlone steps is one CTA's, which then counts
+// the gradient (GRAD).  17 bytes read and 4 written a step; bound by instruction issue (71 % of
+// the slots, 30 % of DRAM's peak: two exponentials, two two-float differences): 4096 x 2048
+// steps in 59 us, 3.0 TB/s.  A batch of at most kAlone steps is one CTA's, which then counts
 // the steps itself first (COUNT; norm is written as count_kernel does): one launch instead of two, where
 // the launches are most of the time.
 constexpr int kAlone = 8192, kAloneThreads = 1024;
@@ -442,6 +431,18 @@ int launch_logits(const LogitsCall& c, bool ent, const RowOut& out, const Src& s
 }
 
 }  // namespace
+
+int rls::tok::num_sms() {
+  static int sms[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!sms[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
 
 int64_t rls::tok::sum_blocks(int64_t need) {
   const int64_t most = 8LL * num_sms();

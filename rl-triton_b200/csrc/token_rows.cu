@@ -37,7 +37,7 @@ int launch(void (*kern)(Rows<T>, RowOut, GradRows<T>, Src), const Rows<T>& in, c
       if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) return RLS_ECUDA;
     } else {
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, NT, smem) != cudaSuccess || n < 1) return RLS_ECUDA;
-      n *= (int)(sum_blocks(1 << 30) / 8);
+      n *= num_sms();
     }
     most = n;
   }
@@ -80,7 +80,7 @@ int launch_cta_rows(const Rows<T>& in, const RowOut& out, const GradRows<T>& gr,
   if (MODE == kBoth)
     while (size < kMostCtas && nvec > (int64_t)size * 4096) size *= 2;
   // few rows: more CTAs for each, down to 1024 vectors a CTA
-  while (size < kMostCtas && in.rows * size < 2 * 148 && nvec > (int64_t)size * 1024) size *= 2;
+  while (size < kMostCtas && in.rows * size < 2 * num_sms() && nvec > (int64_t)size * 1024) size *= 2;
   const int64_t each = (nvec + size - 1) / size;
   if constexpr (MODE == kBoth) {
     if (each > 4096) return plain<T, ENT, MODE, Src>(in, out, gr, src, s);
