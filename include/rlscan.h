@@ -91,7 +91,8 @@ typedef struct rls_segment {
 size_t rls_workspace_bytes(int64_t num_elements);
 /* Reads (and clears) the device error latch of a workspace; synchronises
  * `stream`.  Returns 0 when no bounded wait ran out, else a bit mask
- * (1 = tile look-back wait, 2 = bulk-copy wait).                          */
+ * (1 = tile look-back wait, 2 = bulk-copy wait, 4 = grid barrier, 8 = cluster
+ * exchange).                                                               */
 int rls_workspace_error(void* ws, void* stream);
 const char* rls_status_string(int status);
 /* For callers that know where their arrays are: until it is called again with

@@ -50,7 +50,7 @@ struct WsHeader {
   unsigned ticket;    // dynamic tile ticket (reset by the last CTA)
   unsigned finished;  // CTAs finished in this launch (reset by the last CTA)
   unsigned epoch;     // launch counter, 30 bits
-  unsigned error;     // latched error bits (1: look-back wait, 2: bulk-copy wait)
+  unsigned error;     // latched error bits (1: look-back wait, 2: bulk-copy wait, 4: grid barrier, 8: cluster exchange)
   unsigned pad[12];
 };
 static_assert(sizeof(WsHeader) == 64, "header is 64 bytes");

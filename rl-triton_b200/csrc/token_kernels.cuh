@@ -1546,9 +1546,9 @@ __global__ void __launch_bounds__(NT, (MODE == kFwd ? 768 : 1024) / NT)
 // cp.async (all K in flight at once): no barrier, only the thread's own wait.
 // 64 KB a CTA, three CTAs an SM: while one adds up, another stores and a third waits.
 // 1.07 GB of logits read and written: 131072 bf16 (four CTAs a row) 454 us, 0.73 of the copy
-// bandwidth, 32768 bf16 (one) 425 us, 0.78, 8192 fp32 376 us, 0.88.  Bound by the
-// row's serial steps between its passes and by instruction issue (half of the
-// slots), not by DRAM.
+// bandwidth, 32768 bf16 (one) 425 us, 0.78, 8192 fp32 376 us, 0.88.  Bound by latency,
+// the row's serial steps between its passes (half of the issue slots and 46 % of DRAM's
+// peak are used at 1024 rows of 131072 bf16).
 template <class T, bool ENT, class Src, int NT, int K, bool CL>
 __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, RowOut out, GradRows<T> gr, Src src) {
   constexpr int M = 2;
@@ -1656,7 +1656,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) both_rows_kernel(Rows<T> in, Row
 // log-probability, loss term and coefficients -- the fp64 and the transcendental steps
 // that would cost a whole warp's time with a warp a row -- and the gradient is
 // written over the stretch again, by vectors that need not respect the rows.
-// Bound by instruction issue (two thirds of the slots): 1.07 GB in rows of 18 fp32 take 281 us forward
+// Bound by instruction issue (73 % of the slots, 39 % of DRAM's peak): 1.07 GB in rows of 18 fp32 take 281 us forward
 // (0.59 of the copy bandwidth) and 652 us with the gradient (0.51), where a warp's lanes
 // in groups of 8 took 887 and 2211; rows of 64 bf16 279 us (0.60), of 512 bf16 252 us
 // (0.66), of 200 fp32 201 us (0.83).  More CTAs an SM are faster at any unrolling (5

@@ -1,9 +1,9 @@
 // torch_token_ops.cpp -- the token-level policy operators (namespace rl_triton)
 // with their gradients.
 //
-// Three operators are differentiable: token_logprobs (by the logits),
-// policy_loss (by the log-probabilities) and policy_loss_logits (by the
-// logits); so is preference_loss (by the log-probabilities).  Each has an
+// Four operators are differentiable: token_logprobs and policy_loss_logits (by the
+// logits), policy_loss and preference_loss (by the log-probabilities), once each
+// and in reverse mode.  Each has an
 // autograd function here that calls operators of its own (names with a leading
 // underscore: the kernels proper) through the dispatcher, so that fake tensors
 // and torch.compile see the same calls.  The functions are in C++ because a
